@@ -48,6 +48,10 @@ SIGNATURES = {
     "cacti_b200_swiglu_fwd_bwd": (_int, [_p, _p, _p, _p, _p, _p, _i64, _int, _int, _int, _st]),
     "cacti_b200_softmax_nll_workspace_bytes": (_sz, [_i64]),
     "cacti_b200_softmax_nll_fwd_bwd": (_int, [_p, _p, _p, _p, _p, _int, _p, _f32, _i64, _i64, _int, _int, _p, _p, _sz, _st]),
+    "cacti_b200_logits_topk": (_int, [_p, _p, _p, _p, _i64, _i64, _i64, _f32, _int, _st]),
+    "cacti_b200_distill_topk_workspace_bytes": (_sz, [_i64]),
+    "cacti_b200_distill_topk_fwd_bwd": (_int, [_p, _p, _p, _p, _p, _int, _p, _int, _p, _i64, _f32, _p, _f32, _i64, _i64,
+                                               _int, _int, _p, _p, _sz, _st]),
     "cacti_b200_gather_rows": (_int, [_p, _p, _p, _int, _i64, _i64, _i64, _int, _p, _st]),
     "cacti_b200_scatter_add_rows_workspace_bytes": (_sz, [_i64, _i64]),
     "cacti_b200_scatter_add_rows": (_int, [_p, _p, _p, _int, _i64, _i64, _i64, _int, _int, _p, _sz, _p, _st]),
@@ -60,6 +64,10 @@ SIGNATURES = {
     "cacti_b200_gemm_strided_batched": (_int, [_p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _int, _int,
                                                C.POINTER(_f32), C.POINTER(_f32), _i64, _i64, _i64, _i64, _i64, _i64,
                                                _i64, _i64, _int, _p, _sz, _st]),
+    "cacti_b200_gated_ffn_fwd_workspace_bytes": (_sz, [_i64, _i64, _i64, _int]),
+    "cacti_b200_gated_ffn_fwd": (_int, [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _int, _p, _sz, _st]),
+    "cacti_b200_gated_ffn_bwd_workspace_bytes": (_sz, [_i64, _i64, _i64, _int]),
+    "cacti_b200_gated_ffn_bwd": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _int, _int, _int, _p, _sz, _st]),
     "cacti_b200_block_pad": (_int, [_p, _p, _i64, _i64, _i64, _i64, _i64, _int, _st]),
     "cacti_b200_attention_fwd": (_int, [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _f32, _int, _st]),
     "cacti_b200_attention_bwd": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _f32, _int, _st]),

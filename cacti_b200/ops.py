@@ -9,6 +9,8 @@ C ABI, which follows the reference ops: rms_norm (src/librarium/llama.rs:442-451
 """
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 from . import capi
@@ -205,6 +207,83 @@ def softmax_nll_fwd_bwd(logits, targets, w=None, w_scalar=1.0, want_grad=True, w
     return loss_sum, loss_rows, (dlogits if want_grad else None), status
 
 
+# ---- K5b --------------------------------------------------------------------------------------
+def _same(what, dev, **ts):
+    """Checks of the arguments whose shapes the C ABI cannot see: {name: (tensor or None, shape or None, dtypes or None)};
+    every tensor given is contiguous and on `dev`."""
+    for name, (t, shape, dtypes) in ts.items():
+        if t is None:
+            continue
+        if t.device != dev:
+            raise ValueError(f"{what}: {name} is on {t.device}, expected {dev}")
+        if not t.is_contiguous():
+            raise ValueError(f"{what}: {name} is not contiguous")
+        if shape is not None and tuple(t.shape) != tuple(shape):
+            raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+        if dtypes is not None and t.dtype not in dtypes:
+            raise ValueError(f"{what}: {name} has dtype {t.dtype}, expected one of {[str(d) for d in dtypes]}")
+
+
+def _on(dev):
+    """The launch goes to the tensors' device and to its current stream, whichever device is current."""
+    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _matrix(what, name, t):
+    if not t.is_cuda:
+        raise ValueError("cacti_b200 takes device tensors only (there is no CPU path)")
+    if t.dim() != 2:
+        raise ValueError(f"{what}: {name} has {t.dim()} dimensions, expected 2")
+    return t.shape
+
+
+def logits_topk(logits, k, temperature=1.0, want_lse=True):
+    """(values [rows, k] of logits' dtype, indices int32 [rows, k], lse f32[rows] | None): the k largest logits of each row,
+    largest first and equal values by ascending index, with the log of the row's sum of exp(logits / temperature)."""
+    rows, vocab = _matrix("logits_topk", "logits", logits)
+    dev = logits.device
+    _same("logits_topk", dev, logits=(logits, None, tuple(_DT)))
+    with _on(dev):
+        values = torch.empty(rows, k, dtype=logits.dtype, device=dev)
+        indices = torch.empty(rows, k, dtype=torch.int32, device=dev)
+        lse = torch.empty(rows, dtype=torch.float32, device=dev) if want_lse else None
+        check(lib().cacti_b200_logits_topk(_ptr(values), _ptr(indices), _ptr(lse), _ptr(logits), rows, vocab, k, temperature,
+                                           _dt(logits), _stream()), "logits_topk")
+    return values, indices, lse
+
+
+def distill_topk_fwd_bwd(logits, t_values, t_indices, t_lse=None, temperature=1.0, w=None, w_scalar=1.0, want_grad=True,
+                         want_sum=True, want_rows=True, dlogits=None, beta=0, status=None):
+    """Distillation loss of the student's logits against a teacher's listed logits (the outputs of logits_topk at the same
+    temperature), and its gradient.  t_lse given: the unlisted positions form one bucket with the teacher's remaining mass;
+    None: the teacher's distribution is renormalised over its list.  Index -1 marks an unused slot.
+    Returns (loss_sum f32[1] | None, loss_rows f32[rows] | None, dlogits | None, status u32[1]), as softmax_nll_fwd_bwd."""
+    what = "distill_topk_fwd_bwd"
+    rows, vocab = _matrix(what, "logits", logits)
+    dev = logits.device
+    k = t_values.shape[-1]
+    _same(what, dev, logits=(logits, None, tuple(_DT)), t_values=(t_values, (rows, k), tuple(_DT)),
+          t_indices=(t_indices, (rows, k), tuple(_IDX)), t_lse=(t_lse, (rows,), (torch.float32,)),
+          w=(w, (rows,), (torch.float32,)), dlogits=(dlogits, (rows, vocab), (logits.dtype,)),
+          status=(status, (1,), (torch.int32,)))
+    if beta and want_grad and dlogits is None:
+        raise ValueError(f"{what}: beta = 1 adds to dlogits, which is not given")
+    with _on(dev):
+        loss_sum = torch.empty(1, dtype=torch.float32, device=dev) if want_sum else None
+        loss_rows = torch.empty(rows, dtype=torch.float32, device=dev) if want_rows else None
+        if loss_sum is not None and (rows == 0 or vocab == 0):
+            loss_sum.zero_()
+        if want_grad and dlogits is None:
+            dlogits = torch.empty_like(logits)
+        status = torch.zeros(1, dtype=torch.int32, device=dev) if status is None else status
+        ws = None if want_rows or not want_sum else _ws(lib().cacti_b200_distill_topk_workspace_bytes(rows), dev)
+        check(lib().cacti_b200_distill_topk_fwd_bwd(
+            _ptr(loss_sum), _ptr(loss_rows), _ptr(dlogits) if want_grad else 0, _ptr(logits), _ptr(t_values), _dt(t_values),
+            _ptr(t_indices), _IDX[t_indices.dtype], _ptr(t_lse), k, temperature, _ptr(w), w_scalar, rows, vocab, _dt(logits),
+            beta, _ptr(status), _ptr(ws), ws.numel() if ws is not None else 0, _stream()), what)
+    return loss_sum, loss_rows, (dlogits if want_grad else None), status
+
+
 # ---- K6 ---------------------------------------------------------------------------------------
 def gather_rows(table, tokens, out=None, status=None):
     vocab, cols = table.shape
@@ -316,6 +395,64 @@ def block_gemm(a, b, trans_a=False, trans_b=False, alpha=1.0, beta=0.0, c=None, 
                                                 int(trans_b), al, be, nrow, ncol, sao, sai, sbo, sbi, sco, sci, _dt(a),
                                                 _ptr(workspace), workspace.numel(), _stream()), "block_gemm")
     return c
+
+
+# ---- G3 ---------------------------------------------------------------------------------------
+_HALF = (torch.float16, torch.bfloat16)
+
+
+def _ffn_shapes(what, x, w_gate):
+    tokens, d = _matrix(what, "x", x)
+    f, _ = _matrix(what, "w_gate", w_gate)
+    return tokens, d, f
+
+
+def _ffn_aligned(d, *ts):
+    return int(d % 8 == 0 and all(t.data_ptr() % 16 == 0 for t in ts))
+
+
+def gated_ffn_fwd(x, w_gate, w_up, save=False, h=None, gate=None, up=None, workspace=None):
+    """h = silu(x w_gate^T) * (x w_up^T), x [tokens, d_model], weights [d_ffn, d_model], in one kernel.  save (or gate and up
+    given) also returns the two projections, which gated_ffn_bwd takes.  Returns (h, gate | None, up | None)."""
+    what = "gated_ffn_fwd"
+    tokens, d, f = _ffn_shapes(what, x, w_gate)
+    dev, dt = x.device, (x.dtype,)
+    _same(what, dev, x=(x, None, _HALF), w_gate=(w_gate, (f, d), dt), w_up=(w_up, (f, d), dt), h=(h, (tokens, f), dt),
+          gate=(gate, (tokens, f), dt), up=(up, (tokens, f), dt))
+    with _on(dev):
+        h = torch.empty(tokens, f, dtype=x.dtype, device=dev) if h is None else h
+        if save or gate is not None or up is not None:
+            gate = torch.empty_like(h) if gate is None else gate
+            up = torch.empty_like(h) if up is None else up
+        if workspace is None and not _ffn_aligned(d, x, w_gate, w_up):
+            workspace = _ws(lib().cacti_b200_gated_ffn_fwd_workspace_bytes(tokens, d, f, 0), dev)
+        check(lib().cacti_b200_gated_ffn_fwd(_ptr(h), _ptr(gate), _ptr(up), _ptr(x), _ptr(w_gate), _ptr(w_up), tokens, d, f,
+                                             _dt(x), _ptr(workspace), workspace.numel() if workspace is not None else 0,
+                                             _stream()), what)
+    return h, gate, up
+
+
+def gated_ffn_bwd(dh, x, w_gate, w_up, gate, up, dx=None, dw_gate=None, dw_up=None, beta_dx=0, beta_dw=0, workspace=None):
+    """(dx, dw_gate, dw_up) of gated_ffn_fwd from dh and the saved projections; beta_dx / beta_dw = 1 add to what the given
+    outputs hold."""
+    what = "gated_ffn_bwd"
+    tokens, d, f = _ffn_shapes(what, x, w_gate)
+    dev, dt = x.device, (x.dtype,)
+    _same(what, dev, x=(x, None, _HALF), dh=(dh, (tokens, f), dt), w_gate=(w_gate, (f, d), dt), w_up=(w_up, (f, d), dt),
+          gate=(gate, (tokens, f), dt), up=(up, (tokens, f), dt), dx=(dx, (tokens, d), dt), dw_gate=(dw_gate, (f, d), dt),
+          dw_up=(dw_up, (f, d), dt))
+    if (beta_dx and dx is None) or (beta_dw and (dw_gate is None or dw_up is None)):
+        raise ValueError(f"{what}: beta = 1 adds to an output that is not given")
+    with _on(dev):
+        dx = torch.empty(tokens, d, dtype=x.dtype, device=dev) if dx is None else dx
+        dw_gate = torch.empty(f, d, dtype=x.dtype, device=dev) if dw_gate is None else dw_gate
+        dw_up = torch.empty(f, d, dtype=x.dtype, device=dev) if dw_up is None else dw_up
+        if workspace is None:
+            workspace = _ws(lib().cacti_b200_gated_ffn_bwd_workspace_bytes(tokens, d, f, _ffn_aligned(d, x, w_gate, w_up)), dev)
+        check(lib().cacti_b200_gated_ffn_bwd(_ptr(dx), _ptr(dw_gate), _ptr(dw_up), _ptr(dh), _ptr(x), _ptr(w_gate),
+                                             _ptr(w_up), _ptr(gate), _ptr(up), tokens, d, f, _dt(x), beta_dx, beta_dw,
+                                             _ptr(workspace), workspace.numel(), _stream()), what)
+    return dx, dw_gate, dw_up
 
 
 # ---- A1 ---------------------------------------------------------------------------------------

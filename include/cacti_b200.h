@@ -223,6 +223,38 @@ int cacti_b200_softmax_nll_fwd_bwd(cacti_b200_dptr loss_sum, cacti_b200_dptr los
                                    cacti_b200_stream stream);
 /* forward only: dlogits = 0 skips the gradient */
 
+/* ---- K5b distillation from a teacher's listed logits --------------------------------------------
+ * No counterpart in the reference: the place of K5 in a step whose target is a teacher's distribution.
+ * logits_topk is the teacher's side: the k largest logits of each row, largest first, equal values (+0 equals -0) by
+ * ascending index, NaN above +inf, as values [rows, k] of dtype and indices [rows, k] int32; lse (optional, f32[rows]) is
+ * log sum_j exp(x_j / temperature) over the whole row: -inf for a row of -inf, NaN for a row that holds a NaN.
+ * 1 <= k <= 256, k <= vocab <= 262144 (else CACTI_B200_ERR_SHAPE), temperature in [1e-4, 1e4]. */
+int cacti_b200_logits_topk(cacti_b200_dptr values, cacti_b200_dptr indices, cacti_b200_dptr lse, cacti_b200_dptr logits,
+                           int64_t rows, int64_t vocab, int64_t k, float temperature, int dtype, cacti_b200_stream stream);
+/* The student's side: with c = 1 / temperature, q = softmax(c x) over the row, and a list of k (index t, teacher logit z):
+ *   t_lse = 0: p = softmax(c z) over the list, r = 0.
+ *   t_lse f32[rows] (the teacher's log sum exp(c z) over its whole row): p_k = exp(c z_k - t_lse), and the positions that
+ *   are not listed form one bucket of teacher mass r = max(0, 1 - sum p) (0 where every position is listed).
+ *   loss_i = sum_k p_k (log p_k - log q_k) + r (log r - log Q),  Q = the student's probability of all unlisted positions
+ *   dlogits_j = T(w_i c (P q_j - p_j)) if j is listed, T(w_i c (P - r / Q) q_j) if not;  P = sum p + r
+ * w, loss_sum, loss_rows, dlogits (0: forward only), beta_dlogits, status and workspace as in
+ * cacti_b200_softmax_nll_fwd_bwd; workspace_bytes from the query below.
+ *   t_values [rows, k] of t_dtype (R_32F, R_16F or R_16BF, independent of dtype), t_indices [rows, k] of R_32I or R_16U.
+ * Index -1 (R_16U: 65535, where that is no index) marks an unused slot, anywhere in a list; a row without used slots (or
+ * whose used logits are all -inf) has loss 0 and gradient 0.  Any other index outside [0, vocab), and an index listed
+ * twice (every slot but the first), writes CACTI_B200_ERR_INDEX_RANGE to *status; the slot is left out and the row's loss
+ * is NaN.  A row of weight 0 is not read: loss 0, gradient 0 (beta 1: dlogits unchanged).
+ * Statistics, listed probabilities and the loss are kept in f64 except for the f32 sums of the exponentials.
+ * 1 <= k <= 256, vocab <= 262144 (else CACTI_B200_ERR_SHAPE), temperature in [1e-4, 1e4].  dlogits must not overlap
+ * logits. */
+size_t cacti_b200_distill_topk_workspace_bytes(int64_t rows);
+int cacti_b200_distill_topk_fwd_bwd(cacti_b200_dptr loss_sum, cacti_b200_dptr loss_rows, cacti_b200_dptr dlogits,
+                                    cacti_b200_dptr logits, cacti_b200_dptr t_values, int t_dtype, cacti_b200_dptr t_indices,
+                                    int index_dtype, cacti_b200_dptr t_lse, int64_t k, float temperature,
+                                    cacti_b200_dptr w_rows, float w_scalar, int64_t rows, int64_t vocab, int dtype,
+                                    int beta_dlogits, cacti_b200_dptr status, cacti_b200_dptr workspace, size_t workspace_bytes,
+                                    cacti_b200_stream stream);
+
 /* ---- K6 embedding gather / scatter-add ----------------------------------------------------
  * gather replaces OuterSelect (src/thunk/op.rs:1229-1314): out[i,:] = table[tok[i],:], a bit-exact copy.
  * scatter_add is its adjoint (a Futhark vjp in the reference): dtable[v,:] (+)= sum_{i: tok[i]=v} dy[i,:],
@@ -323,6 +355,30 @@ int cacti_b200_gemm_strided_batched_tri(cacti_b200_dptr c, cacti_b200_dptr a, ca
                                         int64_t stride_c_outer, int64_t stride_c_inner, int tri_mode, int64_t diag,
                                         int operand_flags, int dtype, cacti_b200_dptr workspace, size_t workspace_bytes,
                                         cacti_b200_stream stream);
+
+/* ---- G3 gated feed-forward block -----------------------------------------------------------------
+ * The two projections, the activation and the product of a layer's MLP (src/librarium/llama.rs:522-527) as one kernel, and
+ * its adjoint.  No single counterpart in the reference.  Packed row-major, weights [d_ffn, d_model] as the matmul thunks take
+ * them with trans_b = 1, R_16F or R_16BF, f32 accumulation:
+ *   g = x w_gate^T, u = x w_up^T, h = T(silu(g) u);  gate = T(g), up = T(u) are written too unless both are 0
+ * silu and the product are formed from the f32 sums and h is rounded once, where the separate thunks round g, u and every
+ * primitive after them; the separate entry points keep their results.
+ * Adjoint, from dh [tokens, d_ffn] and the saved gate and up, s = sigmoid(gate):
+ *   dg = T(dh up s (1 + gate (1 - s))), du = T(dh gate s)
+ *   dx = T(dg w_gate + du w_up + beta_dx dx),  dw_gate = T(dg^T x + beta_dw dw_gate),  dw_up = T(du^T x + beta_dw dw_up)
+ * (sums in f32, one rounding; the old value is added in f32 before it, as in cacti_b200_gemm).  tokens = 0 is legal: the
+ * adjoint then writes zero weight gradients (beta_dw = 0).  d_model = 0 or d_ffn = 0 is CACTI_B200_ERR_SHAPE.
+ * Outputs may not overlap inputs or one another.  Workspaces: 256-byte aligned; `aligned` = 1 asks for what suffices when
+ * d_model is a multiple of 8 and x, w_gate and w_up are 16-byte aligned (operands that are not are repacked), 0 for any. */
+size_t cacti_b200_gated_ffn_fwd_workspace_bytes(int64_t tokens, int64_t d_model, int64_t d_ffn, int aligned);
+int cacti_b200_gated_ffn_fwd(cacti_b200_dptr h, cacti_b200_dptr gate, cacti_b200_dptr up, cacti_b200_dptr x,
+                             cacti_b200_dptr w_gate, cacti_b200_dptr w_up, int64_t tokens, int64_t d_model, int64_t d_ffn,
+                             int dtype, cacti_b200_dptr workspace, size_t workspace_bytes, cacti_b200_stream stream);
+size_t cacti_b200_gated_ffn_bwd_workspace_bytes(int64_t tokens, int64_t d_model, int64_t d_ffn, int aligned);
+int cacti_b200_gated_ffn_bwd(cacti_b200_dptr dx, cacti_b200_dptr dw_gate, cacti_b200_dptr dw_up, cacti_b200_dptr dh,
+                             cacti_b200_dptr x, cacti_b200_dptr w_gate, cacti_b200_dptr w_up, cacti_b200_dptr gate,
+                             cacti_b200_dptr up, int64_t tokens, int64_t d_model, int64_t d_ffn, int dtype, int beta_dx,
+                             int beta_dw, cacti_b200_dptr workspace, size_t workspace_bytes, cacti_b200_stream stream);
 
 /* ---- A1 block padding and fused causal attention ------------------------------------------------------------
  * block_pad replaces BlockPadFutThunkSpec (src/thunk/op.rs:4065-4186), which the reference stages before a block

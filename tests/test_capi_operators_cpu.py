@@ -1,0 +1,69 @@
+"""Argument checks of the distillation and gated feed-forward entry points: none of these calls launches anything."""
+from cacti_b200 import capi
+
+P = 0x1000          # non-null and aligned, never dereferenced: every call below is refused first
+
+
+def _topk(values=P, indices=P, lse=P, logits=P, rows=4, vocab=100, k=10, temperature=1.0, dtype=capi.R_16F):
+    return capi.lib().cacti_b200_logits_topk(values, indices, lse, logits, rows, vocab, k, temperature, dtype, None)
+
+
+def _distill(loss_sum=P, loss_rows=P, dlogits=P, logits=P, tv=P, td=capi.R_16F, ti=P, idt=capi.R_32I, lse=0, k=4, temperature=1.0,
+             w=0, rows=4, vocab=100, dtype=capi.R_16F, beta=0, status=0, ws=0, wsb=0):
+    return capi.lib().cacti_b200_distill_topk_fwd_bwd(loss_sum, loss_rows, dlogits, logits, tv, td, ti, idt, lse, k, temperature, w,
+                                                      1.0, rows, vocab, dtype, beta, status, ws, wsb, None)
+
+
+def _fwd(h=P, gate=0, up=0, x=P, wg=P, wu=P, t=4, d=16, f=24, dtype=capi.R_16F, ws=0, wsb=0):
+    return capi.lib().cacti_b200_gated_ffn_fwd(h, gate, up, x, wg, wu, t, d, f, dtype, ws, wsb, None)
+
+
+def _bwd(dx=P, dwg=P, dwu=P, dh=P, x=P, wg=P, wu=P, gate=P, up=P, t=4, d=16, f=24, dtype=capi.R_16F, bx=0, bw=0, ws=0x1000, wsb=1 << 30):
+    return capi.lib().cacti_b200_gated_ffn_bwd(dx, dwg, dwu, dh, x, wg, wu, gate, up, t, d, f, dtype, bx, bw, ws, wsb, None)
+
+
+def test_topk_refusals():
+    assert _topk(rows=-1) == _topk(vocab=-5) == _topk(k=-1) == capi.ERR_INVALID_VALUE
+    assert _topk(values=0) == _topk(indices=0) == _topk(logits=0) == capi.ERR_INVALID_VALUE
+    assert _topk(values=P + 1) == _topk(logits=P + 1) == _topk(indices=P + 2) == _topk(lse=P + 2) == capi.ERR_INVALID_VALUE
+    assert _topk(logits=P + 2, dtype=capi.R_32F) == capi.ERR_INVALID_VALUE
+    for t in (0.0, -1.0, float("nan"), float("inf"), 1e-5, 1e5):
+        assert _topk(temperature=t) == capi.ERR_INVALID_VALUE
+    assert _topk(dtype=capi.R_32I) == capi.ERR_DTYPE
+    assert _topk(k=0) == _topk(k=101) == _topk(vocab=1000, k=257) == _topk(vocab=262145) == _topk(vocab=0) == capi.ERR_SHAPE
+    assert _topk(rows=0) == capi.OK
+
+
+def test_distill_refusals():
+    assert _distill(rows=-1) == _distill(vocab=-1) == _distill(beta=2) == capi.ERR_INVALID_VALUE
+    assert _distill(logits=0) == _distill(tv=0) == _distill(ti=0) == capi.ERR_INVALID_VALUE
+    for name in ("loss_sum", "loss_rows", "lse", "w", "status"):
+        assert _distill(**{name: P + 2}) == capi.ERR_INVALID_VALUE, name
+    assert _distill(logits=P + 1) == _distill(dlogits=P + 1) == _distill(tv=P + 1) == _distill(ti=P + 2) == capi.ERR_INVALID_VALUE
+    for t in (0.0, -2.0, float("nan"), float("inf"), 1e-5, 1e5):
+        assert _distill(temperature=t) == capi.ERR_INVALID_VALUE
+    assert _distill(dtype=capi.R_16U) == _distill(td=capi.R_32I) == _distill(idt=capi.R_32F) == capi.ERR_DTYPE
+    assert _distill(k=0) == _distill(k=257) == _distill(vocab=262145) == capi.ERR_SHAPE
+    assert _distill(loss_rows=0) == _distill(loss_rows=0, ws=P, wsb=8) == _distill(loss_rows=0, ws=P + 1, wsb=4096) == capi.ERR_WORKSPACE
+    assert _distill(rows=0) == _distill(vocab=0) == capi.OK
+    assert capi.lib().cacti_b200_distill_topk_workspace_bytes(8192) >= 8192 * 4
+
+
+def test_gated_ffn_refusals():
+    assert _fwd(t=-1) == _fwd(d=-1) == _fwd(f=-1) == capi.ERR_INVALID_VALUE
+    assert _fwd(h=0) == _fwd(x=0) == _fwd(wg=0) == _fwd(wu=0) == capi.ERR_INVALID_VALUE
+    assert _fwd(gate=P) == _fwd(up=P) == _fwd(x=P + 1) == capi.ERR_INVALID_VALUE
+    assert _fwd(dtype=capi.R_32F) == capi.ERR_DTYPE
+    assert _fwd(d=0) == _fwd(f=0) == _fwd(t=1 << 31) == capi.ERR_SHAPE
+    assert _fwd(t=0) == capi.OK
+    assert _bwd(t=-1) == _bwd(bx=2) == _bwd(bw=-1) == capi.ERR_INVALID_VALUE
+    for name in ("dx", "dwg", "dwu", "dh", "x", "wg", "wu", "gate", "up"):
+        assert _bwd(**{name: 0}) == capi.ERR_INVALID_VALUE, name
+        assert _bwd(**{name: P + 1}) == capi.ERR_INVALID_VALUE, name
+    assert _bwd(dtype=capi.R_32F) == capi.ERR_DTYPE
+    assert _bwd(d=0) == _bwd(f=0) == capi.ERR_SHAPE
+    assert _bwd(ws=0) == _bwd(ws=0x1010) == _bwd(wsb=100) == capi.ERR_WORKSPACE
+    L = capi.lib()
+    for t, d, f in ((1, 8, 8), (77, 1003, 277), (2048, 3200, 8640)):
+        assert L.cacti_b200_gated_ffn_bwd_workspace_bytes(t, d, f, 0) >= L.cacti_b200_gated_ffn_bwd_workspace_bytes(t, d, f, 1) >= 4 * t * f
+        assert L.cacti_b200_gated_ffn_fwd_workspace_bytes(t, d, f, 0) >= L.cacti_b200_gated_ffn_fwd_workspace_bytes(t, d, f, 1)
