@@ -16,6 +16,7 @@
 //
 // The tile walk is static: no global counter, so calls may overlap on any streams and graphs.
 #include "gemm_common.cuh"
+#include <utility>
 
 namespace cb {
 
@@ -284,6 +285,12 @@ static int ffn_operand(Operand& o, uint64_t ptr, int64_t rows, int64_t cols, uin
   return rc;
 }
 
+// Sizes whose tile, k-block and vector counts fit 32-bit indices (any that fit the device's memory do).
+static bool ffn_sizes_ok(int64_t tokens, int64_t D, int64_t F) {
+  constexpr int64_t kMax = 1 << 24, kElems = 1LL << 34;
+  return D > 0 && F > 0 && tokens <= kMax && D <= kMax && F <= kMax && tokens * (F + 64) < kElems && tokens * D < kElems && F * D < kElems;
+}
+
 static bool ffn_rows_aligned(uint64_t ptr, int64_t cols) { return ((ptr | (uint64_t)(cols * 2)) & 15) == 0; }
 
 static uint32_t ffn_idesc(bool bf16, int a_mn, int b_mn, int n, int m) {
@@ -339,21 +346,383 @@ static int ffn_fwd_run(uint64_t h, uint64_t gate, uint64_t up, uint64_t x, uint6
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------
-template <typename T>
+// dg and du, rows zero-padded from F to Fp = a multiple of 64 elements, so that no box of the products is partly out of range.
+// One 16-byte vector of each a thread and trip; VEC: the inputs' rows are 16-byte aligned.
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
-gated_ffn_adjoint_kernel(T* __restrict__ dG, T* __restrict__ dU, const T* __restrict__ dH, const T* __restrict__ G,
-                         const T* __restrict__ U, int64_t n, int64_t F) {
-  // dG and dU are the two halves of rows of 2 F
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t o = i + i / F * F;
-    const float g = Elem<T>::to_f32(G[i]), u = Elem<T>::to_f32(U[i]), dh = Elem<T>::to_f32(dH[i]);
-    const float s = sigmoid_f32(g);
-    dG[o] = Elem<T>::from_f32(dh * u * (s * (1.f + g * (1.f - s))));
-    dU[o] = Elem<T>::from_f32(dh * (g * s));
+ffn_adjoint_kernel(T* __restrict__ dG, T* __restrict__ dU, const T* __restrict__ dH, const T* __restrict__ G,
+                   const T* __restrict__ U, unsigned nvec, unsigned F, unsigned vpr /* vectors per padded row */) {
+  for (unsigned i = blockIdx.x * blockDim.x + threadIdx.x; i < nvec; i += gridDim.x * blockDim.x) {
+    const unsigned row = i / vpr, c = (i - row * vpr) * 8;
+    float g[8], u[8], d[8];
+    const long long src = (long long)row * F + c;
+    if (VEC) {
+      const bool in = c < F;
+      const uint4 z = make_uint4(0, 0, 0, 0);
+      unpack<T>(in ? ld_stream(G + src) : z, g);
+      unpack<T>(in ? ld_stream(U + src) : z, u);
+      unpack<T>(in ? ld_stream(dH + src) : z, d);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const bool in = c + e < F;
+        g[e] = in ? Elem<T>::to_f32(G[src + e]) : 0.f;
+        u[e] = in ? Elem<T>::to_f32(U[src + e]) : 0.f;
+        d[e] = in ? Elem<T>::to_f32(dH[src + e]) : 0.f;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float s = sigmoid_f32(g[e]);
+      const float dg = d[e] * u[e] * (s * (1.f + g[e] * (1.f - s)));
+      u[e] = d[e] * (g[e] * s);
+      g[e] = dg;
+    }
+    reinterpret_cast<uint4*>(dG)[i] = pack<T>(g);
+    reinterpret_cast<uint4*>(dU)[i] = pack<T>(u);
   }
 }
 
-static size_t ffn_align(size_t n) { return (n + 255) / 256 * 256; }
+// The products of the adjoint.  pr[0]: dx, contraction over `parts` = 2 operand pairs of nkb k-blocks, cut into `splits`
+// ranges; pr[1]: dWg and, `tiles` further on, dWu.
+struct FfnProduct { GemmParams g; int a_mn, nkb, tiles; };
+struct FfnBwdParams {
+  FfnProduct pr[2];
+  int splits;                    // ranges of dx's contraction; 1: none, else partial sums go to `part`
+  float* part;                   // [splits][M][N] f32
+  int nx, total;                 // items of dx (tiles * splits), all items
+  int light0, extra;             // see FfnWalk
+};
+
+// Static walk of worker w of W: the dx items w, w + W, ... first, which are the longest; workers that got one fewer (w >=
+// light0) then take `extra` weight-gradient tiles each, about as many as one dx item lasts, and the rest goes round.
+struct FfnWalk {
+  int w, W, pos, phase, end1;
+  __device__ __forceinline__ void init(const FfnBwdParams& p, int w_, int W_) {
+    w = w_; W = W_; pos = w; phase = 0;
+    const int n = p.extra * (W - p.light0), rest = p.total - p.nx;
+    end1 = p.nx + (n < rest ? n : rest);
+  }
+  __device__ __forceinline__ int next(const FfnBwdParams& p) {
+    int t;
+    if (phase == 0) {
+      if (pos < p.nx) { t = pos; pos += W; return t; }
+      phase = 1;
+      pos = p.nx + w - p.light0;
+      if (w < p.light0) pos = end1;
+    }
+    if (phase == 1) {
+      if (pos < end1) { t = pos; pos += W - p.light0; return t; }
+      phase = 2;
+      pos = end1 + (W - 1 - w);          // the ragged end falls to the workers that were light
+    }
+    if (pos < p.total) { t = pos; pos += W; return t; }
+    return -1;
+  }
+};
+
+struct FfnItem { int prod, part, tm, tn, kb0, kb1, split; };
+__device__ __forceinline__ FfnItem ffn_item(const FfnBwdParams& p, int t) {
+  FfnItem it;
+  it.split = 0; it.part = 0;
+  if (t < p.nx) {
+    it.prod = 0;
+    const int tiles = p.pr[0].tiles, nk = 2 * p.pr[0].nkb;
+    it.split = t / tiles;                // neighbours in time share a range of the contraction, and so operand panels
+    t -= it.split * tiles;
+    it.kb0 = (int)((long long)nk * it.split / p.splits);
+    it.kb1 = (int)((long long)nk * (it.split + 1) / p.splits);
+  } else {
+    it.prod = 1;
+    t -= p.nx;
+    it.part = t / p.pr[1].tiles;
+    t -= it.part * p.pr[1].tiles;
+    it.kb0 = 0; it.kb1 = p.pr[1].nkb;
+  }
+  const GemmParams& g = p.pr[it.prod].g;
+  ffn_decode(t, g.tiles_m, g.tiles_n, g.group_m, it.tm, it.tn);
+  return it;
+}
+
+// Epilogue of a range of dx's contraction: the f32 accumulator to its place in the partial sums.
+template <int BN>
+__device__ __forceinline__ void ffn_partial_tile(float* __restrict__ part, int M, int N, uint32_t tmem_base, int acc, int row, int tn,
+                                                 int q, int lane, uint32_t tempty_addr) {
+#pragma unroll 1
+  for (int c = 0; c < BN / 32; ++c) {
+    const int col0 = tn * BN + c * 32;
+    if (col0 >= N) break;                // warp-uniform
+    uint32_t v[32];
+    tc_ld32(tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN + c * 32), v);
+    tc_ld_wait();
+    if (row < M) {
+      float* out = part + (long long)row * N + col0;
+      if ((N & 3) == 0) {                // col0 + 4 i + 3 < N whenever col0 + 4 i < N
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (col0 + 4 * i < N) __stcg(reinterpret_cast<uint4*>(out) + i, make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) if (col0 + i < N) __stcg(out + i, __uint_as_float(v[i]));
+      }
+    }
+  }
+  tc_fence_before();
+  __syncwarp();
+  if (lane == 0) mbar_arrive_cluster(tempty_addr);
+}
+
+// The two-SM matmul kernel over the items of all three products.  A is dg / du, stored [tokens][Fp]: K-major for dx, MN-major
+// for the weight gradients, the same 64 x 64 boxes either way; B is MN-major throughout (weights [F][D], x [tokens][D]).
+template <typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
+ffn_bwd_kernel(const __grid_constant__ FfnMaps maps, T* __restrict__ dX, T* __restrict__ dWg, T* __restrict__ dWu,
+               const __grid_constant__ FfnBwdParams p) {
+  constexpr int BN = 256, HB = 128, STAGES = 6;
+  constexpr uint32_t A_BYTES = kBM * kBK * 2, STAGE_BYTES = kFfnStageBytes;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* tiles = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint64_t* full = reinterpret_cast<uint64_t*>(tiles + (size_t)STAGES * STAGE_BYTES);
+  uint64_t* empty = full + STAGES;
+  uint64_t* tfull = empty + STAGES;
+  uint64_t* tempty = tfull + 2;
+  uint64_t* cbar = tempty + 2;                  // one per epilogue warp: old C boxes have arrived
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(cbar + 4);
+  unsigned char* cstage = tiles + (size_t)STAGES * STAGE_BYTES + 1024;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int worker = blockIdx.x >> 1, nworkers = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) { mbar_init(full + s, 1); mbar_init(empty + s, 1); }
+    for (int a = 0; a < 2; ++a) { mbar_init(tfull + a, 1); mbar_init(tempty + a, 8); }
+    for (int w = 0; w < 4; ++w) mbar_init(cbar + w, 1);
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();                           // the peer's barriers are initialised before anything signals them
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  FfnWalk walk;
+  walk.init(p, worker, nworkers);
+
+  if (warp == 0 && lane == 0) {
+    // ---------------- TMA producer (both CTAs) ----------------
+    int s = 0; unsigned ph = 0;
+    bool ok = true;
+    for (int t = walk.next(p); ok && t >= 0; t = walk.next(p)) {
+      const FfnItem it = ffn_item(p, t);
+      const FfnProduct& pr = p.pr[it.prod];
+      // a last column tile with at most 128 columns runs as an N = 128 MMA: each CTA then supplies 64 rows of B
+      const int hb = (pr.g.N - it.tn * BN <= HB) ? HB / 2 : HB;
+      const int m0 = it.tm * 256 + (int)rank * kBM, n0 = it.tn * BN + (int)rank * hb;
+      for (int kb = it.kb0; kb < it.kb1; ++kb) {
+        if (!mbar_wait_bounded(empty + s, ph ^ 1, kDevErrGemmTimeout)) { ok = false; break; }
+        unsigned char* sa = tiles + (size_t)s * STAGE_BYTES;
+        unsigned char* sb = sa + A_BYTES;
+        const uint32_t fb = map_to_rank(smem_u32(full + s), 0);
+        if (rank == 0) mbar_expect_tx(full + s, 2 * STAGE_BYTES);
+        const int part = it.prod ? it.part : (kb >= pr.nkb ? 1 : 0);
+        const int k0 = (it.prod ? kb : kb - part * pr.nkb) * kBK;
+        const CUtensorMap* ma = &maps.a[part];
+        const CUtensorMap* mb = it.prod ? &maps.b[2] : &maps.b[part];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (pr.a_mn) tma_load_4d_pair(sa + h * 8192, ma, fb, m0 + h * 64, k0, 0, 0);
+          else tma_load_4d_pair(sa + h * 8192, ma, fb, k0, m0 + h * 64, 0, 0);
+          tma_load_4d_pair(sb + h * 8192, mb, fb, n0 + h * 64, k0, 0, 0);
+        }
+        if (++s == STAGES) { s = 0; ph ^= 1; }
+      }
+    }
+    // the leader's last commits still arrive on this CTA's empty barriers: wait for them before leaving
+    for (int i = 0; ok && i < STAGES; ++i) {
+      ok = mbar_wait_bounded(empty + s, ph ^ 1, kDevErrGemmTimeout);
+      if (++s == STAGES) { s = 0; ph ^= 1; }
+    }
+  } else if (warp == 1 && lane == 0 && rank == 0) {
+    // ---------------- MMA issuer (leader CTA) ----------------
+    int s = 0; unsigned ph = 0;
+    int local = 0;
+    bool ok = true;
+    for (int t = walk.next(p); ok && t >= 0; t = walk.next(p), ++local) {
+      const FfnItem it = ffn_item(p, t);
+      const FfnProduct& pr = p.pr[it.prod];
+      const uint32_t idesc = (pr.g.N - it.tn * BN <= HB) ? idesc_with_n(pr.g.idesc, HB) : pr.g.idesc;      // see the producer
+      const uint32_t a_step = pr.a_mn ? 2048 : 32, a_lbo = pr.a_mn ? 512 : 1;
+      const int acc = local & 1;
+      if (!mbar_wait_bounded(tempty + acc, (unsigned)((local >> 1) & 1) ^ 1, kDevErrGemmTimeout)) break;
+      tc_fence_after();
+      const uint32_t tacc = tmem_base + (uint32_t)acc * BN;
+      for (int kb = it.kb0; kb < it.kb1; ++kb) {
+        if (!mbar_wait_bounded(full + s, ph, kDevErrGemmTimeout)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t sa = smem_u32(tiles + (size_t)s * STAGE_BYTES), sb = sa + A_BYTES;
+#pragma unroll
+        for (int k4 = 0; k4 < kBK / 16; ++k4)
+          tc_mma_f16_pair(tacc, make_desc(sa + k4 * a_step, a_lbo, 64), make_desc(sb + k4 * 2048, 512, 64), idesc,
+                          (kb > it.kb0 || k4) ? 1u : 0u);
+        tc_commit_pair(empty + s);
+        if (++s == STAGES) { s = 0; ph ^= 1; }
+      }
+      if (!ok) break;
+      tc_commit_pair(tfull + acc);
+    }
+  } else if (warp >= 2) {
+    // ---------------- epilogue (both CTAs, each on its own 128 rows) ----------------
+    const int q = warp & 3;
+    int local = 0;
+    unsigned cpar = 0;                          // phase of this warp's old-C barrier
+    for (int t = walk.next(p); t >= 0; t = walk.next(p), ++local) {
+      const FfnItem it = ffn_item(p, t);
+      const int acc = local & 1;
+      if (!mbar_wait_bounded_warp(tfull + acc, (unsigned)((local >> 1) & 1), kDevErrGemmTimeout)) break;
+      tc_fence_after();
+      const int row0 = it.tm * 256 + (int)rank * kBM + q * 32;
+      const uint32_t te = map_to_rank(smem_u32(tempty + acc), 0);
+      const GemmParams& g = p.pr[it.prod].g;
+      if (it.prod == 0 && p.splits > 1)
+        ffn_partial_tile<BN>(p.part + (long long)it.split * g.M * g.N, g.M, g.N, tmem_base, acc, row0 + lane, it.tn, q, lane, te);
+      else
+        epilogue_tile<T, BN>(g, maps.c[it.prod + it.part], it.prod == 0 ? dX : it.part ? dWu : dWg, tmem_base, acc, row0, it.tn, 0, 0, q,
+                             lane, cstage + (size_t)(warp - 2) * 8192, te, cbar + (warp - 2), cpar);
+    }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();                           // both CTAs have finished reading TMEM and signalling each other
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
+  }
+}
+constexpr size_t kFfnBwdSmem = (size_t)6 * kFfnStageBytes + 1024 + 1024 + 4 * 8192;
+
+// dx = T(sum of the ranges' partial sums in order + beta * old)
+template <typename T>
+__global__ void __launch_bounds__(256)
+ffn_join_kernel(T* __restrict__ out, const float* __restrict__ part, long long n, int splits, int beta) {
+  dependent_wait();
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
+    float v = 0.f;
+    for (int s = 0; s < splits; ++s) v += __ldcg(part + (long long)s * n + i);
+    if (beta) v += Elem<T>::to_f32(out[i]);
+    out[i] = Elem<T>::from_f32(v);
+  }
+}
+
+// What a backward call does, from its sizes alone.
+struct FfnBwdPlan { int64_t Fp; size_t dpart, part; int tiles_x, tiles_w, nkb_x, nkb_w, splits, workers; };
+static FfnBwdPlan ffn_bwd_plan(int64_t T, int64_t D, int64_t F) {
+  FfnBwdPlan b;
+  b.Fp = packed_cols(F);
+  b.dpart = ((size_t)T * b.Fp * 2 + 255) / 256 * 256;
+  const int64_t tn = (D + 255) / 256;
+  const int64_t tx = (T + 255) / 256 * tn, tw = (F + 255) / 256 * tn;
+  b.tiles_x = (int)tx; b.tiles_w = (int)tw;
+  b.nkb_x = (int)(b.Fp / kBK); b.nkb_w = (int)((T + kBK - 1) / kBK);
+  const int64_t W = kNumSMs / 2;
+  // dx's contraction is cut when one of its tiles would last longer than a worker's share of all the work (few tokens:
+  // few tiles, each 2 F deep); ranges of at least 8 k-blocks
+  const int64_t work = tx * 2 * b.nkb_x + 2 * tw * b.nkb_w, share = (work + W - 1) / W;
+  int64_t s = (2 * b.nkb_x + share - 1) / share;
+  if (s > 2 * b.nkb_x / 8) s = 2 * b.nkb_x / 8;
+  if (s > 16) s = 16;
+  if (s < 1) s = 1;
+  b.splits = (int)s;
+  b.part = s > 1 ? ((size_t)s * T * D * 4 + 255) / 256 * 256 : 0;
+  const int64_t items = tx * s + 2 * tw;
+  b.workers = (int)(items < W ? items : W);
+  return b;
+}
+
+static int ffn_result(FfnProduct& pr, CUtensorMap* map, uint64_t c, int64_t M, int64_t N, int a_mn, int nkb, int beta, bool bf16) {
+  GemmParams& g = pr.g;
+  g = GemmParams{};
+  g.M = (int)M; g.N = (int)N;
+  g.nb_inner = g.nb_outer = 1;
+  g.tiles_m = (int)((M + 255) / 256); g.tiles_n = (int)((N + 255) / 256);
+  g.ldc = N; g.alpha = 1.f; g.beta = beta ? 1.f : 0.f;
+  g.idesc = ffn_idesc(bf16, a_mn, 1, 256, 256);
+  const uint64_t all = c | (uint64_t)(N * 2);
+  g.c_align = (all & 15) == 0 ? 16 : (all & 7) == 0 ? 8 : (all & 3) == 0 ? 4 : 2;
+  g.group_m = g.tiles_m < 8 ? g.tiles_m : 8;
+  pr.a_mn = a_mn; pr.nkb = nkb; pr.tiles = g.tiles_m * g.tiles_n;
+  g.c_tma = (all & 15) == 0;
+  return g.c_tma ? encode_operand(map, Operand{c, M, N, N, 0, 0, 0, 0}, 1, 1, 64, 32, bf16) : CACTI_B200_OK;
+}
+
+template <typename T>
+static int ffn_bwd_run(uint64_t dx, uint64_t dwg, uint64_t dwu, uint64_t dh, uint64_t x, uint64_t wg, uint64_t wu, uint64_t gate,
+                       uint64_t up, int64_t tokens, int64_t D, int64_t F, int beta_dx, int beta_dw, uint64_t ws, size_t ws_bytes,
+                       cudaStream_t st) {
+  const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+  const FfnBwdPlan b = ffn_bwd_plan(tokens, D, F);
+  size_t off = 2 * b.dpart + b.part;
+  if (!ws || (ws & 255) || ws_bytes < off) return CACTI_B200_ERR_WORKSPACE;
+  Operand ox, og, ou;
+  for (const auto& [ptr, rows] : {std::pair<uint64_t, int64_t>{x, tokens}, {wg, F}, {wu, F}}) {     // before anything is launched
+    if (!ffn_rows_aligned(ptr, D)) off += packed_bytes(rows, D, 1);
+  }
+  if (ws_bytes < off) return CACTI_B200_ERR_WORKSPACE;
+  off = 2 * b.dpart + b.part;
+  const unsigned vpr = (unsigned)(b.Fp / 8), nvec = (unsigned)(tokens * vpr);
+  const unsigned want = (nvec + 255) / 256, cap = kNumSMs * 32;
+  const bool vec = ffn_rows_aligned(dh, F) && ffn_rows_aligned(gate, F) && ffn_rows_aligned(up, F);
+  auto adj = vec ? ffn_adjoint_kernel<T, true> : ffn_adjoint_kernel<T, false>;
+  adj<<<want < cap ? want : cap, 256, 0, st>>>(reinterpret_cast<T*>(ws), reinterpret_cast<T*>(ws + b.dpart),
+                                               reinterpret_cast<const T*>(dh), reinterpret_cast<const T*>(gate),
+                                               reinterpret_cast<const T*>(up), nvec, (unsigned)F, vpr);
+  int rc = check_launch();
+  if (!rc) rc = ffn_operand(ox, x, tokens, D, ws, ws_bytes, off, st);
+  if (!rc) rc = ffn_operand(og, wg, F, D, ws, ws_bytes, off, st);
+  if (!rc) rc = ffn_operand(ou, wu, F, D, ws, ws_bytes, off, st);
+  if (rc) return rc;
+  FfnMaps maps;
+  for (int i = 0; i < 2 && !rc; ++i)
+    rc = encode_operand(&maps.a[i], Operand{ws + i * b.dpart, tokens, b.Fp, b.Fp, 0, 0, 0, 0}, 1, 1, 64, 64, bf16);
+  if (!rc) rc = encode_operand(&maps.b[0], og, 1, 1, 64, 64, bf16);
+  if (!rc) rc = encode_operand(&maps.b[1], ou, 1, 1, 64, 64, bf16);
+  if (!rc) rc = encode_operand(&maps.b[2], ox, 1, 1, 64, 64, bf16);
+  if (rc) return rc;
+  for (auto& m : maps.c) m = maps.a[0];
+  FfnBwdParams p;
+  rc = ffn_result(p.pr[0], &maps.c[0], dx, tokens, D, 0, b.nkb_x, beta_dx, bf16);
+  if (!rc) rc = ffn_result(p.pr[1], &maps.c[1], dwg, F, D, 1, b.nkb_w, beta_dw, bf16);
+  if (rc) return rc;
+  FfnProduct up_pr;                             // the up half differs from the gate half in its result's map and alignment only
+  rc = ffn_result(up_pr, &maps.c[2], dwu, F, D, 1, b.nkb_w, beta_dw, bf16);
+  if (rc) return rc;
+  if (up_pr.g.c_align < p.pr[1].g.c_align) p.pr[1].g.c_align = up_pr.g.c_align;
+  p.pr[1].g.c_tma &= up_pr.g.c_tma;
+  p.splits = b.splits;
+  p.part = reinterpret_cast<float*>(ws + 2 * b.dpart);
+  p.nx = b.tiles_x * b.splits;
+  p.total = p.nx + 2 * b.tiles_w;
+  p.light0 = p.nx % b.workers;
+  const int cx = 2 * b.nkb_x / b.splits;
+  p.extra = p.light0 ? (cx + b.nkb_w / 2) / b.nkb_w : 0;
+  auto kern = ffn_bwd_kernel<T>;
+  static bool attr_set[kMaxDevices] = {};
+  ensure_dynamic_smem(kern, kFfnBwdSmem, attr_set);
+  kern<<<(unsigned)(2 * b.workers), kGemmThreads, kFfnBwdSmem, st>>>(maps, reinterpret_cast<T*>(dx), reinterpret_cast<T*>(dwg),
+                                                                     reinterpret_cast<T*>(dwu), p);
+  rc = check_launch();
+  if (!rc && b.splits > 1) {
+    const long long n = (long long)tokens * D, blocks = (n + 255) / 256;
+    launch_dependent(ffn_join_kernel<T>, (unsigned)(blocks < kNumSMs * 8 ? blocks : kNumSMs * 8), 256u, st, reinterpret_cast<T*>(dx),
+                     (const float*)p.part, n, b.splits, beta_dx);
+    rc = check_launch();
+  }
+  return rc;
+}
 
 }  // namespace cb
 
@@ -370,7 +739,7 @@ int cacti_b200_gated_ffn_fwd(cacti_b200_dptr h, cacti_b200_dptr gate, cacti_b200
   using namespace cb;
   if (tokens < 0 || d_model < 0 || d_ffn < 0) return CACTI_B200_ERR_INVALID_VALUE;
   if (dtype != CACTI_B200_R_16F && dtype != CACTI_B200_R_16BF) return CACTI_B200_ERR_DTYPE;
-  if (tokens > 0x3fffffffLL || d_model > 0x3fffffffLL || d_ffn > 0x3fffffffLL || d_model == 0 || d_ffn == 0) return CACTI_B200_ERR_SHAPE;
+  if (!ffn_sizes_ok(tokens, d_model, d_ffn)) return CACTI_B200_ERR_SHAPE;
   if (tokens == 0) return CACTI_B200_OK;
   if (!h || !x || !w_gate || !w_up || !gate != !up) return CACTI_B200_ERR_INVALID_VALUE;
   if ((h | gate | up | x | w_gate | w_up) & 1) return CACTI_B200_ERR_INVALID_VALUE;
@@ -381,11 +750,12 @@ int cacti_b200_gated_ffn_fwd(cacti_b200_dptr h, cacti_b200_dptr gate, cacti_b200
 }
 
 size_t cacti_b200_gated_ffn_bwd_workspace_bytes(int64_t tokens, int64_t d_model, int64_t d_ffn, int aligned) {
-  (void)aligned;
   if (tokens < 0 || d_model < 0 || d_ffn < 0) return 0;
-  const size_t a = cacti_b200_gemm_workspace_bytes(tokens, d_model, 2 * d_ffn, 1, 1);
-  const size_t b = cacti_b200_gemm_workspace_bytes(d_ffn, d_model, tokens, 1, 1);
-  return cb::ffn_align((size_t)tokens * d_ffn * 4) + cb::ffn_align((size_t)d_ffn * d_model * 4) + (a > b ? a : b) + 256;
+  if (tokens == 0 || d_model == 0 || d_ffn == 0) return 256;
+  const cb::FfnBwdPlan b = cb::ffn_bwd_plan(tokens, d_model, d_ffn);
+  size_t n = 2 * b.dpart + b.part + 256;
+  if (!aligned || d_model % 8) n += cb::packed_bytes(tokens, d_model, 1) + 2 * cb::packed_bytes(d_ffn, d_model, 1);
+  return n;
 }
 
 int cacti_b200_gated_ffn_bwd(cacti_b200_dptr dx, cacti_b200_dptr dw_gate, cacti_b200_dptr dw_up, cacti_b200_dptr dh,
@@ -395,7 +765,7 @@ int cacti_b200_gated_ffn_bwd(cacti_b200_dptr dx, cacti_b200_dptr dw_gate, cacti_
   using namespace cb;
   if (tokens < 0 || d_model < 0 || d_ffn < 0 || ((beta_dx | beta_dw) & ~1)) return CACTI_B200_ERR_INVALID_VALUE;
   if (dtype != CACTI_B200_R_16F && dtype != CACTI_B200_R_16BF) return CACTI_B200_ERR_DTYPE;
-  if (tokens > 0x3fffffffLL || d_model > 0x3fffffffLL || d_ffn > 0x3fffffffLL || d_model == 0 || d_ffn == 0) return CACTI_B200_ERR_SHAPE;
+  if (!ffn_sizes_ok(tokens, d_model, d_ffn)) return CACTI_B200_ERR_SHAPE;
   if (!dw_gate || !dw_up) return CACTI_B200_ERR_INVALID_VALUE;
   if (tokens > 0 && (!dx || !dh || !x || !w_gate || !w_up || !gate || !up)) return CACTI_B200_ERR_INVALID_VALUE;
   if ((dx | dw_gate | dw_up | dh | x | w_gate | w_up | gate | up) & 1) return CACTI_B200_ERR_INVALID_VALUE;
@@ -406,31 +776,10 @@ int cacti_b200_gated_ffn_bwd(cacti_b200_dptr dx, cacti_b200_dptr dw_gate, cacti_
         if (cudaMemsetAsync(reinterpret_cast<void*>(w), 0, (size_t)d_ffn * d_model * 2, st) != cudaSuccess) return check_launch();
     return CACTI_B200_OK;
   }
-  if (!workspace || (workspace & 255) || workspace_bytes < cacti_b200_gated_ffn_bwd_workspace_bytes(tokens, d_model, d_ffn, 0))
-    return CACTI_B200_ERR_WORKSPACE;
-  // [dg | du] as rows of 2 d_ffn and [w_gate; w_up] one below the other: dx is one product over 2 d_ffn, rounded once
-  const size_t part = ffn_align((size_t)tokens * d_ffn * 4), wpart = ffn_align((size_t)d_ffn * d_model * 4);
-  const uint64_t dg = workspace, du = dg + (uint64_t)d_ffn * 2, wcat = workspace + part, ws = wcat + wpart;
-  const size_t wsb = workspace_bytes - part - wpart, wb = (size_t)d_ffn * d_model * 2;
-  if (cudaMemcpyAsync(reinterpret_cast<void*>(wcat), reinterpret_cast<const void*>(w_gate), wb, cudaMemcpyDeviceToDevice, st) != cudaSuccess ||
-      cudaMemcpyAsync(reinterpret_cast<void*>(wcat + wb), reinterpret_cast<const void*>(w_up), wb, cudaMemcpyDeviceToDevice, st) != cudaSuccess)
-    return check_launch();
-  const int64_t n = tokens * d_ffn;
-  const int64_t want = (n + 255) / 256, cap = (int64_t)kNumSMs * 32;
-  auto go = [&](auto tag) -> int {
-    using T = decltype(tag);
-    gated_ffn_adjoint_kernel<T><<<(unsigned)(want < cap ? want : cap), 256, 0, st>>>(
-        reinterpret_cast<T*>(dg), reinterpret_cast<T*>(du), reinterpret_cast<const T*>(dh), reinterpret_cast<const T*>(gate),
-        reinterpret_cast<const T*>(up), n, d_ffn);
-    return check_launch();
-  };
-  int rc = dtype == CACTI_B200_R_16F ? go(__half{}) : go(__nv_bfloat16{});
-  const float one = 1.f, zero = 0.f;
-  const float *bx = beta_dx ? &one : &zero, *bw = beta_dw ? &one : &zero;
-  const int64_t f2 = 2 * d_ffn;
-  if (!rc) rc = cacti_b200_gemm(dx, dg, wcat, tokens, d_model, f2, f2, d_model, d_model, 0, 0, &one, bx, dtype, ws, wsb, stream);
-  if (!rc) rc = cacti_b200_gemm(dw_gate, dg, x, d_ffn, d_model, tokens, f2, d_model, d_model, 1, 0, &one, bw, dtype, ws, wsb, stream);
-  if (!rc) rc = cacti_b200_gemm(dw_up, du, x, d_ffn, d_model, tokens, f2, d_model, d_model, 1, 0, &one, bw, dtype, ws, wsb, stream);
-  return rc;
+  if (dtype == CACTI_B200_R_16F)
+    return ffn_bwd_run<__half>(dx, dw_gate, dw_up, dh, x, w_gate, w_up, gate, up, tokens, d_model, d_ffn, beta_dx, beta_dw, workspace,
+                               workspace_bytes, st);
+  return ffn_bwd_run<__nv_bfloat16>(dx, dw_gate, dw_up, dh, x, w_gate, w_up, gate, up, tokens, d_model, d_ffn, beta_dx, beta_dw,
+                                    workspace, workspace_bytes, st);
 }
 }
