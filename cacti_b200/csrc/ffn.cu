@@ -14,13 +14,16 @@
 // Backward: one element-wise pass (dg, du), then one launch for all three products: its tiles are those of dx (contraction
 // over the gate part and then the up part, one accumulator, one rounding) followed by those of dWg and dWu.
 //
-// The tile walk is static: no global counter, so calls may overlap on any streams and graphs.
+// Calls may overlap on any streams and graphs: the forward's tile walk is static, the backward's draws its items from a
+// counter in the call's own workspace.  The backward's items differ in length (2 F and T deep), and their contractions are so long
+// that workers on a static walk drift apart and no longer share operand panels in L2: at 16384 x 3200 x 8640, sustained, the
+// static walk took 3.58 ms.
 #include "gemm_common.cuh"
 #include <utility>
 
 namespace cb {
 
-struct FfnMaps { CUtensorMap a[2], b[3], c[3]; };
+struct FfnMaps { CUtensorMap a[2], b[3], c[3], ak[2]; };
 
 // silu's sigmoid, f32 with the fast exponential and division: relative error below 2^-20 for |g| < 30, far below the 16-bit
 // rounding that follows; g = -inf gives s = 0.
@@ -321,7 +324,7 @@ static int ffn_fwd_run(uint64_t h, uint64_t gate, uint64_t up, uint64_t x, uint6
   rc = encode_operand(&maps.a[0], ox, 1, 1, 64, p.a_rows, bf16);
   if (!rc) rc = encode_operand(&maps.b[0], og, 1, 1, 64, half, bf16);
   if (!rc) rc = encode_operand(&maps.b[1], ou, 1, 1, 64, half, bf16);
-  maps.a[1] = maps.a[0]; maps.b[2] = maps.b[0];
+  maps.a[1] = maps.ak[0] = maps.ak[1] = maps.a[0]; maps.b[2] = maps.b[0];
   for (int i = 0; i < 3; ++i) {
     maps.c[i] = maps.a[0];
     const uint64_t ptr = i == 0 ? h : i == 1 ? gate : up;
@@ -351,7 +354,9 @@ static int ffn_fwd_run(uint64_t h, uint64_t gate, uint64_t up, uint64_t x, uint6
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
 ffn_adjoint_kernel(T* __restrict__ dG, T* __restrict__ dU, const T* __restrict__ dH, const T* __restrict__ G,
-                   const T* __restrict__ U, unsigned nvec, unsigned F, unsigned vpr /* vectors per padded row */) {
+                   const T* __restrict__ U, unsigned nvec, unsigned F, unsigned vpr /* vectors per padded row */,
+                   unsigned* __restrict__ next) {
+  if (blockIdx.x == 0 && threadIdx.x == 0) *next = 0;           // the item counter of the products that follow
   for (unsigned i = blockIdx.x * blockDim.x + threadIdx.x; i < nvec; i += gridDim.x * blockDim.x) {
     const unsigned row = i / vpr, c = (i - row * vpr) * 8;
     float g[8], u[8], d[8];
@@ -385,40 +390,13 @@ ffn_adjoint_kernel(T* __restrict__ dG, T* __restrict__ dU, const T* __restrict__
 
 // The products of the adjoint.  pr[0]: dx, contraction over `parts` = 2 operand pairs of nkb k-blocks, cut into `splits`
 // ranges; pr[1]: dWg and, `tiles` further on, dWu.
-struct FfnProduct { GemmParams g; int a_mn, nkb, tiles; };
+struct FfnProduct { GemmParams g; int nkb, tiles; };
 struct FfnBwdParams {
   FfnProduct pr[2];
   int splits;                    // ranges of dx's contraction; 1: none, else partial sums go to `part`
   float* part;                   // [splits][M][N] f32
   int nx, total;                 // items of dx (tiles * splits), all items
-  int light0, extra;             // see FfnWalk
-};
-
-// Static walk of worker w of W: the dx items w, w + W, ... first, which are the longest; workers that got one fewer (w >=
-// light0) then take `extra` weight-gradient tiles each, about as many as one dx item lasts, and the rest goes round.
-struct FfnWalk {
-  int w, W, pos, phase, end1;
-  __device__ __forceinline__ void init(const FfnBwdParams& p, int w_, int W_) {
-    w = w_; W = W_; pos = w; phase = 0;
-    const int n = p.extra * (W - p.light0), rest = p.total - p.nx;
-    end1 = p.nx + (n < rest ? n : rest);
-  }
-  __device__ __forceinline__ int next(const FfnBwdParams& p) {
-    int t;
-    if (phase == 0) {
-      if (pos < p.nx) { t = pos; pos += W; return t; }
-      phase = 1;
-      pos = p.nx + w - p.light0;
-      if (w < p.light0) pos = end1;
-    }
-    if (phase == 1) {
-      if (pos < end1) { t = pos; pos += W - p.light0; return t; }
-      phase = 2;
-      pos = end1 + (W - 1 - w);          // the ragged end falls to the workers that were light
-    }
-    if (pos < p.total) { t = pos; pos += W; return t; }
-    return -1;
-  }
+  unsigned* next;                // items drawn so far beyond the workers' first ones
 };
 
 struct FfnItem { int prod, part, tm, tn, kb0, kb1, split; };
@@ -473,7 +451,7 @@ __device__ __forceinline__ void ffn_partial_tile(float* __restrict__ part, int M
 }
 
 // The two-SM matmul kernel over the items of all three products.  A is dg / du, stored [tokens][Fp]: K-major for dx, MN-major
-// for the weight gradients, the same 64 x 64 boxes either way; B is MN-major throughout (weights [F][D], x [tokens][D]).
+// for the weight gradients; B is MN-major throughout (weights [F][D], x [tokens][D]).
 template <typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
 ffn_bwd_kernel(const __grid_constant__ FfnMaps maps, T* __restrict__ dX, T* __restrict__ dWg, T* __restrict__ dWu,
@@ -488,6 +466,7 @@ ffn_bwd_kernel(const __grid_constant__ FfnMaps maps, T* __restrict__ dX, T* __re
   uint64_t* tempty = tfull + 2;
   uint64_t* cbar = tempty + 2;                  // one per epilogue warp: old C boxes have arrived
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(cbar + 4);
+  SchedSmem* sched = reinterpret_cast<SchedSmem*>(tmem_slot + 4);
   unsigned char* cstage = tiles + (size_t)STAGES * STAGE_BYTES + 1024;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -497,6 +476,9 @@ ffn_bwd_kernel(const __grid_constant__ FfnMaps maps, T* __restrict__ dX, T* __re
     for (int s = 0; s < STAGES; ++s) { mbar_init(full + s, 1); mbar_init(empty + s, 1); }
     for (int a = 0; a < 2; ++a) { mbar_init(tfull + a, 1); mbar_init(tempty + a, 8); }
     for (int w = 0; w < 4; ++w) mbar_init(cbar + w, 1);
+    // schedule ring: in the leader read by the MMA thread and four epilogue warps (empty), in the peer by the producer
+    // thread and four epilogue warps, which report to the leader's empty_peer
+    for (int i = 0; i < kSchedDepth; ++i) { mbar_init(sched->full + i, 1); mbar_init(sched->empty + i, 5); mbar_init(sched->empty_peer + i, 5); }
     mbar_fence_init();
   }
   if (warp == 1) {
@@ -508,37 +490,59 @@ ffn_bwd_kernel(const __grid_constant__ FfnMaps maps, T* __restrict__ dX, T* __re
   cluster_sync_all();                           // the peer's barriers are initialised before anything signals them
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  FfnWalk walk;
-  walk.init(p, worker, nworkers);
+  // the leader's barriers on which the peer CTA's consumers report their reads of the schedule ring
+  const uint32_t leader_empty_peer0 = map_to_rank(smem_u32(sched->empty_peer), 0);
 
   if (warp == 0 && lane == 0) {
     // ---------------- TMA producer (both CTAs) ----------------
     int s = 0; unsigned ph = 0;
     bool ok = true;
-    for (int t = walk.next(p); ok && t >= 0; t = walk.next(p)) {
+    const uint32_t full0 = map_to_rank(smem_u32(full), 0);
+    unsigned sn = 0;
+    int t = worker, nxt = -1;                   // the grid never has more workers than items
+    for (;;) {
+      if (rank == 0) {
+        if (!sched_publish<true>(sched, sn, t)) { ok = false; break; }
+        if (t < 0) break;
+        const unsigned drawn = (unsigned)nworkers + atomicAdd(p.next, 1u);     // in flight while this item's loads are issued
+        nxt = drawn < (unsigned)p.total ? (int)drawn : -1;
+      } else {
+        t = sched_take<true>(sched, sn, true, leader_empty_peer0);
+        if (t < 0) { ok = t == -1; break; }
+      }
       const FfnItem it = ffn_item(p, t);
       const FfnProduct& pr = p.pr[it.prod];
       // a last column tile with at most 128 columns runs as an N = 128 MMA: each CTA then supplies 64 rows of B
       const int hb = (pr.g.N - it.tn * BN <= HB) ? HB / 2 : HB;
       const int m0 = it.tm * 256 + (int)rank * kBM, n0 = it.tn * BN + (int)rank * hb;
-      for (int kb = it.kb0; kb < it.kb1; ++kb) {
-        if (!mbar_wait_bounded(empty + s, ph ^ 1, kDevErrGemmTimeout)) { ok = false; break; }
-        unsigned char* sa = tiles + (size_t)s * STAGE_BYTES;
-        unsigned char* sb = sa + A_BYTES;
-        const uint32_t fb = map_to_rank(smem_u32(full + s), 0);
-        if (rank == 0) mbar_expect_tx(full + s, 2 * STAGE_BYTES);
-        const int part = it.prod ? it.part : (kb >= pr.nkb ? 1 : 0);
-        const int k0 = (it.prod ? kb : kb - part * pr.nkb) * kBK;
-        const CUtensorMap* ma = &maps.a[part];
-        const CUtensorMap* mb = it.prod ? &maps.b[2] : &maps.b[part];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (pr.a_mn) tma_load_4d_pair(sa + h * 8192, ma, fb, m0 + h * 64, k0, 0, 0);
-          else tma_load_4d_pair(sa + h * 8192, ma, fb, k0, m0 + h * 64, 0, 0);
-          tma_load_4d_pair(sb + h * 8192, mb, fb, n0 + h * 64, k0, 0, 0);
+      // one run of k-blocks of one operand pair (dx: the gate part, then the up part)
+      auto run = [&](auto a_mn, const CUtensorMap* ma, const CUtensorMap* mb, int kb0, int kb1) {
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait_bounded(empty + s, ph ^ 1, kDevErrGemmTimeout)) { ok = false; return; }
+          unsigned char* sa = tiles + (size_t)s * STAGE_BYTES;
+          unsigned char* sb = sa + A_BYTES;
+          const uint32_t fb = full0 + (uint32_t)s * 8u;
+          if (rank == 0) mbar_expect_tx(full + s, 2 * STAGE_BYTES);
+          if (a_mn) {
+            tma_load_4d_pair(sa, ma, fb, m0, kb * kBK, 0, 0);
+            tma_load_4d_pair(sa + 8192, ma, fb, m0 + 64, kb * kBK, 0, 0);
+          } else {
+            tma_load_4d_pair(sa, ma, fb, kb * kBK, m0, 0, 0);
+          }
+          tma_load_4d_pair(sb, mb, fb, n0, kb * kBK, 0, 0);
+          tma_load_4d_pair(sb + 8192, mb, fb, n0 + 64, kb * kBK, 0, 0);
+          if (++s == STAGES) { s = 0; ph ^= 1; }
         }
-        if (++s == STAGES) { s = 0; ph ^= 1; }
+      };
+      if (it.prod) {
+        run(std::true_type{}, &maps.a[it.part], &maps.b[2], it.kb0, it.kb1);
+      } else {
+        const int mid = it.kb1 < pr.nkb ? it.kb1 : pr.nkb;
+        run(std::false_type{}, &maps.ak[0], &maps.b[0], it.kb0, mid);
+        if (ok) run(std::false_type{}, &maps.ak[1], &maps.b[1], it.kb0 > pr.nkb ? it.kb0 - pr.nkb : 0, it.kb1 - pr.nkb);
       }
+      if (!ok) break;
+      t = nxt;
     }
     // the leader's last commits still arrive on this CTA's empty barriers: wait for them before leaving
     for (int i = 0; ok && i < STAGES; ++i) {
@@ -550,26 +554,35 @@ ffn_bwd_kernel(const __grid_constant__ FfnMaps maps, T* __restrict__ dX, T* __re
     int s = 0; unsigned ph = 0;
     int local = 0;
     bool ok = true;
-    for (int t = walk.next(p); ok && t >= 0; t = walk.next(p), ++local) {
+    const uint32_t sa0 = smem_u32(tiles);
+    const uint64_t desc_a[2] = {make_desc(sa0, 1, 64), make_desc(sa0, 512, 64)};      // K-major (dx), MN-major
+    const uint64_t desc_b = make_desc(sa0 + A_BYTES, 512, 64);
+    unsigned sn = 0;
+    for (;; ++local) {
+      const int t = sched_take<false>(sched, sn, true, 0);
+      if (t < 0) break;
       const FfnItem it = ffn_item(p, t);
       const FfnProduct& pr = p.pr[it.prod];
       const uint32_t idesc = (pr.g.N - it.tn * BN <= HB) ? idesc_with_n(pr.g.idesc, HB) : pr.g.idesc;      // see the producer
-      const uint32_t a_step = pr.a_mn ? 2048 : 32, a_lbo = pr.a_mn ? 512 : 1;
       const int acc = local & 1;
       if (!mbar_wait_bounded(tempty + acc, (unsigned)((local >> 1) & 1) ^ 1, kDevErrGemmTimeout)) break;
       tc_fence_after();
       const uint32_t tacc = tmem_base + (uint32_t)acc * BN;
-      for (int kb = it.kb0; kb < it.kb1; ++kb) {
-        if (!mbar_wait_bounded(full + s, ph, kDevErrGemmTimeout)) { ok = false; break; }
-        tc_fence_after();
-        const uint32_t sa = smem_u32(tiles + (size_t)s * STAGE_BYTES), sb = sa + A_BYTES;
+      auto run = [&](auto a_mn) {
+        for (int kb = it.kb0; kb < it.kb1; ++kb) {
+          if (!mbar_wait_bounded(full + s, ph, kDevErrGemmTimeout)) { ok = false; return; }
+          tc_fence_after();
+          // the address field of a descriptor counts 16 bytes: stages and k steps are additions to it
+          const uint64_t da = desc_a[a_mn ? 1 : 0] + (uint64_t)(s * (STAGE_BYTES / 16)), db = desc_b + (uint64_t)(s * (STAGE_BYTES / 16));
 #pragma unroll
-        for (int k4 = 0; k4 < kBK / 16; ++k4)
-          tc_mma_f16_pair(tacc, make_desc(sa + k4 * a_step, a_lbo, 64), make_desc(sb + k4 * 2048, 512, 64), idesc,
-                          (kb > it.kb0 || k4) ? 1u : 0u);
-        tc_commit_pair(empty + s);
-        if (++s == STAGES) { s = 0; ph ^= 1; }
-      }
+          for (int k4 = 0; k4 < kBK / 16; ++k4)
+            tc_mma_f16_pair(tacc, da + k4 * (a_mn ? 128 : 2), db + k4 * 128, idesc, (kb > it.kb0 || k4) ? 1u : 0u);
+          tc_commit_pair(empty + s);
+          if (++s == STAGES) { s = 0; ph ^= 1; }
+        }
+      };
+      if (it.prod) run(std::true_type{});
+      else run(std::false_type{});
       if (!ok) break;
       tc_commit_pair(tfull + acc);
     }
@@ -578,7 +591,10 @@ ffn_bwd_kernel(const __grid_constant__ FfnMaps maps, T* __restrict__ dX, T* __re
     const int q = warp & 3;
     int local = 0;
     unsigned cpar = 0;                          // phase of this warp's old-C barrier
-    for (int t = walk.next(p); t >= 0; t = walk.next(p), ++local) {
+    unsigned sn = 0;
+    for (;; ++local) {
+      const int t = rank == 0 ? sched_take_warp<false>(sched, sn, lane, 0) : sched_take_warp<true>(sched, sn, lane, leader_empty_peer0);
+      if (t < 0) break;
       const FfnItem it = ffn_item(p, t);
       const int acc = local & 1;
       if (!mbar_wait_bounded_warp(tfull + acc, (unsigned)((local >> 1) & 1), kDevErrGemmTimeout)) break;
@@ -654,7 +670,7 @@ static int ffn_result(FfnProduct& pr, CUtensorMap* map, uint64_t c, int64_t M, i
   const uint64_t all = c | (uint64_t)(N * 2);
   g.c_align = (all & 15) == 0 ? 16 : (all & 7) == 0 ? 8 : (all & 3) == 0 ? 4 : 2;
   g.group_m = g.tiles_m < 8 ? g.tiles_m : 8;
-  pr.a_mn = a_mn; pr.nkb = nkb; pr.tiles = g.tiles_m * g.tiles_n;
+  pr.nkb = nkb; pr.tiles = g.tiles_m * g.tiles_n;
   g.c_tma = (all & 15) == 0;
   return g.c_tma ? encode_operand(map, Operand{c, M, N, N, 0, 0, 0, 0}, 1, 1, 64, 32, bf16) : CACTI_B200_OK;
 }
@@ -665,29 +681,35 @@ static int ffn_bwd_run(uint64_t dx, uint64_t dwg, uint64_t dwu, uint64_t dh, uin
                        cudaStream_t st) {
   const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
   const FfnBwdPlan b = ffn_bwd_plan(tokens, D, F);
-  size_t off = 2 * b.dpart + b.part;
+  // workspace: item counter | dg | du | dx's partial sums | repacked operands
+  const uint64_t dg = ws + 256;
+  unsigned* counter = reinterpret_cast<unsigned*>(ws);
+  size_t off = 256 + 2 * b.dpart + b.part;
   if (!ws || (ws & 255) || ws_bytes < off) return CACTI_B200_ERR_WORKSPACE;
   Operand ox, og, ou;
   for (const auto& [ptr, rows] : {std::pair<uint64_t, int64_t>{x, tokens}, {wg, F}, {wu, F}}) {     // before anything is launched
     if (!ffn_rows_aligned(ptr, D)) off += packed_bytes(rows, D, 1);
   }
   if (ws_bytes < off) return CACTI_B200_ERR_WORKSPACE;
-  off = 2 * b.dpart + b.part;
+  off = 256 + 2 * b.dpart + b.part;
   const unsigned vpr = (unsigned)(b.Fp / 8), nvec = (unsigned)(tokens * vpr);
   const unsigned want = (nvec + 255) / 256, cap = kNumSMs * 32;
   const bool vec = ffn_rows_aligned(dh, F) && ffn_rows_aligned(gate, F) && ffn_rows_aligned(up, F);
   auto adj = vec ? ffn_adjoint_kernel<T, true> : ffn_adjoint_kernel<T, false>;
-  adj<<<want < cap ? want : cap, 256, 0, st>>>(reinterpret_cast<T*>(ws), reinterpret_cast<T*>(ws + b.dpart),
+  adj<<<want < cap ? want : cap, 256, 0, st>>>(reinterpret_cast<T*>(dg), reinterpret_cast<T*>(dg + b.dpart),
                                                reinterpret_cast<const T*>(dh), reinterpret_cast<const T*>(gate),
-                                               reinterpret_cast<const T*>(up), nvec, (unsigned)F, vpr);
+                                               reinterpret_cast<const T*>(up), nvec, (unsigned)F, vpr, counter);
   int rc = check_launch();
   if (!rc) rc = ffn_operand(ox, x, tokens, D, ws, ws_bytes, off, st);
   if (!rc) rc = ffn_operand(og, wg, F, D, ws, ws_bytes, off, st);
   if (!rc) rc = ffn_operand(ou, wu, F, D, ws, ws_bytes, off, st);
   if (rc) return rc;
   FfnMaps maps;
-  for (int i = 0; i < 2 && !rc; ++i)
-    rc = encode_operand(&maps.a[i], Operand{ws + i * b.dpart, tokens, b.Fp, b.Fp, 0, 0, 0, 0}, 1, 1, 64, 64, bf16);
+  for (int i = 0; i < 2 && !rc; ++i) {
+    const Operand o{dg + i * b.dpart, tokens, b.Fp, b.Fp, 0, 0, 0, 0};
+    rc = encode_operand(&maps.a[i], o, 1, 1, 64, 64, bf16);
+    if (!rc) rc = encode_operand(&maps.ak[i], o, 1, 1, 64, kBM, bf16);
+  }
   if (!rc) rc = encode_operand(&maps.b[0], og, 1, 1, 64, 64, bf16);
   if (!rc) rc = encode_operand(&maps.b[1], ou, 1, 1, 64, 64, bf16);
   if (!rc) rc = encode_operand(&maps.b[2], ox, 1, 1, 64, 64, bf16);
@@ -703,12 +725,10 @@ static int ffn_bwd_run(uint64_t dx, uint64_t dwg, uint64_t dwu, uint64_t dh, uin
   if (up_pr.g.c_align < p.pr[1].g.c_align) p.pr[1].g.c_align = up_pr.g.c_align;
   p.pr[1].g.c_tma &= up_pr.g.c_tma;
   p.splits = b.splits;
-  p.part = reinterpret_cast<float*>(ws + 2 * b.dpart);
+  p.part = reinterpret_cast<float*>(dg + 2 * b.dpart);
   p.nx = b.tiles_x * b.splits;
   p.total = p.nx + 2 * b.tiles_w;
-  p.light0 = p.nx % b.workers;
-  const int cx = 2 * b.nkb_x / b.splits;
-  p.extra = p.light0 ? (cx + b.nkb_w / 2) / b.nkb_w : 0;
+  p.next = counter;
   auto kern = ffn_bwd_kernel<T>;
   static bool attr_set[kMaxDevices] = {};
   ensure_dynamic_smem(kern, kFfnBwdSmem, attr_set);

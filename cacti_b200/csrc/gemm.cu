@@ -89,86 +89,9 @@ struct WorkIter {
 // kernel, of the peer CTA) through a ring of kSchedDepth entries in shared memory guarded by mbarriers; -1 ends the
 // walk.  The counter of a launch is g_tile_next[slot]; the last worker to finish (g_tile_done[slot]) puts both back
 // to zero for the next launch that uses the slot.
-constexpr int kSchedDepth = 4;
 __device__ unsigned g_tile_next[kSkSlots];
 __device__ unsigned g_tile_done[kSkSlots];
 
-struct SchedSmem {
-  uint64_t full[kSchedDepth];          // an entry has been published (1 arrival: the scheduling thread)
-  uint64_t empty[kSchedDepth];         // this CTA's consumers have read it
-  uint64_t empty_peer[kSchedDepth];    // two-SM kernel, leader only: the peer CTA's consumers have read theirs
-  int ring[kSchedDepth];
-};
-
-__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, unsigned parity) {   // acquire at cluster scope
-  unsigned ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity), "r"(g_mbar_suspend_ns) : "memory");
-  return ok != 0;
-}
-__device__ __forceinline__ bool mbar_wait_bounded_cluster(uint64_t* bar, unsigned parity, unsigned err_code) {
-  for (unsigned it = 0; it < kMbarPolls; ++it)
-    if (mbar_try_wait_cluster(bar, parity)) return true;
-  atomicMax(&g_dev_error, err_code);
-  return false;
-}
-// Consumer side of the ring for one thread (n: entries read so far).  Returns the tile, -1 at the end of the walk, -2
-// when the wait ran out.  `arrive`: this thread reports the read (one thread per consuming warp does).
-// CLUSTER: the entry was written by the other CTA of the pair, and the read is reported to that CTA's barrier.
-template <bool CLUSTER>
-__device__ __forceinline__ int sched_take(SchedSmem* sm, unsigned& n, bool arrive, uint32_t leader_empty_peer0) {
-  const int sl = (int)(n % kSchedDepth);
-  const unsigned ph = (n / kSchedDepth) & 1u;
-  const bool ok = CLUSTER ? mbar_wait_bounded_cluster(sm->full + sl, ph, kDevErrGemmTimeout)
-                          : mbar_wait_bounded(sm->full + sl, ph, kDevErrGemmTimeout);
-  if (!ok) return -2;
-  const int tile = *reinterpret_cast<volatile int*>(&sm->ring[sl]);
-  if (arrive) {
-    if (CLUSTER) mbar_arrive_cluster(leader_empty_peer0 + (uint32_t)sl * 8u);
-    else mbar_arrive(sm->empty + sl);
-  }
-  ++n;
-  return tile;
-}
-// The same for a whole warp (all lanes get the tile; lane 0 reports the read after every lane has it).
-template <bool CLUSTER>
-__device__ __forceinline__ int sched_take_warp(SchedSmem* sm, unsigned& n, int lane, uint32_t leader_empty_peer0) {
-  const int sl = (int)(n % kSchedDepth);
-  const unsigned ph = (n / kSchedDepth) & 1u;
-  const bool ok = CLUSTER ? mbar_wait_bounded_cluster(sm->full + sl, ph, kDevErrGemmTimeout)
-                          : mbar_wait_bounded(sm->full + sl, ph, kDevErrGemmTimeout);
-  if (!__all_sync(0xffffffffu, ok)) return -2;
-  const int tile = *reinterpret_cast<volatile int*>(&sm->ring[sl]);
-  __syncwarp();
-  if (lane == 0) {
-    if (CLUSTER) mbar_arrive_cluster(leader_empty_peer0 + (uint32_t)sl * 8u);
-    else mbar_arrive(sm->empty + sl);
-  }
-  ++n;
-  return tile;
-}
-// Scheduling thread: publish `tile` (or -1) as entry n.  PAIR: also into the peer CTA's ring.
-template <bool PAIR>
-__device__ __forceinline__ bool sched_publish(SchedSmem* sm, unsigned& n, int tile) {
-  const int sl = (int)(n % kSchedDepth);
-  const unsigned ph = (n / kSchedDepth) & 1u;
-  if (!mbar_wait_bounded(sm->empty + sl, ph ^ 1u, kDevErrGemmTimeout)) return false;
-  if (PAIR && !mbar_wait_bounded_cluster(sm->empty_peer + sl, ph ^ 1u, kDevErrGemmTimeout)) return false;
-  sm->ring[sl] = tile;
-  mbar_arrive(sm->full + sl);                                  // release: the entry is visible to who sees the arrival
-  if (PAIR) {
-    uint32_t peer_ring, peer_full;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer_ring) : "r"(smem_u32(&sm->ring[sl])), "r"(1u));
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer_full) : "r"(smem_u32(sm->full + sl)), "r"(1u));
-    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_ring), "r"((uint32_t)tile) : "memory");
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(peer_full) : "memory");
-  }
-  ++n;
-  return true;
-}
 // Next tile for the scheduling thread: workers' first tiles are their own indices, the rest come from the counter.
 __device__ __forceinline__ long long sched_draw(int slot, long long nworkers, long long total) {
   const long long t = nworkers + (long long)atomicAdd(&g_tile_next[slot], 1u);
