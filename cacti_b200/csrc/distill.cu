@@ -47,110 +47,462 @@ __device__ __forceinline__ int teacher_index(const DistillParams& p, int64_t i) 
   return v < p.vocab ? v : (v == 65535 ? -1 : -2);
 }
 
-__device__ __forceinline__ double block_sum_f64(double v, double* smem) {
+// ---- layout of a row in 16-byte vectors ---------------------------------------------------------------------------
+// A row may start at any element address.  Its vectors are those of memory: vector v covers the 16 bytes at (address rounded
+// down) + 16 v, its element e is row element v VEC + e - head.  The first and the last vector may hold elements of the
+// neighbouring rows ("foreign"); they are never the first bytes before, or the last after, the whole tensor: there the vector is
+// fetched element by element.
+template <typename T> struct RowVecs {
+  const unsigned char* base;     // address of vector 0
+  int head;                      // foreign elements at the start of vector 0
+  int nvec;
+  __device__ __forceinline__ RowVecs(const T* row, int V) {
+    const uint64_t a = reinterpret_cast<uint64_t>(row);
+    base = reinterpret_cast<const unsigned char*>(a & ~15ull);
+    head = (int)(a & 15) / (int)sizeof(T);
+    nvec = (head + V + Elem<T>::VEC - 1) / Elem<T>::VEC;
+  }
+};
+
+__device__ __forceinline__ double warp_sum_f64(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  const int w = threadIdx.x >> 5, nw = blockDim.x >> 5;
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) smem[w] = v;
-  __syncthreads();
-  double r = 0.;
-  for (int i = 0; i < nw; ++i) r += smem[i];
-  return r;
+  return v;
 }
 
-// One CTA a row, the row read three times from memory (the later times from L2).  Thread t < k owns slot t of the list; a
-// bitmap in shared memory says which positions are listed.
-template <typename T, bool BWD>
-__global__ void __launch_bounds__(kDistillThreads)
-distill_rows_kernel(T* __restrict__ dL, const T* __restrict__ L, const DistillParams p) {
-  extern __shared__ unsigned bitmap[];
-  __shared__ int s_idx[kDistillMaxK];
-  __shared__ float s_red[33];
-  __shared__ double s_redd[32];
-  const int words = (p.vocab + 31) / 32, V = p.vocab;
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    const float w = p.w_rows ? p.w_rows[row] : p.w_scalar;
-    const T* x = L + row * V;
-    T* d = BWD ? dL + row * V : nullptr;
-    if (w == 0.f) {                                             // not read: loss 0, gradient 0
-      if (threadIdx.x == 0 && p.loss_rows) p.loss_rows[row] = 0.f;
-      if (BWD && !p.beta) for (int j = threadIdx.x; j < V; j += blockDim.x) d[j] = Elem<T>::from_f32(0.f);
-      continue;
-    }
-    for (int i = threadIdx.x; i < words; i += blockDim.x) bitmap[i] = 0u;
-    const int t = threadIdx.x;
-    int idx = t < p.k ? teacher_index(p, row * p.k + t) : -1;
-    if (t < kDistillMaxK) s_idx[t] = idx;
-    __syncthreads();
-    bool bad = idx == -2;
-    if (idx >= 0) for (int j = 0; j < t; ++j) if (s_idx[j] == idx) { bad = true; break; }
-    if (bad) idx = -1;
-    const bool row_bad = __syncthreads_or(bad) != 0;
-    double zs = -INFINITY;
-    float xk = 0.f;
-    if (idx >= 0) {
-      zs = p.inv_temp * teacher_value(p, row * p.k + t);
-      xk = Elem<T>::to_f32(x[idx]);
-      atomicOr(bitmap + (idx >> 5), 1u << (idx & 31));
-    }
-    // the list's probabilities
-    double pk = 0., lse_t;
-    if (p.t_lse) {
-      lse_t = (double)p.t_lse[row];
-    } else {
-      double zm = zs;                                           // maximum: through the float reduction would round it
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) { const double v = __shfl_xor_sync(0xffffffffu, zm, o); zm = v > zm || v != v ? v : zm; }
-      __syncthreads();
-      if ((t & 31) == 0) s_redd[t >> 5] = zm;
-      __syncthreads();
-      for (int i = 0; i < (int)(blockDim.x >> 5); ++i) zm = s_redd[i] > zm || s_redd[i] != s_redd[i] ? s_redd[i] : zm;
-      lse_t = zm + log(block_sum_f64(zs == -INFINITY ? 0. : exp(zs - zm), s_redd));
-    }
-    if (zs != -INFINITY) pk = exp(zs - lse_t);
-    const double psum = block_sum_f64(pk, s_redd);
-    const double ent = block_sum_f64(pk != 0. ? pk * (zs - lse_t) : 0., s_redd);
-    const int listed = (int)block_sum_f64(idx >= 0 ? 1. : 0., s_redd);
-    // the student's row: maximum, then the sums over listed and unlisted positions
-    float m = -INFINITY;
-    for (int j = t; j < V; j += blockDim.x) m = fmaxf(m, Elem<T>::to_f32(x[j]));
-    m = block_reduce<MaxOp>(m, s_red);
-    // differences to the maximum, so that a row of values like the type's lowest loses nothing
-    const double px = block_sum_f64(pk != 0. ? pk * ((double)xk - (double)m) : 0., s_redd);
-    const float c = (float)(p.inv_temp * 1.4426950408889634);    // exponentials are 2^((x - m) c)
-    float zr = 0.f;
-    for (int j = t; j < V; j += blockDim.x)
-      if (!((bitmap[j >> 5] >> (j & 31)) & 1u)) zr += exp2f_approx((Elem<T>::to_f32(x[j]) - m) * c);
-    const float ek = idx >= 0 ? exp2f_approx((xk - m) * c) : 0.f;
-    const double rest = block_sum_f64((double)zr, s_redd), all = rest + block_sum_f64((double)ek, s_redd);
-    double r = p.t_lse && listed && listed < V ? 1. - psum : 0.;
-    if (r < 0.) r = 0.;
-    const double mass = psum + r;
-    if (t == 0) {
-      if (row_bad && p.status) atomicMax(p.status, (unsigned)CACTI_B200_ERR_INDEX_RANGE);
-      if (p.loss_rows) {
-        double loss = mass != 0. ? ent - p.inv_temp * px + psum * log(all) : 0.;
-        if (r > 0.) loss += r * (log(r) - log(rest) + log(all));
-        p.loss_rows[row] = row_bad ? __int_as_float(0x7fc00000) : (float)loss;
-      }
-    }
-    if (BWD) {
-      const double wc = (double)w * p.inv_temp;
-      const float g_all = mass != 0. ? (float)(wc * mass / all) : 0.f;
-      const float g_rest = mass != 0. ? (float)(wc * (mass / all - (r > 0. && rest > 0. ? r / rest : 0.))) : 0.f;
-      for (int j = t; j < V; j += blockDim.x) {
-        if ((bitmap[j >> 5] >> (j & 31)) & 1u) continue;
-        const float v = exp2f_approx((Elem<T>::to_f32(x[j]) - m) * c) * g_rest;
-        d[j] = p.beta ? Elem<T>::from_f32(Elem<T>::to_f32(d[j]) + round_to<T>(v)) : Elem<T>::from_f32(v);
-      }
-      if (idx >= 0) {
-        const float v = ek * g_all - (float)(wc * pk);
-        d[idx] = p.beta ? Elem<T>::from_f32(Elem<T>::to_f32(d[idx]) + round_to<T>(v)) : Elem<T>::from_f32(v);
-      }
-    }
-    __syncthreads();
+// Roles of a CTA (a cluster of C CTAs shares a row, each a run of its vectors):
+//   list warps, one per ring slot: fetch the slot's row (bulk copy), turn the teacher's list into probabilities (f64), take the
+//     listed student logits out of the staged row (they become -inf there), and, when the row is done, write the listed positions'
+//     gradient and the loss;
+//   MW main warps: maximum and exponentials of the unlisted positions in registers (one pass over shared memory), one
+//     combination of (maximum, sum) over the CTA and the cluster, then gradient = exponential times a factor, stored from
+//     registers.  The slot is free for the next row as soon as the exponentials are taken.
+constexpr int kDistillNV = 8;                                  // vectors a main thread holds
+constexpr int kDistillMaxC = 8;
+struct DistillRow {              // from the list warp to the main warps
+  float m_top, z_top;            // maximum of the listed logits (of this CTA's vectors) and sum of their exponentials
+  float g_mass, g_r;             // w c P and w c r
+  int skip;                      // weight 0
+};
+struct DistillFin { float m, z_all, z_rest; };                 // back to the list warp
+struct DistillRec { float m, z_rest, m_top, z_top; };          // a CTA's part of a row, to the cluster
+
+template <int MW, int R> struct DistillSmem {
+  uint64_t full[R], marked[R], consumed[R], stored[R];
+  uint64_t rec_bar[2];
+  DistillRec rec[2][kDistillMaxC];
+  float2 red[2][MW];
+  DistillRow row[R];
+  DistillFin fin[R];
+  alignas(16) int idx[R][kDistillMaxK];
+};
+
+__device__ __forceinline__ uint32_t distill_ctarank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ uint32_t distill_nctas() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void distill_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool distill_wait_cluster(uint64_t* bar, unsigned parity) {
+  for (unsigned it = 0; it < kMbarPolls; ++it) {
+    unsigned ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity), "r"(g_mbar_suspend_ns) : "memory");
+    if (ok) return true;
   }
+  atomicMax(&g_dev_error, kDevErrStageTimeout);
+  return false;
+}
+
+// 2^((x - m) c); m is finite or the result is meant to be NaN
+__device__ __forceinline__ float exp_rel(float x, float m, float c) { return exp2f_approx((x - m) * c); }
+
+// One vector of gradient values to memory; foreign elements are left out.
+template <typename T>
+__device__ __forceinline__ void distill_store(T* __restrict__ drow, int v, int head, int V, bool vec_ok, int beta, const float (&d)[Elem<T>::VEC]) {
+  constexpr int VEC = Elem<T>::VEC;
+  const int j0 = v * VEC - head;
+  if (vec_ok && j0 >= 0 && j0 + VEC <= V) {
+    if (beta) st_stream(drow + j0, pack_accumulate<T>(d, ld_stream(drow + j0)));
+    else st_stream(drow + j0, pack<T>(d));
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      if (j0 + e >= 0 && j0 + e < V) {
+        T* o = drow + j0 + e;
+        *o = beta ? Elem<T>::from_f32(Elem<T>::to_f32(*o) + round_to<T>(d[e])) : Elem<T>::from_f32(d[e]);
+      }
+    }
+  }
+}
+
+// HOLD: a CTA's part of a row is at most MW * 32 * kDistillNV vectors and its exponentials stay in registers; otherwise they are
+// formed again for the gradient (parts above 64 KB: f32 rows beyond 131072).
+template <typename T, int MW, int R, bool HOLD, bool BWD>
+__global__ void __launch_bounds__((MW + R) * 32)
+distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constant__ DistillParams p, unsigned slot_bytes) {
+  constexpr int VEC = Elem<T>::VEC, MT = MW * 32;
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  using Smem = DistillSmem<MW, R>;
+  Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
+  unsigned char* ring = smem_raw + (sizeof(Smem) + 127) / 128 * 128;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, V = p.vocab;
+  const int C = (int)distill_nctas(), rank = (int)distill_ctarank();
+  const int64_t row0 = blockIdx.x / C, stride = gridDim.x / C;
+  const float c = (float)(p.inv_temp * 1.4426950408889634);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < R; ++s) { mbar_init(sm.full + s, 1); mbar_init(sm.marked + s, 1); mbar_init(sm.consumed + s, MW); mbar_init(sm.stored + s, MW); }
+    for (int i = 0; i < 2; ++i) mbar_init(sm.rec_bar + i, C);
+    mbar_fence_init();
+  }
+  __syncthreads();
+  if (C > 1) asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+
+  if (warp >= MW) {
+    // ---------------- list warp of slot s ----------------
+    const int s = warp - MW;
+    unsigned char* buf = ring + (size_t)s * slot_bytes;
+    T* sx = reinterpret_cast<T*>(buf);
+    unsigned ph = 0;
+    bool ok = true;
+    const uint64_t t_begin = reinterpret_cast<uint64_t>(L), t_end = t_begin + (uint64_t)p.rows * V * sizeof(T);
+    float w_row = 0.f;
+    // fetch a row's vectors of this CTA; whole vectors inside the tensor only
+    auto issue = [&](int64_t row) {
+      w_row = p.w_rows ? p.w_rows[row] : p.w_scalar;
+      if (lane == 0 && w_row != 0.f) {
+        const RowVecs<T> rv(L + row * V, V);
+        const int v0 = (int)((int64_t)rv.nvec * rank / C), v1 = (int)((int64_t)rv.nvec * (rank + 1) / C);
+        const unsigned char *a = rv.base + (size_t)v0 * 16, *b = rv.base + (size_t)v1 * 16;
+        unsigned skip = 0;
+        if (reinterpret_cast<uint64_t>(a) < t_begin) { a += 16; skip = 16; }
+        if (reinterpret_cast<uint64_t>(b) > t_end) b -= 16;
+        const unsigned bytes = b > a ? (unsigned)(b - a) : 0u;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_expect_tx(sm.full + s, bytes);
+        if (bytes) bulk_g2s(buf + skip, a, bytes, sm.full + s);
+      }
+    };
+    int64_t row = row0 + s * stride;
+    if (row < p.rows) issue(row);
+    unsigned full_ph = 0;                                       // rows of weight 0 do not pass through `full`
+    for (; row < p.rows; row += (int64_t)R * stride) {
+      const float w = w_row;
+      const bool skip = w == 0.f;
+      const RowVecs<T> rv(L + row * V, V);
+      const int v0 = (int)((int64_t)rv.nvec * rank / C), v1 = (int)((int64_t)rv.nvec * (rank + 1) / C);
+      const int jlo = v0 * VEC - rv.head, jhi = v1 * VEC - rv.head;          // row elements of this CTA: [jlo, jhi)
+      int idx[kDistillMaxK / 32];
+      double pk[kDistillMaxK / 32];
+      float xk[kDistillMaxK / 32];
+      double psum = 0., ent = 0., r = 0.;
+      bool row_bad = false;
+      if (!skip) {
+        // ---- the list: indices, validity ----
+        double zs[kDistillMaxK / 32];
+#pragma unroll
+        for (int i = 0; i < kDistillMaxK / 32; ++i) {
+          const int k = i * 32 + lane;
+          idx[i] = -1; zs[i] = 0.;
+          if (i * 32 < p.k) {
+            if (k < p.k) {
+              idx[i] = teacher_index(p, row * p.k + k);
+              zs[i] = p.inv_temp * teacher_value(p, row * p.k + k);
+            }
+            sm.idx[s][k] = idx[i];
+          }
+        }
+        const double tl = p.t_lse ? (double)p.t_lse[row] : 0.;
+        __syncwarp();
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < kDistillMaxK / 32; ++i) bad |= idx[i] == -2;
+        unsigned dup = 0;
+#pragma unroll
+        for (int i0 = 0; i0 < kDistillMaxK / 32; ++i0) {
+          if (i0 * 32 < p.k) {
+            for (int q = 0; q < 8; ++q) {                       // slots i0 * 32 + 4 q ... + 3 against this lane's later ones
+              const int4 o = *reinterpret_cast<const int4*>(&sm.idx[s][i0 * 32 + q * 4]);
+#pragma unroll
+              for (int i = i0; i < kDistillMaxK / 32; ++i) {
+                if (i * 32 < p.k) {
+                  const int lim = i == i0 ? lane - q * 4 : 4;   // of these four, those before this slot
+                  const bool hit = (o.x == idx[i] && lim > 0) || (o.y == idx[i] && lim > 1) || (o.z == idx[i] && lim > 2) || (o.w == idx[i] && lim > 3);
+                  dup |= (hit && idx[i] >= 0 ? 1u : 0u) << i;
+                }
+              }
+            }
+          }
+        }
+        bad |= dup != 0;
+        row_bad = __any_sync(0xffffffffu, bad);
+        // ---- its probabilities ----
+        double zm = -INFINITY;
+        int cnt = 0;
+#pragma unroll
+        for (int i = 0; i < kDistillMaxK / 32; ++i) {
+          if (idx[i] < 0 || ((dup >> i) & 1u)) { idx[i] = -1; zs[i] = -INFINITY; }
+          else ++cnt;
+          zm = zs[i] > zm || zs[i] != zs[i] ? zs[i] : zm;
+        }
+        double lse_t = tl;
+        if (!p.t_lse) {
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) { const double v = __shfl_xor_sync(0xffffffffu, zm, o); zm = v > zm || v != v ? v : zm; }
+          double e = 0.;
+#pragma unroll
+          for (int i = 0; i < kDistillMaxK / 32; ++i)
+            if (i * 32 < p.k && zs[i] != -INFINITY) e += exp(zs[i] - zm);
+          lse_t = zm + log(warp_sum_f64(e));
+        }
+#pragma unroll
+        for (int i = 0; i < kDistillMaxK / 32; ++i) {
+          pk[i] = 0.;
+          if (i * 32 < p.k && zs[i] != -INFINITY) {
+            pk[i] = exp(zs[i] - lse_t);
+            psum += pk[i];
+            if (pk[i] != 0.) ent += pk[i] * (zs[i] - lse_t);
+          }
+        }
+        psum = warp_sum_f64(psum);
+        ent = warp_sum_f64(ent);
+        cnt = __reduce_add_sync(0xffffffffu, cnt);
+        if (p.t_lse && cnt && cnt < V) r = fmax(0., 1. - psum);
+        // ---- the listed logits out of the staged row ----
+        ok = mbar_wait_bounded_warp(sm.full + s, full_ph, kDevErrStageTimeout);
+        full_ph ^= 1u;
+        if (!ok) break;
+        if (lane < VEC) {
+          // foreign elements, and edge vectors that were not copied because they reach outside the tensor
+          for (int side = 0; side < 2; ++side) {
+            const int v = side ? v1 - 1 : v0;
+            if (v < v0 || v >= v1 || (side && v == v0)) continue;
+            const unsigned char* a = rv.base + (size_t)v * 16;
+            const int j = v * VEC - rv.head + lane;
+            const bool in = j >= 0 && j < V;
+            const bool outside = reinterpret_cast<uint64_t>(a) < t_begin || reinterpret_cast<uint64_t>(a) + 16 > t_end;
+            if (!in) sx[(v - v0) * VEC + lane] = Elem<T>::from_f32(-INFINITY);
+            else if (outside) sx[(v - v0) * VEC + lane] = L[row * V + j];
+          }
+        }
+        __syncwarp();
+        float mt = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kDistillMaxK / 32; ++i) {
+          xk[i] = -INFINITY;
+          if (idx[i] >= jlo && idx[i] < jhi && idx[i] >= 0) {
+            T* at = sx + (idx[i] - jlo);
+            xk[i] = Elem<T>::to_f32(*at);
+            *at = Elem<T>::from_f32(-INFINITY);
+          } else {
+            idx[i] = -1;                                        // another CTA's
+          }
+          mt = fmaxf(mt, xk[i]);
+        }
+        mt = warp_reduce<MaxOp>(mt);
+        const float ref = mt == -INFINITY ? 0.f : mt;
+        float zt = 0.f;
+#pragma unroll
+        for (int i = 0; i < kDistillMaxK / 32; ++i) if (idx[i] >= 0) zt += exp_rel(xk[i], ref, c);
+        zt = warp_reduce<SumOp>(zt);
+        if (lane == 0) {
+          const double wc = (double)w * p.inv_temp;
+          sm.row[s] = DistillRow{mt, zt, (float)(wc * (psum + r)), (float)(wc * r), 0};
+        }
+      } else if (lane == 0) {
+        sm.row[s] = DistillRow{0.f, 0.f, 0.f, 0.f, 1};
+      }
+      __syncwarp();
+      if (lane == 0) distill_arrive(sm.marked + s);
+      // ---- the slot is free once the main warps have taken its exponentials: next row ----
+      ok = mbar_wait_bounded_warp(sm.consumed + s, ph, kDevErrStageTimeout);
+      if (!ok) break;
+      if (row + (int64_t)R * stride < p.rows) issue(row + (int64_t)R * stride);
+      // ---- the row is done: listed positions and loss ----
+      ok = mbar_wait_bounded_warp(sm.stored + s, ph, kDevErrStageTimeout);
+      ph ^= 1u;
+      if (!ok) break;
+      if (skip) {
+        if (lane == 0 && rank == 0 && p.loss_rows) p.loss_rows[row] = 0.f;
+        continue;
+      }
+      const DistillFin f = sm.fin[s];
+      const double mass = psum + r;
+      if (BWD) {
+        const double wc = (double)w * p.inv_temp;
+        const float ga = mass != 0. ? (float)(wc * mass / (double)f.z_all) : 0.f;
+        const float ref = f.m == -INFINITY ? 0.f : f.m;
+#pragma unroll
+        for (int i = 0; i < kDistillMaxK / 32; ++i) {
+          if (idx[i] >= 0) {
+            const float v = exp_rel(xk[i], ref, c) * ga - (float)(wc * pk[i]);
+            T* o = dL + row * V + idx[i];
+            *o = p.beta ? Elem<T>::from_f32(Elem<T>::to_f32(*o) + round_to<T>(v)) : Elem<T>::from_f32(v);
+          }
+        }
+      }
+      if (p.loss_rows) {
+        // sum p (x_k - m): differences to the maximum, so that a row of values like the type's lowest loses nothing.
+        // Every CTA of a cluster adds its own listed positions: the first one finds the others' in global memory.
+        double px = 0.;
+#pragma unroll
+        for (int i = 0; i < kDistillMaxK / 32; ++i) {
+          if (i * 32 < p.k && pk[i] != 0.) {
+            float x = xk[i];
+            if (C > 1 && rank == 0 && idx[i] < 0) {
+              const int j = teacher_index(p, row * p.k + i * 32 + lane);
+              x = Elem<T>::to_f32(L[row * V + j]);
+            }
+            px += pk[i] * ((double)x - (double)f.m);
+          }
+        }
+        px = warp_sum_f64(px);
+        if (lane == 0 && rank == 0) {
+          const double la = log((double)f.z_all);
+          double loss = mass != 0. ? ent - p.inv_temp * px + psum * la : 0.;
+          if (r > 0.) loss += r * (log(r) - log((double)f.z_rest) + la);
+          p.loss_rows[row] = row_bad ? __int_as_float(0x7fc00000) : (float)loss;
+        }
+      }
+      if (lane == 0 && rank == 0 && row_bad && p.status) atomicMax(p.status, (unsigned)CACTI_B200_ERR_INDEX_RANGE);
+    }
+  } else {
+    // ---------------- main warps ----------------
+    const int t = threadIdx.x;
+    int s = 0;
+    unsigned ph = 0, par = 0, rph[2] = {0, 0};
+    for (int64_t row = row0; row < p.rows; row += stride, par ^= 1u) {
+      // a wait that ran out is agreed on at the CTA's barrier below; until then the warp goes on with what is there
+      bool gave_up = !mbar_wait_bounded_warp(sm.marked + s, ph, kDevErrStageTimeout);
+      const DistillRow info = sm.row[s];
+      const RowVecs<T> rv(L + row * V, V);
+      const int v0 = (int)((int64_t)rv.nvec * rank / C), n = (int)((int64_t)rv.nvec * (rank + 1) / C) - v0;
+      T* drow = BWD ? dL + row * V : nullptr;
+      const bool vec_ok = BWD && ((reinterpret_cast<uint64_t>(drow) ^ reinterpret_cast<uint64_t>(L + row * V)) & 15) == 0;
+      if (info.skip) {
+        if (BWD && !p.beta) {
+          const float z[VEC] = {};
+          for (int v = t; v < n; v += MT) distill_store<T>(drow, v0 + v, rv.head, V, vec_ok, 0, z);
+        }
+        if (lane == 0) { distill_arrive(sm.consumed + s); distill_arrive(sm.stored + s); }
+        if (++s == R) { s = 0; ph ^= 1u; }
+        par ^= 1u;                                              // nothing exchanged
+        if (gave_up) break;
+        continue;
+      }
+      const uint4* srow = reinterpret_cast<const uint4*>(ring + (size_t)s * slot_bytes);
+      // maximum and exponentials against the warp's own maximum
+      constexpr int NV = HOLD ? kDistillNV : 1;
+      float a[NV][VEC];
+      float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, zq[4] = {0.f, 0.f, 0.f, 0.f};
+      float mw, ref;
+      if (HOLD) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+          if (t + k * MT < n) {
+            unpack<T>(srow[t + k * MT], a[k]);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) mq[e & 3] = fmaxf(mq[e & 3], a[k][e]);
+          }
+        }
+        mw = warp_reduce<MaxOp>(fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])));
+        ref = mw == -INFINITY ? 0.f : mw;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+          if (t + k * MT < n) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) { a[k][e] = exp_rel(a[k][e], ref, c); zq[e & 3] += a[k][e]; }
+          }
+        }
+        if (lane == 0) distill_arrive(sm.consumed + s);         // (the warp reduction below orders the reads before it)
+      } else {
+        for (int v = t; v < n; v += MT) {
+          unpack<T>(srow[v], a[0]);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) mq[e & 3] = fmaxf(mq[e & 3], a[0][e]);
+        }
+        mw = warp_reduce<MaxOp>(fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])));
+        ref = mw == -INFINITY ? 0.f : mw;
+        for (int v = t; v < n; v += MT) {
+          unpack<T>(srow[v], a[0]);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) zq[e & 3] += exp_rel(a[0][e], ref, c);
+        }
+      }
+      const float zw = warp_reduce<SumOp>((zq[0] + zq[1]) + (zq[2] + zq[3]));
+      if (lane == 0) sm.red[par][warp] = make_float2(mw, zw);
+      unsigned any;
+      asm volatile(
+          "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %2, 0;\n\tbar.red.or.pred p, 1, %1, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(any) : "n"(MT), "r"((unsigned)gave_up) : "memory");
+      if (any) break;
+      float2 rd = lane < MW ? sm.red[par][lane] : make_float2(-INFINITY, 0.f);
+      float m = warp_reduce<MaxOp>(rd.x);
+      float mr = m == -INFINITY ? 0.f : m;
+      float z_rest = warp_reduce<SumOp>(rd.y * exp_rel(rd.x, mr, c));
+      float m_top = info.m_top, z_top = info.z_top;
+      if (C > 1) {
+        // every CTA hands its part to all of the cluster; the parts are combined in rank order everywhere
+        if (warp == 0 && lane < C) {
+          const DistillRec mine{m, z_rest, m_top, z_top};
+          uint32_t dst, bar;
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(dst) : "r"(smem_u32(&sm.rec[par][rank])), "r"(lane));
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(smem_u32(&sm.rec_bar[par])), "r"(lane));
+          asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "f"(mine.m), "f"(mine.z_rest), "f"(mine.m_top), "f"(mine.z_top) : "memory");
+          asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+        }
+        gave_up = !__all_sync(0xffffffffu, distill_wait_cluster(sm.rec_bar + par, rph[par]));
+        rph[par] ^= 1u;
+        const DistillRec o = lane < C ? sm.rec[par][lane] : DistillRec{-INFINITY, 0.f, -INFINITY, 0.f};
+        m = warp_reduce<MaxOp>(o.m);
+        mr = m == -INFINITY ? 0.f : m;
+        z_rest = warp_reduce<SumOp>(o.z_rest * exp_rel(o.m, mr, c));
+        m_top = warp_reduce<MaxOp>(o.m_top);
+        const float tr = m_top == -INFINITY ? 0.f : m_top;
+        z_top = warp_reduce<SumOp>(o.z_top * exp_rel(o.m_top, tr, c));
+      }
+      // against the maximum of the whole row, listed positions included
+      const float mall = fmaxf(m, m_top), mref = mall == -INFINITY ? 0.f : mall;
+      z_rest *= exp_rel(m, mref, c);
+      const float z_all = z_rest + z_top * exp_rel(m_top, mref, c);
+      if (t == 0) sm.fin[s] = DistillFin{mall, z_all, z_rest};
+      if (BWD) {
+        // (P / E - r / E_rest) e, with e formed against the warp's maximum
+        const float g = info.g_mass != 0.f ? info.g_mass / z_all - (info.g_r != 0.f && z_rest > 0.f ? info.g_r / z_rest : 0.f) : 0.f;
+        if (HOLD) {
+          // a warp whose part is all -inf has no reference: its exponentials are 0
+          const float f = mw == -INFINITY && mall != -INFINITY ? g * 0.f : g * exp_rel(ref, mref, c);
+#pragma unroll
+          for (int k = 0; k < NV; ++k) {
+            if (t + k * MT < n) {
+#pragma unroll
+              for (int e = 0; e < VEC; ++e) a[k][e] *= f;
+              distill_store<T>(drow, v0 + t + k * MT, rv.head, V, vec_ok, p.beta, a[k]);
+            }
+          }
+        } else {
+          for (int v = t; v < n; v += MT) {
+            unpack<T>(srow[v], a[0]);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) a[0][e] = exp_rel(a[0][e], mref, c) * g;
+            distill_store<T>(drow, v0 + v, rv.head, V, vec_ok, p.beta, a[0]);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) {
+        if (!HOLD) distill_arrive(sm.consumed + s);
+        distill_arrive(sm.stored + s);
+      }
+      if (++s == R) { s = 0; ph ^= 1u; }
+      if (gave_up) break;
+    }
+  }
+  __syncwarp();
+  // no CTA leaves while another may still write into its records
+  if (C > 1) asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
 // loss_sum = sum_i w_i loss_i in a fixed order: 1024 strided partial sums, then a tree.  Rows of weight 0 add nothing.
@@ -170,16 +522,54 @@ distill_loss_sum_kernel(float* __restrict__ loss_sum, const float* __restrict__ 
   if (threadIdx.x == 0) *loss_sum = (float)sm[0];
 }
 
+template <typename T, int MW, int R, bool HOLD>
+static int launch_distill_as(uint64_t dl, uint64_t l, const DistillParams& p, int C, unsigned slot_bytes, cudaStream_t st) {
+  const size_t smem = (sizeof(DistillSmem<MW, R>) + 127) / 128 * 128 + (size_t)R * slot_bytes;
+  auto kern = dl ? distill_kernel<T, MW, R, HOLD, true> : distill_kernel<T, MW, R, HOLD, false>;
+  const int per_sm = resident_ctas(kern, (MW + R) * 32, smem);
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3((MW + R) * 32); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)C; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+  cfg.attrs = at; cfg.numAttrs = 1;
+  // rows are dealt to clusters in turn: exactly as many clusters as run at once (a GPC's SMs are no multiple of C)
+  int64_t clusters = (int64_t)kNumSMs * per_sm;
+  if (C > 1) {
+    struct Key { const void* k; int dev, C; size_t smem; int n; };
+    static thread_local Key cache[64];
+    static thread_local int used = 0;
+    const void* kp = reinterpret_cast<const void*>(kern);
+    const int dev = device_ordinal();
+    int n = 0;
+    for (int i = 0; i < used && !n; ++i)
+      if (cache[i].k == kp && cache[i].dev == dev && cache[i].C == C && cache[i].smem == smem) n = cache[i].n;
+    if (!n) {
+      cfg.gridDim = dim3((unsigned)C);
+      if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) { (void)cudaGetLastError(); n = kNumSMs / C / 2; }
+      if (used < 64) cache[used++] = Key{kp, dev, C, smem, n};
+    }
+    clusters = n;
+  }
+  if (clusters > p.rows) clusters = p.rows;
+  cfg.gridDim = dim3((unsigned)(clusters * C));
+  cudaLaunchKernelEx(&cfg, kern, reinterpret_cast<T*>(dl), reinterpret_cast<const T*>(l), p, slot_bytes);
+  return check_launch();
+}
+
 template <typename T>
 static int launch_distill(uint64_t dl, uint64_t l, const DistillParams& p, cudaStream_t st) {
-  const size_t smem = (size_t)((p.vocab + 31) / 32) * 4;
-  const int64_t cap = (int64_t)kNumSMs * 8;
-  const unsigned grid = (unsigned)(p.rows < cap ? p.rows : cap);
-  T* dL = reinterpret_cast<T*>(dl);
-  const T* L = reinterpret_cast<const T*>(l);
-  if (dl) distill_rows_kernel<T, true><<<grid, kDistillThreads, smem, st>>>(dL, L, p);
-  else distill_rows_kernel<T, false><<<grid, kDistillThreads, smem, st>>>(dL, L, p);
-  return check_launch();
+  constexpr int VEC = Elem<T>::VEC;
+  const int nvec = (p.vocab + 2 * VEC - 2) / VEC;               // of the worst-aligned row
+  // CTAs a row: as many as keep a part within 4096 vectors (64 KB, three to an SM's shared memory)
+  int C = 1;
+  while (C < kDistillMaxC && (nvec + C - 1) / C > 4096) C *= 2;
+  const unsigned part = (unsigned)((nvec + C - 1) / C + 1) * 16;
+  const unsigned slot = (part + 127) / 128 * 128;
+  const int per = (nvec + C - 1) / C;
+  if (per <= 4 * 32 * kDistillNV) return launch_distill_as<T, 4, 3, true>(dl, l, p, C, slot, st);
+  if (per <= 16 * 32 * kDistillNV) return launch_distill_as<T, 16, 3, true>(dl, l, p, C, slot, st);
+  return launch_distill_as<T, 16, 1, false>(dl, l, p, C, slot, st);
 }
 
 }  // namespace cb
