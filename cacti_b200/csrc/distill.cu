@@ -16,7 +16,6 @@ namespace cb {
 
 constexpr int kDistillMaxK = 256;
 constexpr int64_t kDistillMaxVocab = 1 << 18;
-constexpr int kDistillThreads = 256;
 
 struct DistillParams {
   const void* t_values;          // teacher logits [rows, k] in t_dtype
@@ -73,10 +72,11 @@ __device__ __forceinline__ double warp_sum_f64(double v) {
 // Roles of a CTA (a cluster of C CTAs shares a row, each a run of its vectors):
 //   list warps, one per ring slot: fetch the slot's row (bulk copy), turn the teacher's list into probabilities (f64), take the
 //     listed student logits out of the staged row (they become -inf there), and, when the row is done, write the listed positions'
-//     gradient and the loss;
-//   MW main warps: maximum and exponentials of the unlisted positions in registers (one pass over shared memory), one
-//     combination of (maximum, sum) over the CTA and the cluster, then gradient = exponential times a factor, stored from
-//     registers.  The slot is free for the next row as soon as the exponentials are taken.
+//     gradient and the loss.  The list of a slot's next row is prepared while the main warps work on other rows;
+//   MW main warps: maximum and exponentials of the unlisted positions, one combination of (maximum, sum) over the CTA and the
+//     cluster, then gradient = exponential times a factor.
+// HOLD: a CTA's part of a row is at most MW * 32 * kDistillNV vectors: the exponentials stay in registers, one a position, and
+// the slot is free for the next row as soon as they are taken.  Otherwise they are formed again for the gradient.
 constexpr int kDistillNV = 8;                                  // vectors a main thread holds
 constexpr int kDistillMaxC = 8;
 struct DistillRow {              // from the list warp to the main warps
@@ -87,15 +87,21 @@ struct DistillRow {              // from the list warp to the main warps
 struct DistillFin { float m, z_all, z_rest; };                 // back to the list warp
 struct DistillRec { float m, z_rest, m_top, z_top; };          // a CTA's part of a row, to the cluster
 
-template <int MW, int R> struct DistillSmem {
+template <int MW, int R> struct alignas(16) DistillSmem {
   uint64_t full[R], marked[R], consumed[R], stored[R];
   uint64_t rec_bar[2];
   DistillRec rec[2][kDistillMaxC];
   float2 red[2][MW];
   DistillRow row[R];
   DistillFin fin[R];
-  alignas(16) int idx[R][kDistillMaxK];
 };
+// behind it: two lists a slot (the row at work and the next one), then the ring
+struct DistillList {             // KP = k rounded up to 32 entries of each
+  double* p;                     // scaled teacher logit, then probability
+  float* x;                      // listed student logit, where it is in this CTA's part
+  int* idx;                      // -1: no entry
+};
+constexpr unsigned kDistillListBytes = 16;                     // per entry
 
 __device__ __forceinline__ uint32_t distill_ctarank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ uint32_t distill_nctas() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
@@ -116,38 +122,114 @@ __device__ __forceinline__ bool distill_wait_cluster(uint64_t* bar, unsigned par
   return false;
 }
 
-// 2^((x - m) c); m is finite or the result is meant to be NaN
+// 2^((x - m) c); m is finite or the result is meant to be NaN.  The difference comes first: rows near the type's largest
+// magnitudes then lose nothing, and the multiply it costs hides behind the ex2 unit, which is the slower one.
 __device__ __forceinline__ float exp_rel(float x, float m, float c) { return exp2f_approx((x - m) * c); }
 
-// One vector of gradient values to memory; foreign elements are left out.
-template <typename T>
-__device__ __forceinline__ void distill_store(T* __restrict__ drow, int v, int head, int V, bool vec_ok, int beta, const float (&d)[Elem<T>::VEC]) {
-  constexpr int VEC = Elem<T>::VEC;
-  const int j0 = v * VEC - head;
-  if (vec_ok && j0 >= 0 && j0 + VEC <= V) {
-    if (beta) st_stream(drow + j0, pack_accumulate<T>(d, ld_stream(drow + j0)));
-    else st_stream(drow + j0, pack<T>(d));
-  } else {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      if (j0 + e >= 0 && j0 + e < V) {
-        T* o = drow + j0 + e;
-        *o = beta ? Elem<T>::from_f32(Elem<T>::to_f32(*o) + round_to<T>(d[e])) : Elem<T>::from_f32(d[e]);
-      }
-    }
-  }
+template <typename T> __device__ __forceinline__ void distill_put(T* o, float v, int beta) {
+  *o = beta ? Elem<T>::from_f32(Elem<T>::to_f32(*o) + round_to<T>(v)) : Elem<T>::from_f32(v);
 }
 
-// HOLD: a CTA's part of a row is at most MW * 32 * kDistillNV vectors and its exponentials stay in registers; otherwise they are
-// formed again for the gradient (parts above 64 KB: f32 rows beyond 131072).
-template <typename T, int MW, int R, bool HOLD, bool BWD>
+// What a list warp knows of a row.
+struct DistillHead { float w; double psum, ent, r; bool bad; };
+
+// Prepare the list of `row`: indices and validity, probabilities, their sums.
+template <typename T>
+__device__ __forceinline__ void distill_prepare(const DistillParams& p, int64_t row, const DistillList& li, int KP, int lane, DistillHead& h) {
+  h.w = p.w_rows ? p.w_rows[row] : p.w_scalar;
+  h.psum = h.ent = h.r = 0.;
+  h.bad = false;
+  if (h.w == 0.f) return;
+  double lse_t = p.t_lse ? (double)p.t_lse[row] : 0.;
+  bool bad = false;
+#pragma unroll 2
+  for (int k = lane; k < KP; k += 32) {
+    int id = -1;
+    double z = 0.;
+    if (k < p.k) { id = teacher_index(p, row * p.k + k); z = p.inv_temp * teacher_value(p, row * p.k + k); }
+    bad |= id == -2;
+    li.idx[k] = id < 0 ? -1 : id;
+    li.p[k] = z;
+  }
+  __syncwarp();
+  // an index listed twice: count equals (itself among them); which slot is the first matters only when there are any
+  bool twice = false;
+#pragma unroll 1
+  for (int k = lane; k < KP; k += 32) {
+    const int own = li.idx[k];
+    int hits = 0;
+#pragma unroll 4
+    for (int j = 0; j < KP; j += 4) {
+      const int4 o = *reinterpret_cast<const int4*>(li.idx + j);
+      hits += (o.x == own) + (o.y == own) + (o.z == own) + (o.w == own);
+    }
+    twice |= own >= 0 && hits > 1;
+  }
+  if (__any_sync(0xffffffffu, twice)) {
+    bad = true;
+#pragma unroll 1
+    for (int k = lane; k < KP; k += 32) {
+      bool earlier = false;
+      for (int j = 0; j < k; ++j) earlier |= li.idx[j] == li.idx[k];
+      li.x[k] = earlier ? 1.f : 0.f;
+    }
+    __syncwarp();
+    for (int k = lane; k < KP; k += 32) if (li.x[k] != 0.f) li.idx[k] = -1;
+    __syncwarp();
+  }
+  h.bad = __any_sync(0xffffffffu, bad);
+  int cnt = 0;
+  double zm = -INFINITY;
+#pragma unroll 1
+  for (int k = lane; k < KP; k += 32) {
+    const bool valid = li.idx[k] >= 0;
+    const double z = valid ? li.p[k] : -INFINITY;
+    li.p[k] = z;
+    cnt += valid;
+    zm = z > zm || z != z ? z : zm;
+  }
+  cnt = __reduce_add_sync(0xffffffffu, cnt);
+  if (!p.t_lse) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) { const double v = __shfl_xor_sync(0xffffffffu, zm, o); zm = v > zm || v != v ? v : zm; }
+    double e = 0.;
+#pragma unroll 1
+    for (int k = lane; k < KP; k += 32) if (li.p[k] != -INFINITY) e += exp(li.p[k] - zm);
+    lse_t = zm + log(warp_sum_f64(e));
+  }
+#pragma unroll 1
+  for (int k = lane; k < KP; k += 32) {
+    const double z = li.p[k];
+    double pk = 0.;
+    if (z != -INFINITY) {
+      pk = exp(z - lse_t);
+      h.psum += pk;
+      if (pk != 0.) h.ent += pk * (z - lse_t);
+    }
+    li.p[k] = pk;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    h.psum += __shfl_xor_sync(0xffffffffu, h.psum, o);
+    h.ent += __shfl_xor_sync(0xffffffffu, h.ent, o);
+  }
+  if (p.t_lse && cnt && cnt < p.vocab) h.r = fmax(0., 1. - h.psum);
+}
+
+enum { kDistillFwd = 0, kDistillBwd = 1, kDistillAcc = 2 };
+
+template <typename T, int MW, int R, bool HOLD, int MODE>
 __global__ void __launch_bounds__((MW + R) * 32)
 distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constant__ DistillParams p, unsigned slot_bytes) {
   constexpr int VEC = Elem<T>::VEC, MT = MW * 32;
+  constexpr bool BWD = MODE != kDistillFwd;
+  constexpr int beta = MODE == kDistillAcc;
   extern __shared__ __align__(128) unsigned char smem_raw[];
   using Smem = DistillSmem<MW, R>;
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
-  unsigned char* ring = smem_raw + (sizeof(Smem) + 127) / 128 * 128;
+  const int KP = (p.k + 31) / 32 * 32;
+  unsigned char* lists = smem_raw + sizeof(Smem);
+  unsigned char* ring = smem_raw + (sizeof(Smem) + (size_t)2 * R * KP * kDistillListBytes + 127) / 128 * 128;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, V = p.vocab;
   const int C = (int)distill_nctas(), rank = (int)distill_ctarank();
   const int64_t row0 = blockIdx.x / C, stride = gridDim.x / C;
@@ -163,16 +245,15 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
   if (warp >= MW) {
     // ---------------- list warp of slot s ----------------
     const int s = warp - MW;
-    unsigned char* buf = ring + (size_t)s * slot_bytes;
-    T* sx = reinterpret_cast<T*>(buf);
-    unsigned ph = 0;
-    bool ok = true;
+    T* sx = reinterpret_cast<T*>(ring + (size_t)s * slot_bytes);
     const uint64_t t_begin = reinterpret_cast<uint64_t>(L), t_end = t_begin + (uint64_t)p.rows * V * sizeof(T);
-    float w_row = 0.f;
+    auto list_of = [&](int b) {
+      unsigned char* at = lists + (size_t)(2 * s + b) * KP * kDistillListBytes;
+      return DistillList{reinterpret_cast<double*>(at), reinterpret_cast<float*>(at + 8 * KP), reinterpret_cast<int*>(at + 12 * KP)};
+    };
     // fetch a row's vectors of this CTA; whole vectors inside the tensor only
     auto issue = [&](int64_t row) {
-      w_row = p.w_rows ? p.w_rows[row] : p.w_scalar;
-      if (lane == 0 && w_row != 0.f) {
+      if (lane == 0) {
         const RowVecs<T> rv(L + row * V, V);
         const int v0 = (int)((int64_t)rv.nvec * rank / C), v1 = (int)((int64_t)rv.nvec * (rank + 1) / C);
         const unsigned char *a = rv.base + (size_t)v0 * 16, *b = rv.base + (size_t)v1 * 16;
@@ -180,215 +261,154 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
         if (reinterpret_cast<uint64_t>(a) < t_begin) { a += 16; skip = 16; }
         if (reinterpret_cast<uint64_t>(b) > t_end) b -= 16;
         const unsigned bytes = b > a ? (unsigned)(b - a) : 0u;
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // marks in the slot before the copy over them
         mbar_expect_tx(sm.full + s, bytes);
-        if (bytes) bulk_g2s(buf + skip, a, bytes, sm.full + s);
+        if (bytes) bulk_g2s(reinterpret_cast<unsigned char*>(sx) + skip, a, bytes, sm.full + s);
       }
     };
+    unsigned ph = 0, full_ph = 0;                               // rows of weight 0 do not pass through `full`
+    int b = 0;
+    DistillHead h, hn;
     int64_t row = row0 + s * stride;
-    if (row < p.rows) issue(row);
-    unsigned full_ph = 0;                                       // rows of weight 0 do not pass through `full`
-    for (; row < p.rows; row += (int64_t)R * stride) {
-      const float w = w_row;
-      const bool skip = w == 0.f;
+    if (row < p.rows) {
+      const float w0 = p.w_rows ? p.w_rows[row] : p.w_scalar;
+      if (w0 != 0.f) issue(row);
+      distill_prepare<T>(p, row, list_of(0), KP, lane, h);
+    }
+    for (; row < p.rows; row += (int64_t)R * stride, b ^= 1, h = hn) {
+      const bool skip = h.w == 0.f;
       const RowVecs<T> rv(L + row * V, V);
       const int v0 = (int)((int64_t)rv.nvec * rank / C), v1 = (int)((int64_t)rv.nvec * (rank + 1) / C);
       const int jlo = v0 * VEC - rv.head, jhi = v1 * VEC - rv.head;          // row elements of this CTA: [jlo, jhi)
-      int idx[kDistillMaxK / 32];
-      double pk[kDistillMaxK / 32];
-      float xk[kDistillMaxK / 32];
-      double psum = 0., ent = 0., r = 0.;
-      bool row_bad = false;
+      const DistillList li = list_of(b);
+      float xe[2] = {-INFINITY, -INFINITY};                     // edge vectors' elements, for the lanes below VEC
       if (!skip) {
-        // ---- the list: indices, validity ----
-        double zs[kDistillMaxK / 32];
-#pragma unroll
-        for (int i = 0; i < kDistillMaxK / 32; ++i) {
-          const int k = i * 32 + lane;
-          idx[i] = -1; zs[i] = 0.;
-          if (i * 32 < p.k) {
-            if (k < p.k) {
-              idx[i] = teacher_index(p, row * p.k + k);
-              zs[i] = p.inv_temp * teacher_value(p, row * p.k + k);
-            }
-            sm.idx[s][k] = idx[i];
-          }
-        }
-        const double tl = p.t_lse ? (double)p.t_lse[row] : 0.;
-        __syncwarp();
-        bool bad = false;
-#pragma unroll
-        for (int i = 0; i < kDistillMaxK / 32; ++i) bad |= idx[i] == -2;
-        unsigned dup = 0;
-#pragma unroll
-        for (int i0 = 0; i0 < kDistillMaxK / 32; ++i0) {
-          if (i0 * 32 < p.k) {
-            for (int q = 0; q < 8; ++q) {                       // slots i0 * 32 + 4 q ... + 3 against this lane's later ones
-              const int4 o = *reinterpret_cast<const int4*>(&sm.idx[s][i0 * 32 + q * 4]);
-#pragma unroll
-              for (int i = i0; i < kDistillMaxK / 32; ++i) {
-                if (i * 32 < p.k) {
-                  const int lim = i == i0 ? lane - q * 4 : 4;   // of these four, those before this slot
-                  const bool hit = (o.x == idx[i] && lim > 0) || (o.y == idx[i] && lim > 1) || (o.z == idx[i] && lim > 2) || (o.w == idx[i] && lim > 3);
-                  dup |= (hit && idx[i] >= 0 ? 1u : 0u) << i;
-                }
-              }
-            }
-          }
-        }
-        bad |= dup != 0;
-        row_bad = __any_sync(0xffffffffu, bad);
-        // ---- its probabilities ----
-        double zm = -INFINITY;
-        int cnt = 0;
-#pragma unroll
-        for (int i = 0; i < kDistillMaxK / 32; ++i) {
-          if (idx[i] < 0 || ((dup >> i) & 1u)) { idx[i] = -1; zs[i] = -INFINITY; }
-          else ++cnt;
-          zm = zs[i] > zm || zs[i] != zs[i] ? zs[i] : zm;
-        }
-        double lse_t = tl;
-        if (!p.t_lse) {
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) { const double v = __shfl_xor_sync(0xffffffffu, zm, o); zm = v > zm || v != v ? v : zm; }
-          double e = 0.;
-#pragma unroll
-          for (int i = 0; i < kDistillMaxK / 32; ++i)
-            if (i * 32 < p.k && zs[i] != -INFINITY) e += exp(zs[i] - zm);
-          lse_t = zm + log(warp_sum_f64(e));
-        }
-#pragma unroll
-        for (int i = 0; i < kDistillMaxK / 32; ++i) {
-          pk[i] = 0.;
-          if (i * 32 < p.k && zs[i] != -INFINITY) {
-            pk[i] = exp(zs[i] - lse_t);
-            psum += pk[i];
-            if (pk[i] != 0.) ent += pk[i] * (zs[i] - lse_t);
-          }
-        }
-        psum = warp_sum_f64(psum);
-        ent = warp_sum_f64(ent);
-        cnt = __reduce_add_sync(0xffffffffu, cnt);
-        if (p.t_lse && cnt && cnt < V) r = fmax(0., 1. - psum);
         // ---- the listed logits out of the staged row ----
-        ok = mbar_wait_bounded_warp(sm.full + s, full_ph, kDevErrStageTimeout);
+        if (!mbar_wait_bounded_warp(sm.full + s, full_ph, kDevErrStageTimeout)) break;
         full_ph ^= 1u;
-        if (!ok) break;
         if (lane < VEC) {
           // foreign elements, and edge vectors that were not copied because they reach outside the tensor
           for (int side = 0; side < 2; ++side) {
             const int v = side ? v1 - 1 : v0;
             if (v < v0 || v >= v1 || (side && v == v0)) continue;
-            const unsigned char* a = rv.base + (size_t)v * 16;
+            const uint64_t a = reinterpret_cast<uint64_t>(rv.base) + (uint64_t)v * 16;
             const int j = v * VEC - rv.head + lane;
-            const bool in = j >= 0 && j < V;
-            const bool outside = reinterpret_cast<uint64_t>(a) < t_begin || reinterpret_cast<uint64_t>(a) + 16 > t_end;
-            if (!in) sx[(v - v0) * VEC + lane] = Elem<T>::from_f32(-INFINITY);
-            else if (outside) sx[(v - v0) * VEC + lane] = L[row * V + j];
+            if (j < 0 || j >= V) sx[(v - v0) * VEC + lane] = Elem<T>::from_f32(-INFINITY);
+            else if (a < t_begin || a + 16 > t_end) sx[(v - v0) * VEC + lane] = L[row * V + j];
           }
         }
         __syncwarp();
         float mt = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < kDistillMaxK / 32; ++i) {
-          xk[i] = -INFINITY;
-          if (idx[i] >= jlo && idx[i] < jhi && idx[i] >= 0) {
-            T* at = sx + (idx[i] - jlo);
-            xk[i] = Elem<T>::to_f32(*at);
-            *at = Elem<T>::from_f32(-INFINITY);
-          } else {
-            idx[i] = -1;                                        // another CTA's
-          }
-          mt = fmaxf(mt, xk[i]);
+        for (int k = lane; k < KP; k += 32) {
+          const int id = li.idx[k];
+          float x = -INFINITY;
+          if (id >= 0 && id >= jlo && id < jhi) { x = Elem<T>::to_f32(sx[id - jlo]); sx[id - jlo] = Elem<T>::from_f32(-INFINITY); }
+          li.x[k] = x;
+          mt = fmaxf(mt, x);
         }
         mt = warp_reduce<MaxOp>(mt);
         const float ref = mt == -INFINITY ? 0.f : mt;
         float zt = 0.f;
-#pragma unroll
-        for (int i = 0; i < kDistillMaxK / 32; ++i) if (idx[i] >= 0) zt += exp_rel(xk[i], ref, c);
+        for (int k = lane; k < KP; k += 32) zt += exp_rel(li.x[k], ref, c);
         zt = warp_reduce<SumOp>(zt);
         if (lane == 0) {
-          const double wc = (double)w * p.inv_temp;
-          sm.row[s] = DistillRow{mt, zt, (float)(wc * (psum + r)), (float)(wc * r), 0};
+          const double wc = (double)h.w * p.inv_temp;
+          sm.row[s] = DistillRow{mt, zt, (float)(wc * (h.psum + h.r)), (float)(wc * h.r), 0};
+        }
+        __syncwarp();
+        if (HOLD && BWD && lane < VEC) {
+          if (v1 > v0) xe[0] = Elem<T>::to_f32(sx[lane]);
+          if (v1 > v0 + 1) xe[1] = Elem<T>::to_f32(sx[(v1 - 1 - v0) * VEC + lane]);
         }
       } else if (lane == 0) {
         sm.row[s] = DistillRow{0.f, 0.f, 0.f, 0.f, 1};
       }
       __syncwarp();
       if (lane == 0) distill_arrive(sm.marked + s);
-      // ---- the slot is free once the main warps have taken its exponentials: next row ----
-      ok = mbar_wait_bounded_warp(sm.consumed + s, ph, kDevErrStageTimeout);
-      if (!ok) break;
-      if (row + (int64_t)R * stride < p.rows) issue(row + (int64_t)R * stride);
+      // ---- the next row's list; its fetch once the main warps have taken this row out of the slot ----
+      const int64_t next = row + (int64_t)R * stride;
+      if (next < p.rows) distill_prepare<T>(p, next, list_of(b ^ 1), KP, lane, hn);
+      if (!mbar_wait_bounded_warp(sm.consumed + s, ph, kDevErrStageTimeout)) break;
+      if (next < p.rows && hn.w != 0.f) issue(next);
       // ---- the row is done: listed positions and loss ----
-      ok = mbar_wait_bounded_warp(sm.stored + s, ph, kDevErrStageTimeout);
+      if (!mbar_wait_bounded_warp(sm.stored + s, ph, kDevErrStageTimeout)) break;
       ph ^= 1u;
-      if (!ok) break;
       if (skip) {
         if (lane == 0 && rank == 0 && p.loss_rows) p.loss_rows[row] = 0.f;
         continue;
       }
       const DistillFin f = sm.fin[s];
-      const double mass = psum + r;
+      const double mass = h.psum + h.r;
       if (BWD) {
-        const double wc = (double)w * p.inv_temp;
-        const float ga = mass != 0. ? (float)(wc * mass / (double)f.z_all) : 0.f;
+        T* drow = dL + row * V;
+        const double wc = (double)h.w * p.inv_temp;
         const float ref = f.m == -INFINITY ? 0.f : f.m;
-#pragma unroll
-        for (int i = 0; i < kDistillMaxK / 32; ++i) {
-          if (idx[i] >= 0) {
-            const float v = exp_rel(xk[i], ref, c) * ga - (float)(wc * pk[i]);
-            T* o = dL + row * V + idx[i];
-            *o = p.beta ? Elem<T>::from_f32(Elem<T>::to_f32(*o) + round_to<T>(v)) : Elem<T>::from_f32(v);
+        if (HOLD && lane < VEC) {
+          // edge vectors, which the main warps leave out
+          const float g = mass != 0. ? (float)(wc * mass / (double)f.z_all - (h.r > 0. && f.z_rest > 0.f ? wc * h.r / (double)f.z_rest : 0.)) : 0.f;
+          for (int side = 0; side < 2; ++side) {
+            const int v = side ? v1 - 1 : v0;
+            const int j0 = v * VEC - rv.head;
+            if (v < v0 || v >= v1 || (side && v == v0) || (j0 >= 0 && j0 + VEC <= V)) continue;
+            if (j0 + lane >= 0 && j0 + lane < V) distill_put<T>(drow + j0 + lane, exp_rel(xe[side], ref, c) * g, beta);
           }
         }
+        __syncwarp();
+        const float ga = mass != 0. ? (float)(wc * mass / (double)f.z_all) : 0.f;
+        for (int k = lane; k < KP; k += 32) {
+          const int id = li.idx[k];
+          if (id >= 0 && id >= jlo && id < jhi) distill_put<T>(drow + id, exp_rel(li.x[k], ref, c) * ga - (float)(wc * li.p[k]), beta);
+        }
       }
-      if (p.loss_rows) {
+      if (rank == 0 && p.loss_rows) {
         // sum p (x_k - m): differences to the maximum, so that a row of values like the type's lowest loses nothing.
-        // Every CTA of a cluster adds its own listed positions: the first one finds the others' in global memory.
+        // Listed logits of the cluster's other parts are read from memory.
         double px = 0.;
-#pragma unroll
-        for (int i = 0; i < kDistillMaxK / 32; ++i) {
-          if (i * 32 < p.k && pk[i] != 0.) {
-            float x = xk[i];
-            if (C > 1 && rank == 0 && idx[i] < 0) {
-              const int j = teacher_index(p, row * p.k + i * 32 + lane);
-              x = Elem<T>::to_f32(L[row * V + j]);
-            }
-            px += pk[i] * ((double)x - (double)f.m);
+        for (int k = lane; k < KP; k += 32) {
+          const double pk = li.p[k];
+          if (pk != 0.) {
+            const int id = li.idx[k];
+            const float x = id >= jlo && id < jhi ? li.x[k] : Elem<T>::to_f32(L[row * V + id]);
+            px += pk * ((double)x - (double)f.m);
           }
         }
         px = warp_sum_f64(px);
-        if (lane == 0 && rank == 0) {
+        if (lane == 0) {
           const double la = log((double)f.z_all);
-          double loss = mass != 0. ? ent - p.inv_temp * px + psum * la : 0.;
-          if (r > 0.) loss += r * (log(r) - log((double)f.z_rest) + la);
-          p.loss_rows[row] = row_bad ? __int_as_float(0x7fc00000) : (float)loss;
+          double loss = mass != 0. ? h.ent - p.inv_temp * px + h.psum * la : 0.;
+          if (h.r > 0.) loss += h.r * (log(h.r) - log((double)f.z_rest) + la);
+          p.loss_rows[row] = h.bad ? __int_as_float(0x7fc00000) : (float)loss;
         }
       }
-      if (lane == 0 && rank == 0 && row_bad && p.status) atomicMax(p.status, (unsigned)CACTI_B200_ERR_INDEX_RANGE);
+      if (lane == 0 && rank == 0 && h.bad && p.status) atomicMax(p.status, (unsigned)CACTI_B200_ERR_INDEX_RANGE);
+      __syncwarp();
     }
   } else {
     // ---------------- main warps ----------------
     const int t = threadIdx.x;
     int s = 0;
     unsigned ph = 0, par = 0, rph[2] = {0, 0};
-    for (int64_t row = row0; row < p.rows; row += stride, par ^= 1u) {
+    for (int64_t row = row0; row < p.rows; row += stride) {
       // a wait that ran out is agreed on at the CTA's barrier below; until then the warp goes on with what is there
       bool gave_up = !mbar_wait_bounded_warp(sm.marked + s, ph, kDevErrStageTimeout);
       const DistillRow info = sm.row[s];
       const RowVecs<T> rv(L + row * V, V);
       const int v0 = (int)((int64_t)rv.nvec * rank / C), n = (int)((int64_t)rv.nvec * (rank + 1) / C) - v0;
-      T* drow = BWD ? dL + row * V : nullptr;
-      const bool vec_ok = BWD && ((reinterpret_cast<uint64_t>(drow) ^ reinterpret_cast<uint64_t>(L + row * V)) & 15) == 0;
+      const int j0 = v0 * VEC - rv.head;                        // row element of this part's first vector
+      // vectors [ilo, ihi) of this part lie wholly inside the row
+      const int ilo = j0 < 0 ? 1 : 0, ihi = j0 + n * VEC > V ? n - 1 : n;
+      T* dpart = BWD ? dL + row * V + j0 : nullptr;
+      const bool vec_ok = BWD && (HOLD || ((reinterpret_cast<uint64_t>(dL) ^ reinterpret_cast<uint64_t>(L)) & 15) == 0);
       if (info.skip) {
-        if (BWD && !p.beta) {
-          const float z[VEC] = {};
-          for (int v = t; v < n; v += MT) distill_store<T>(drow, v0 + v, rv.head, V, vec_ok, 0, z);
+        if (BWD && !beta) {
+          const T zero = Elem<T>::from_f32(0.f);
+          for (int i = t; i < n; i += MT) {
+            if (vec_ok && i >= ilo && i < ihi) st_stream(dpart + i * VEC, make_uint4(0, 0, 0, 0));
+            else for (int e = 0; e < VEC; ++e) if (j0 + i * VEC + e >= 0 && j0 + i * VEC + e < V) dpart[i * VEC + e] = zero;
+          }
         }
         if (lane == 0) { distill_arrive(sm.consumed + s); distill_arrive(sm.stored + s); }
         if (++s == R) { s = 0; ph ^= 1u; }
-        par ^= 1u;                                              // nothing exchanged
         if (gave_up) break;
         continue;
       }
@@ -408,6 +428,7 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
           }
         }
         mw = warp_reduce<MaxOp>(fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])));
+        if (lane == 0) distill_arrive(sm.consumed + s);         // the reduction has ordered the warp's reads before it
         ref = mw == -INFINITY ? 0.f : mw;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
@@ -416,7 +437,6 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
             for (int e = 0; e < VEC; ++e) { a[k][e] = exp_rel(a[k][e], ref, c); zq[e & 3] += a[k][e]; }
           }
         }
-        if (lane == 0) distill_arrive(sm.consumed + s);         // (the warp reduction below orders the reads before it)
       } else {
         for (int v = t; v < n; v += MT) {
           unpack<T>(srow[v], a[0]);
@@ -446,11 +466,10 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
       if (C > 1) {
         // every CTA hands its part to all of the cluster; the parts are combined in rank order everywhere
         if (warp == 0 && lane < C) {
-          const DistillRec mine{m, z_rest, m_top, z_top};
           uint32_t dst, bar;
           asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(dst) : "r"(smem_u32(&sm.rec[par][rank])), "r"(lane));
           asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(smem_u32(&sm.rec_bar[par])), "r"(lane));
-          asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "f"(mine.m), "f"(mine.z_rest), "f"(mine.m_top), "f"(mine.z_top) : "memory");
+          asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "f"(m), "f"(z_rest), "f"(m_top), "f"(z_top) : "memory");
           asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
         }
         gave_up = !__all_sync(0xffffffffu, distill_wait_cluster(sm.rec_bar + par, rph[par]));
@@ -463,6 +482,7 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
         const float tr = m_top == -INFINITY ? 0.f : m_top;
         z_top = warp_reduce<SumOp>(o.z_top * exp_rel(o.m_top, tr, c));
       }
+      par ^= 1u;
       // against the maximum of the whole row, listed positions included
       const float mall = fmaxf(m, m_top), mref = mall == -INFINITY ? 0.f : mall;
       z_rest *= exp_rel(m, mref, c);
@@ -476,18 +496,28 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
           const float f = mw == -INFINITY && mall != -INFINITY ? g * 0.f : g * exp_rel(ref, mref, c);
 #pragma unroll
           for (int k = 0; k < NV; ++k) {
-            if (t + k * MT < n) {
+            const int i = t + k * MT;
+            if (i >= ilo && i < ihi) {
+              T* o = dpart + i * VEC;
 #pragma unroll
               for (int e = 0; e < VEC; ++e) a[k][e] *= f;
-              distill_store<T>(drow, v0 + t + k * MT, rv.head, V, vec_ok, p.beta, a[k]);
+              if (beta) st_stream(o, pack_accumulate<T>(a[k], ld_stream(o)));
+              else st_stream(o, pack<T>(a[k]));
             }
           }
         } else {
-          for (int v = t; v < n; v += MT) {
-            unpack<T>(srow[v], a[0]);
+          for (int i = t; i < n; i += MT) {
+            unpack<T>(srow[i], a[0]);
+            T* o = dpart + i * VEC;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) a[0][e] = exp_rel(a[0][e], mref, c) * g;
-            distill_store<T>(drow, v0 + v, rv.head, V, vec_ok, p.beta, a[0]);
+            if (vec_ok && i >= ilo && i < ihi) {
+              if (beta) st_stream(o, pack_accumulate<T>(a[0], ld_stream(o)));
+              else st_stream(o, pack<T>(a[0]));
+            } else {
+#pragma unroll
+              for (int e = 0; e < VEC; ++e) if (j0 + i * VEC + e >= 0 && j0 + i * VEC + e < V) distill_put<T>(o + e, a[0][e], beta);
+            }
           }
         }
       }
@@ -524,8 +554,10 @@ distill_loss_sum_kernel(float* __restrict__ loss_sum, const float* __restrict__ 
 
 template <typename T, int MW, int R, bool HOLD>
 static int launch_distill_as(uint64_t dl, uint64_t l, const DistillParams& p, int C, unsigned slot_bytes, cudaStream_t st) {
-  const size_t smem = (sizeof(DistillSmem<MW, R>) + 127) / 128 * 128 + (size_t)R * slot_bytes;
-  auto kern = dl ? distill_kernel<T, MW, R, HOLD, true> : distill_kernel<T, MW, R, HOLD, false>;
+  const size_t lists = (size_t)2 * R * ((p.k + 31) / 32 * 32) * kDistillListBytes;
+  const size_t smem = (sizeof(DistillSmem<MW, R>) + lists + 127) / 128 * 128 + (size_t)R * slot_bytes;
+  auto kern = !dl ? distill_kernel<T, MW, R, HOLD, kDistillFwd>
+                  : p.beta ? distill_kernel<T, MW, R, HOLD, kDistillAcc> : distill_kernel<T, MW, R, HOLD, kDistillBwd>;
   const int per_sm = resident_ctas(kern, (MW + R) * 32, smem);
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3((MW + R) * 32); cfg.dynamicSmemBytes = smem; cfg.stream = st;
@@ -567,8 +599,10 @@ static int launch_distill(uint64_t dl, uint64_t l, const DistillParams& p, cudaS
   const unsigned part = (unsigned)((nvec + C - 1) / C + 1) * 16;
   const unsigned slot = (part + 127) / 128 * 128;
   const int per = (nvec + C - 1) / C;
-  if (per <= 4 * 32 * kDistillNV) return launch_distill_as<T, 4, 3, true>(dl, l, p, C, slot, st);
-  if (per <= 16 * 32 * kDistillNV) return launch_distill_as<T, 16, 3, true>(dl, l, p, C, slot, st);
+  // registers hold the exponentials where vectors of logits and gradient coincide; a shifted gradient is stored by element
+  const bool same = !dl || ((dl ^ l) & 15) == 0;
+  if (same && per <= 4 * 32 * kDistillNV) return launch_distill_as<T, 4, 3, true>(dl, l, p, C, slot, st);
+  if (same && per <= 16 * 32 * kDistillNV) return launch_distill_as<T, 16, 3, true>(dl, l, p, C, slot, st);
   return launch_distill_as<T, 16, 1, false>(dl, l, p, C, slot, st);
 }
 
