@@ -70,34 +70,37 @@ __device__ __forceinline__ double warp_sum_f64(double v) {
 }
 
 // Roles of a CTA (a cluster of C CTAs shares a row, each a run of its vectors):
-//   list warps, one per ring slot: fetch the slot's row (bulk copy), turn the teacher's list into probabilities (f64), take the
-//     listed student logits out of the staged row (they become -inf there), and, when the row is done, write the listed positions'
-//     gradient and the loss.  The list of a slot's next row is prepared while the main warps work on other rows;
+//   list warps, one per ring slot: fetch the slot's row (bulk copy), turn the teacher's list into probabilities, take the listed
+//     student logits out of the staged row (they become -inf there), and, when the row's gradient lies in the slot, put the listed
+//     positions' gradient in, send it off (bulk copy) and write the loss.  The list of a slot's next row is prepared while the
+//     main warps work;
 //   MW main warps: maximum and exponentials of the unlisted positions, one combination of (maximum, sum) over the CTA and the
-//     cluster, then gradient = exponential times a factor.
-// HOLD: a CTA's part of a row is at most MW * 32 * kDistillNV vectors: the exponentials stay in registers, one a position, and
-// the slot is free for the next row as soon as they are taken.  Otherwise they are formed again for the gradient.
+//     cluster, then gradient = exponential times a factor, written over the staged row.
+// HOLD: a CTA's part of a row is at most MW * 32 * kDistillNV vectors: the exponentials stay in registers, one a position.
+// Otherwise they are formed again for the gradient.
 constexpr int kDistillNV = 8;                                  // vectors a main thread holds
 constexpr int kDistillMaxC = 8;
+constexpr int kDistillSeen = 128;                              // words of a list's index filter
 struct DistillRow {              // from the list warp to the main warps
   float m_top, z_top;            // maximum of the listed logits (of this CTA's vectors) and sum of their exponentials
   float g_mass, g_r;             // w c P and w c r
   int skip;                      // weight 0
 };
 struct DistillFin { float m, z_all, z_rest; };                 // back to the list warp
-struct DistillRec { float m, z_rest, m_top, z_top; };          // a CTA's part of a row, to the cluster
+struct alignas(16) DistillRec { float m, z_rest, m_top, z_top; };          // a CTA's part of a row, to the cluster
 
 template <int MW, int R> struct alignas(16) DistillSmem {
-  uint64_t full[R], marked[R], consumed[R], stored[R];
+  uint64_t full[R], marked[R], stored[R];
   uint64_t rec_bar[2];
   DistillRec rec[2][kDistillMaxC];
   float2 red[2][MW];
   DistillRow row[R];
   DistillFin fin[R];
+  unsigned seen[R][kDistillSeen];
 };
 // behind it: two lists a slot (the row at work and the next one), then the ring
 struct DistillList {             // KP = k rounded up to 32 entries of each
-  double* p;                     // scaled teacher logit, then probability
+  double* p;                     // scaled teacher logit, later the probability
   float* x;                      // listed student logit, where it is in this CTA's part
   int* idx;                      // -1: no entry
 };
@@ -133,68 +136,96 @@ template <typename T> __device__ __forceinline__ void distill_put(T* o, float v,
 // What a list warp knows of a row.
 struct DistillHead { float w; double psum, ent, r; bool bad; };
 
+// exp(d) to about 1e-10: 2^n times the Taylor series of exp(f ln2), |f| <= 1/2, to the eighth power (the next term is
+// (ln2 / 2)^9 / 9! = 2e-10).  A third of the latency of the library's, which a single warp does not hide.  The f32 functions
+// would do for ordinary rows; where the student gives a listed word a logit of -65504, the loss shows their 1e-7.
+__device__ __forceinline__ double exp_list(double d) {
+  const double y = d * 1.4426950408889634;
+  if (!(y > -1000.)) return y != y ? y : 0.;
+  if (y > 1000.) return INFINITY;
+  const double n = rint(y), x = (y - n) * 0.6931471805599453;
+  double s = 1. / 40320.;
+  s = fma(s, x, 1. / 5040.);
+  s = fma(s, x, 1. / 720.);
+  s = fma(s, x, 1. / 120.);
+  s = fma(s, x, 1. / 24.);
+  s = fma(s, x, 1. / 6.);
+  s = fma(s, x, 0.5);
+  s = fma(s, x, 1.);
+  s = fma(s, x, 1.);
+  return s * __hiloint2double(((int)n + 1023) << 20, 0);
+}
+
 // Prepare the list of `row`: indices and validity, probabilities, their sums.
 template <typename T>
-__device__ __forceinline__ void distill_prepare(const DistillParams& p, int64_t row, const DistillList& li, int KP, int lane, DistillHead& h) {
+__device__ __forceinline__ void distill_prepare(const DistillParams& p, int64_t row, const DistillList& li, unsigned* seen, int KP, int lane, DistillHead& h) {
   h.w = p.w_rows ? p.w_rows[row] : p.w_scalar;
   h.psum = h.ent = h.r = 0.;
   h.bad = false;
   if (h.w == 0.f) return;
   double lse_t = p.t_lse ? (double)p.t_lse[row] : 0.;
-  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < kDistillSeen / 32; ++i) seen[i * 32 + lane] = 0u;
+  __syncwarp();
+  // An index listed twice: of two equal ones at least one finds its bit in the filter set; only such slots are compared
+  // with the whole list.
+  bool bad = false, suspect = false;
 #pragma unroll 2
   for (int k = lane; k < KP; k += 32) {
     int id = -1;
     double z = 0.;
     if (k < p.k) { id = teacher_index(p, row * p.k + k); z = p.inv_temp * teacher_value(p, row * p.k + k); }
     bad |= id == -2;
+    if (id >= 0) {
+      const unsigned hash = ((unsigned)id * 2654435761u) >> 20;                 // 12 bits
+      const unsigned bit = 1u << (hash & 31);
+      suspect |= (atomicOr(seen + (hash >> 5), bit) & bit) != 0;
+    }
     li.idx[k] = id < 0 ? -1 : id;
-    li.p[k] = z;
+    li.p[k] = id < 0 ? -INFINITY : z;
   }
   __syncwarp();
-  // an index listed twice: count equals (itself among them); which slot is the first matters only when there are any
-  bool twice = false;
-#pragma unroll 1
-  for (int k = lane; k < KP; k += 32) {
-    const int own = li.idx[k];
-    int hits = 0;
-#pragma unroll 4
-    for (int j = 0; j < KP; j += 4) {
-      const int4 o = *reinterpret_cast<const int4*>(li.idx + j);
-      hits += (o.x == own) + (o.y == own) + (o.z == own) + (o.w == own);
-    }
-    twice |= own >= 0 && hits > 1;
-  }
-  if (__any_sync(0xffffffffu, twice)) {
-    bad = true;
+  if (__any_sync(0xffffffffu, suspect)) {
+    bool twice = false;
 #pragma unroll 1
     for (int k = lane; k < KP; k += 32) {
-      bool earlier = false;
-      for (int j = 0; j < k; ++j) earlier |= li.idx[j] == li.idx[k];
-      li.x[k] = earlier ? 1.f : 0.f;
+      const int own = li.idx[k];
+      int hits = 0;
+#pragma unroll 2
+      for (int j = 0; j < KP; j += 4) {
+        const int4 o = *reinterpret_cast<const int4*>(li.idx + j);
+        hits += (o.x == own) + (o.y == own) + (o.z == own) + (o.w == own);
+      }
+      twice |= own >= 0 && hits > 1;
     }
-    __syncwarp();
-    for (int k = lane; k < KP; k += 32) if (li.x[k] != 0.f) li.idx[k] = -1;
-    __syncwarp();
+    if (__any_sync(0xffffffffu, twice)) {                       // every slot but the first of its index goes
+      bad = true;
+#pragma unroll 1
+      for (int k = lane; k < KP; k += 32) {
+        bool earlier = false;
+        for (int j = 0; j < k; ++j) earlier |= li.idx[j] == li.idx[k];
+        li.x[k] = earlier ? 1.f : 0.f;
+      }
+      __syncwarp();
+      for (int k = lane; k < KP; k += 32) if (li.x[k] != 0.f) { li.idx[k] = -1; li.p[k] = -INFINITY; }
+      __syncwarp();
+    }
   }
   h.bad = __any_sync(0xffffffffu, bad);
   int cnt = 0;
-  double zm = -INFINITY;
+  if (p.t_lse) {
 #pragma unroll 1
-  for (int k = lane; k < KP; k += 32) {
-    const bool valid = li.idx[k] >= 0;
-    const double z = valid ? li.p[k] : -INFINITY;
-    li.p[k] = z;
-    cnt += valid;
-    zm = z > zm || z != z ? z : zm;
-  }
-  cnt = __reduce_add_sync(0xffffffffu, cnt);
-  if (!p.t_lse) {
+    for (int k = lane; k < KP; k += 32) cnt += li.idx[k] >= 0;
+    cnt = __reduce_add_sync(0xffffffffu, cnt);
+  } else {
+    double zm = -INFINITY;
+#pragma unroll 1
+    for (int k = lane; k < KP; k += 32) { const double z = li.p[k]; zm = z > zm || z != z ? z : zm; }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) { const double v = __shfl_xor_sync(0xffffffffu, zm, o); zm = v > zm || v != v ? v : zm; }
     double e = 0.;
 #pragma unroll 1
-    for (int k = lane; k < KP; k += 32) if (li.p[k] != -INFINITY) e += exp(li.p[k] - zm);
+    for (int k = lane; k < KP; k += 32) if (li.p[k] != -INFINITY) e += exp_list(li.p[k] - zm);
     lse_t = zm + log(warp_sum_f64(e));
   }
 #pragma unroll 1
@@ -202,7 +233,7 @@ __device__ __forceinline__ void distill_prepare(const DistillParams& p, int64_t 
     const double z = li.p[k];
     double pk = 0.;
     if (z != -INFINITY) {
-      pk = exp(z - lse_t);
+      pk = exp_list(z - lse_t);
       h.psum += pk;
       if (pk != 0.) h.ent += pk * (z - lse_t);
     }
@@ -235,8 +266,8 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
   const int64_t row0 = blockIdx.x / C, stride = gridDim.x / C;
   const float c = (float)(p.inv_temp * 1.4426950408889634);
   if (threadIdx.x == 0) {
-    for (int s = 0; s < R; ++s) { mbar_init(sm.full + s, 1); mbar_init(sm.marked + s, 1); mbar_init(sm.consumed + s, MW); mbar_init(sm.stored + s, MW); }
-    for (int i = 0; i < 2; ++i) mbar_init(sm.rec_bar + i, C);
+    for (int s = 0; s < R; ++s) { mbar_init(sm.full + s, 1); mbar_init(sm.marked + s, 1); mbar_init(sm.stored + s, MW); }
+    for (int i = 0; i < 2; ++i) mbar_init(sm.rec_bar + i, 1);
     mbar_fence_init();
   }
   __syncthreads();
@@ -273,15 +304,17 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
     if (row < p.rows) {
       const float w0 = p.w_rows ? p.w_rows[row] : p.w_scalar;
       if (w0 != 0.f) issue(row);
-      distill_prepare<T>(p, row, list_of(0), KP, lane, h);
+      distill_prepare<T>(p, row, list_of(0), sm.seen[s], KP, lane, h);
     }
+    // vectors of gradient and logits coincide: whole vectors leave by bulk copy, otherwise the slot is copied out by element
+    const bool same = ((reinterpret_cast<uint64_t>(dL) ^ reinterpret_cast<uint64_t>(L)) & 15) == 0;
     for (; row < p.rows; row += (int64_t)R * stride, b ^= 1, h = hn) {
       const bool skip = h.w == 0.f;
       const RowVecs<T> rv(L + row * V, V);
-      const int v0 = (int)((int64_t)rv.nvec * rank / C), v1 = (int)((int64_t)rv.nvec * (rank + 1) / C);
-      const int jlo = v0 * VEC - rv.head, jhi = v1 * VEC - rv.head;          // row elements of this CTA: [jlo, jhi)
+      const int v0 = (int)((int64_t)rv.nvec * rank / C), n = (int)((int64_t)rv.nvec * (rank + 1) / C) - v0;
+      const int j0 = v0 * VEC - rv.head, j1 = j0 + n * VEC;                  // row elements of this CTA: [j0, j1)
+      const int ilo = j0 < 0 ? 1 : 0, ihi = j1 > V ? n - 1 : n;              // vectors [ilo, ihi) lie wholly inside the row
       const DistillList li = list_of(b);
-      float xe[2] = {-INFINITY, -INFINITY};                     // edge vectors' elements, for the lanes below VEC
       if (!skip) {
         // ---- the listed logits out of the staged row ----
         if (!mbar_wait_bounded_warp(sm.full + s, full_ph, kDevErrStageTimeout)) break;
@@ -289,12 +322,12 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
         if (lane < VEC) {
           // foreign elements, and edge vectors that were not copied because they reach outside the tensor
           for (int side = 0; side < 2; ++side) {
-            const int v = side ? v1 - 1 : v0;
-            if (v < v0 || v >= v1 || (side && v == v0)) continue;
-            const uint64_t a = reinterpret_cast<uint64_t>(rv.base) + (uint64_t)v * 16;
-            const int j = v * VEC - rv.head + lane;
-            if (j < 0 || j >= V) sx[(v - v0) * VEC + lane] = Elem<T>::from_f32(-INFINITY);
-            else if (a < t_begin || a + 16 > t_end) sx[(v - v0) * VEC + lane] = L[row * V + j];
+            const int i = side ? n - 1 : 0;
+            if (i < 0 || (side && i == 0) || (i >= ilo && i < ihi)) continue;
+            const uint64_t a = reinterpret_cast<uint64_t>(rv.base) + (uint64_t)(v0 + i) * 16;
+            const int j = j0 + i * VEC + lane;
+            if (j < 0 || j >= V) sx[i * VEC + lane] = Elem<T>::from_f32(-INFINITY);
+            else if (a < t_begin || a + 16 > t_end) sx[i * VEC + lane] = L[row * V + j];
           }
         }
         __syncwarp();
@@ -302,7 +335,7 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
         for (int k = lane; k < KP; k += 32) {
           const int id = li.idx[k];
           float x = -INFINITY;
-          if (id >= 0 && id >= jlo && id < jhi) { x = Elem<T>::to_f32(sx[id - jlo]); sx[id - jlo] = Elem<T>::from_f32(-INFINITY); }
+          if (id >= 0 && id >= j0 && id < j1) { x = Elem<T>::to_f32(sx[id - j0]); sx[id - j0] = Elem<T>::from_f32(-INFINITY); }
           li.x[k] = x;
           mt = fmaxf(mt, x);
         }
@@ -315,49 +348,56 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
           const double wc = (double)h.w * p.inv_temp;
           sm.row[s] = DistillRow{mt, zt, (float)(wc * (h.psum + h.r)), (float)(wc * h.r), 0};
         }
-        __syncwarp();
-        if (HOLD && BWD && lane < VEC) {
-          if (v1 > v0) xe[0] = Elem<T>::to_f32(sx[lane]);
-          if (v1 > v0 + 1) xe[1] = Elem<T>::to_f32(sx[(v1 - 1 - v0) * VEC + lane]);
-        }
       } else if (lane == 0) {
         sm.row[s] = DistillRow{0.f, 0.f, 0.f, 0.f, 1};
       }
       __syncwarp();
       if (lane == 0) distill_arrive(sm.marked + s);
-      // ---- the next row's list; its fetch once the main warps have taken this row out of the slot ----
       const int64_t next = row + (int64_t)R * stride;
-      if (next < p.rows) distill_prepare<T>(p, next, list_of(b ^ 1), KP, lane, hn);
-      if (!mbar_wait_bounded_warp(sm.consumed + s, ph, kDevErrStageTimeout)) break;
-      if (next < p.rows && hn.w != 0.f) issue(next);
-      // ---- the row is done: listed positions and loss ----
+      if (next < p.rows) distill_prepare<T>(p, next, list_of(b ^ 1), sm.seen[s], KP, lane, hn);
+      // ---- the row's gradient is in the slot: listed positions, off with it, loss ----
       if (!mbar_wait_bounded_warp(sm.stored + s, ph, kDevErrStageTimeout)) break;
       ph ^= 1u;
       if (skip) {
         if (lane == 0 && rank == 0 && p.loss_rows) p.loss_rows[row] = 0.f;
+        if (next < p.rows && hn.w != 0.f) issue(next);
         continue;
       }
       const DistillFin f = sm.fin[s];
       const double mass = h.psum + h.r;
       if (BWD) {
-        T* drow = dL + row * V;
+        T* dpart = dL + row * V + j0;
         const double wc = (double)h.w * p.inv_temp;
         const float ref = f.m == -INFINITY ? 0.f : f.m;
-        if (HOLD && lane < VEC) {
-          // edge vectors, which the main warps leave out
-          const float g = mass != 0. ? (float)(wc * mass / (double)f.z_all - (h.r > 0. && f.z_rest > 0.f ? wc * h.r / (double)f.z_rest : 0.)) : 0.f;
-          for (int side = 0; side < 2; ++side) {
-            const int v = side ? v1 - 1 : v0;
-            const int j0 = v * VEC - rv.head;
-            if (v < v0 || v >= v1 || (side && v == v0) || (j0 >= 0 && j0 + VEC <= V)) continue;
-            if (j0 + lane >= 0 && j0 + lane < V) distill_put<T>(drow + j0 + lane, exp_rel(xe[side], ref, c) * g, beta);
+        const float ga = mass != 0. ? (float)(wc * mass / (double)f.z_all) : 0.f;
+        for (int k = lane; k < KP; k += 32) {
+          const int at = li.idx[k] - j0;
+          if (li.idx[k] >= 0 && at >= 0 && at < j1 - j0) {
+            // (in Accumulate mode the old value is there already, unless it is added when the element is copied out)
+            const int i = at / VEC;
+            distill_put<T>(sx + at, exp_rel(li.x[k], ref, c) * ga - (float)(wc * li.p[k]), beta && same && i >= ilo && i < ihi);
           }
         }
         __syncwarp();
-        const float ga = mass != 0. ? (float)(wc * mass / (double)f.z_all) : 0.f;
-        for (int k = lane; k < KP; k += 32) {
-          const int id = li.idx[k];
-          if (id >= 0 && id >= jlo && id < jhi) distill_put<T>(drow + id, exp_rel(li.x[k], ref, c) * ga - (float)(wc * li.p[k]), beta);
+        if (same) {
+          if (lane < VEC) {
+            for (int side = 0; side < 2; ++side) {
+              const int i = side ? n - 1 : 0;
+              if (i < 0 || (side && i == 0) || (i >= ilo && i < ihi)) continue;
+              const int e = i * VEC + lane;
+              if (j0 + e >= 0 && j0 + e < V) distill_put<T>(dpart + e, Elem<T>::to_f32(sx[e]), beta);
+            }
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0 && ihi > ilo) {
+            bulk_s2g(dpart + ilo * VEC, sx + ilo * VEC, (unsigned)(ihi - ilo) * 16u);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+        } else {
+          const int e0 = j0 < 0 ? -j0 : 0, e1 = j1 > V ? V - j0 : j1 - j0;
+          for (int e = e0 + lane; e < e1; e += 32) distill_put<T>(dpart + e, Elem<T>::to_f32(sx[e]), beta);
+          __syncwarp();
         }
       }
       if (rank == 0 && p.loss_rows) {
@@ -368,21 +408,27 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
           const double pk = li.p[k];
           if (pk != 0.) {
             const int id = li.idx[k];
-            const float x = id >= jlo && id < jhi ? li.x[k] : Elem<T>::to_f32(L[row * V + id]);
+            const float x = id >= j0 && id < j1 ? li.x[k] : Elem<T>::to_f32(L[row * V + id]);
             px += pk * ((double)x - (double)f.m);
           }
         }
         px = warp_sum_f64(px);
+        // the three logarithms side by side
+        const double lg = log(lane == 0 ? (double)f.z_all : lane == 1 ? h.r : (double)f.z_rest);
+        const double la = __shfl_sync(0xffffffffu, lg, 0), lr = __shfl_sync(0xffffffffu, lg, 1), lz = __shfl_sync(0xffffffffu, lg, 2);
         if (lane == 0) {
-          const double la = log((double)f.z_all);
           double loss = mass != 0. ? h.ent - p.inv_temp * px + h.psum * la : 0.;
-          if (h.r > 0.) loss += h.r * (log(h.r) - log((double)f.z_rest) + la);
+          if (h.r > 0.) loss += h.r * (lr - lz + la);
           p.loss_rows[row] = h.bad ? __int_as_float(0x7fc00000) : (float)loss;
         }
       }
       if (lane == 0 && rank == 0 && h.bad && p.status) atomicMax(p.status, (unsigned)CACTI_B200_ERR_INDEX_RANGE);
+      // the slot may be filled again once the copy out has read it
+      if (BWD && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
       __syncwarp();
+      if (next < p.rows && hn.w != 0.f) issue(next);
     }
+    if (BWD && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   } else {
     // ---------------- main warps ----------------
     const int t = threadIdx.x;
@@ -398,41 +444,62 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
       // vectors [ilo, ihi) of this part lie wholly inside the row
       const int ilo = j0 < 0 ? 1 : 0, ihi = j0 + n * VEC > V ? n - 1 : n;
       T* dpart = BWD ? dL + row * V + j0 : nullptr;
-      const bool vec_ok = BWD && (HOLD || ((reinterpret_cast<uint64_t>(dL) ^ reinterpret_cast<uint64_t>(L)) & 15) == 0);
+      const bool same = BWD && ((reinterpret_cast<uint64_t>(dL) ^ reinterpret_cast<uint64_t>(L)) & 15) == 0;
       if (info.skip) {
         if (BWD && !beta) {
           const T zero = Elem<T>::from_f32(0.f);
           for (int i = t; i < n; i += MT) {
-            if (vec_ok && i >= ilo && i < ihi) st_stream(dpart + i * VEC, make_uint4(0, 0, 0, 0));
+            if (same && i >= ilo && i < ihi) st_stream(dpart + i * VEC, make_uint4(0, 0, 0, 0));
             else for (int e = 0; e < VEC; ++e) if (j0 + i * VEC + e >= 0 && j0 + i * VEC + e < V) dpart[i * VEC + e] = zero;
           }
         }
-        if (lane == 0) { distill_arrive(sm.consumed + s); distill_arrive(sm.stored + s); }
+        if (lane == 0) distill_arrive(sm.stored + s);
         if (++s == R) { s = 0; ph ^= 1u; }
         if (gave_up) break;
         continue;
       }
-      const uint4* srow = reinterpret_cast<const uint4*>(ring + (size_t)s * slot_bytes);
+      uint4* srow = reinterpret_cast<uint4*>(ring + (size_t)s * slot_bytes);
       // maximum and exponentials against the warp's own maximum
       constexpr int NV = HOLD ? kDistillNV : 1;
       float a[NV][VEC];
       float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, zq[4] = {0.f, 0.f, 0.f, 0.f};
       float mw, ref;
       if (HOLD) {
+        // (the row is read from shared memory twice: its raw vectors beside the exponentials would not fit the registers)
+        mw = -INFINITY;
+        if constexpr (sizeof(T) == 2) {
+          // the maximum on packed pairs: a quarter of the instructions, and the same value
+          using P2 = typename Pair16<T>::type;
+          P2 mp[2] = {Pair16<T>::neg_inf(), Pair16<T>::neg_inf()};
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-          if (t + k * MT < n) {
-            unpack<T>(srow[t + k * MT], a[k]);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) mq[e & 3] = fmaxf(mq[e & 3], a[k][e]);
+          for (int k = 0; k < NV; ++k) {
+            if (t + k * MT < n) {
+              const uint4 raw = srow[t + k * MT];
+              const P2* q = reinterpret_cast<const P2*>(&raw);
+              mp[0] = __hmax2(mp[0], __hmax2(q[0], q[1]));
+              mp[1] = __hmax2(mp[1], __hmax2(q[2], q[3]));
+            }
           }
+          mp[0] = __hmax2(mp[0], mp[1]);
+          mw = fmaxf(Elem<T>::to_f32(mp[0].x), Elem<T>::to_f32(mp[0].y));
+        } else {
+#pragma unroll
+          for (int k = 0; k < NV; ++k) {
+            if (t + k * MT < n) {
+              float x[VEC];
+              unpack<T>(srow[t + k * MT], x);
+#pragma unroll
+              for (int e = 0; e < VEC; ++e) mq[e & 3] = fmaxf(mq[e & 3], x[e]);
+            }
+          }
+          mw = fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3]));
         }
-        mw = warp_reduce<MaxOp>(fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])));
-        if (lane == 0) distill_arrive(sm.consumed + s);         // the reduction has ordered the warp's reads before it
+        mw = warp_reduce<MaxOp>(mw);
         ref = mw == -INFINITY ? 0.f : mw;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
           if (t + k * MT < n) {
+            unpack<T>(srow[t + k * MT], a[k]);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) { a[k][e] = exp_rel(a[k][e], ref, c); zq[e & 3] += a[k][e]; }
           }
@@ -465,12 +532,15 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
       float m_top = info.m_top, z_top = info.z_top;
       if (C > 1) {
         // every CTA hands its part to all of the cluster; the parts are combined in rank order everywhere
-        if (warp == 0 && lane < C) {
-          uint32_t dst, bar;
-          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(dst) : "r"(smem_u32(&sm.rec[par][rank])), "r"(lane));
-          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(smem_u32(&sm.rec_bar[par])), "r"(lane));
-          asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "f"(m), "f"(z_rest), "f"(m_top), "f"(z_top) : "memory");
-          asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+        if (warp == 0) {
+          if (lane == 0) mbar_expect_tx(sm.rec_bar + par, (unsigned)(C * sizeof(DistillRec)));
+          if (lane < C) {
+            uint32_t dst, bar;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(dst) : "r"(smem_u32(&sm.rec[par][rank])), "r"(lane));
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(smem_u32(&sm.rec_bar[par])), "r"(lane));
+            asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];"
+                         ::"r"(dst), "f"(m), "f"(z_rest), "f"(m_top), "f"(z_top), "r"(bar) : "memory");
+          }
         }
         gave_up = !__all_sync(0xffffffffu, distill_wait_cluster(sm.rec_bar + par, rph[par]));
         rph[par] ^= 1u;
@@ -497,35 +567,26 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
 #pragma unroll
           for (int k = 0; k < NV; ++k) {
             const int i = t + k * MT;
-            if (i >= ilo && i < ihi) {
-              T* o = dpart + i * VEC;
+            if (i < n) {
 #pragma unroll
               for (int e = 0; e < VEC; ++e) a[k][e] *= f;
-              if (beta) st_stream(o, pack_accumulate<T>(a[k], ld_stream(o)));
-              else st_stream(o, pack<T>(a[k]));
+              if (beta && same && i >= ilo && i < ihi) srow[i] = pack_accumulate<T>(a[k], ld_stream(dpart + i * VEC));
+              else srow[i] = pack<T>(a[k]);
             }
           }
         } else {
           for (int i = t; i < n; i += MT) {
             unpack<T>(srow[i], a[0]);
-            T* o = dpart + i * VEC;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) a[0][e] = exp_rel(a[0][e], mref, c) * g;
-            if (vec_ok && i >= ilo && i < ihi) {
-              if (beta) st_stream(o, pack_accumulate<T>(a[0], ld_stream(o)));
-              else st_stream(o, pack<T>(a[0]));
-            } else {
-#pragma unroll
-              for (int e = 0; e < VEC; ++e) if (j0 + i * VEC + e >= 0 && j0 + i * VEC + e < V) distill_put<T>(o + e, a[0][e], beta);
-            }
+            if (beta && same && i >= ilo && i < ihi) srow[i] = pack_accumulate<T>(a[0], ld_stream(dpart + i * VEC));
+            else srow[i] = pack<T>(a[0]);
           }
         }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // written here, read by the copy out
       }
       __syncwarp();
-      if (lane == 0) {
-        if (!HOLD) distill_arrive(sm.consumed + s);
-        distill_arrive(sm.stored + s);
-      }
+      if (lane == 0) distill_arrive(sm.stored + s);
       if (++s == R) { s = 0; ph ^= 1u; }
       if (gave_up) break;
     }
@@ -599,10 +660,8 @@ static int launch_distill(uint64_t dl, uint64_t l, const DistillParams& p, cudaS
   const unsigned part = (unsigned)((nvec + C - 1) / C + 1) * 16;
   const unsigned slot = (part + 127) / 128 * 128;
   const int per = (nvec + C - 1) / C;
-  // registers hold the exponentials where vectors of logits and gradient coincide; a shifted gradient is stored by element
-  const bool same = !dl || ((dl ^ l) & 15) == 0;
-  if (same && per <= 4 * 32 * kDistillNV) return launch_distill_as<T, 4, 3, true>(dl, l, p, C, slot, st);
-  if (same && per <= 16 * 32 * kDistillNV) return launch_distill_as<T, 16, 3, true>(dl, l, p, C, slot, st);
+  if (per <= 4 * 32 * kDistillNV) return launch_distill_as<T, 4, 3, true>(dl, l, p, C, slot, st);
+  if (per <= 16 * 32 * kDistillNV) return launch_distill_as<T, 16, 3, true>(dl, l, p, C, slot, st);
   return launch_distill_as<T, 16, 1, false>(dl, l, p, C, slot, st);
 }
 
