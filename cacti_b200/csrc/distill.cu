@@ -81,19 +81,27 @@ __device__ __forceinline__ double warp_sum_f64(double v) {
 constexpr int kDistillNV = 8;                                  // vectors a main thread holds
 constexpr int kDistillMaxC = 8;
 constexpr int kDistillSeen = 128;                              // words of a list's index filter
+// What exponentials are taken against: e(x) = 2^((x - sub) c + off).  Ordinarily sub = 0 and off = -(a large logit times c,
+// rounded to a whole number): one multiply-add an exponential, and two references differ by an exact power of two.  Where that
+// product is no longer a small whole number (rows near the type's largest magnitudes) sub is the row's maximum and off = 0.
+struct DistillRef { float sub, off; };
 struct DistillRow {              // from the list warp to the main warps
-  float m_top, z_top;            // maximum of the listed logits (of this CTA's vectors) and sum of their exponentials
+  DistillRef ref;                // from the listed logits and a sample of the others; off = NaN: none to be had
+  float z_top;                   // sum of the listed exponentials (of this CTA's vectors)
   float g_mass, g_r;             // w c P and w c r
   int skip;                      // weight 0
 };
-struct DistillFin { float m, z_all, z_rest; };                 // back to the list warp
-struct alignas(16) DistillRec { float m, z_rest, m_top, z_top; };          // a CTA's part of a row, to the cluster
+// A sum of exponentials under its reference.  Listed and unlisted positions keep references of their own until the end: where
+// the list holds nearly everything, the rest is still known.
+struct alignas(16) DistillSum { DistillRef ref; float z, pad; };
+struct DistillFin { DistillRef ref; float z_all, z_rest, shift_rest; };      // back to the list warp
+struct DistillRec { DistillSum rest, top; };                   // a CTA's part of a row, to the cluster
 
 template <int MW, int R> struct alignas(16) DistillSmem {
   uint64_t full[R], marked[R], stored[R];
   uint64_t rec_bar[2];
   DistillRec rec[2][kDistillMaxC];
-  float2 red[2][MW];
+  float red[2][MW];
   DistillRow row[R];
   DistillFin fin[R];
   unsigned seen[R][kDistillSeen];
@@ -125,9 +133,60 @@ __device__ __forceinline__ bool distill_wait_cluster(uint64_t* bar, unsigned par
   return false;
 }
 
-// 2^((x - m) c); m is finite or the result is meant to be NaN.  The difference comes first: rows near the type's largest
-// magnitudes then lose nothing, and the multiply it costs hides behind the ex2 unit, which is the slower one.
-__device__ __forceinline__ float exp_rel(float x, float m, float c) { return exp2f_approx((x - m) * c); }
+__device__ __forceinline__ float distill_arg(float x, const DistillRef& r, float c) { return fmaf(x - r.sub, c, r.off); }
+__device__ __forceinline__ float distill_exp(float x, const DistillRef& r, float c) { return exp2f_approx(distill_arg(x, r, c)); }
+// The reference for a largest logit m.
+__device__ __forceinline__ DistillRef distill_ref(float m, float c) {
+  const float a = m * c;
+  return fabsf(a) < 4194304.f ? DistillRef{0.f, -rintf(a)} : DistillRef{m, 0.f};
+}
+// log2 of e under a over e under b; positive where b's logits are the larger ones
+__device__ __forceinline__ float distill_shift(const DistillRef& a, const DistillRef& b, float c) {
+  return (float)(((double)b.sub - (double)a.sub) * (double)c + ((double)a.off - (double)b.off));
+}
+
+// two f32 operations an instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+// a + b under the larger reference
+__device__ __forceinline__ DistillSum distill_add(const DistillSum& a, const DistillSum& b, float c) {
+  if (a.z == 0.f) return b;
+  if (b.z == 0.f) return a;
+  const float s = distill_shift(a.ref, b.ref, c);
+  if (s > 0.f) return DistillSum{b.ref, fmaf(a.z, exp2f_approx(-s), b.z), 0.f};
+  return DistillSum{a.ref, fmaf(b.z, exp2f_approx(s), a.z), 0.f};
+}
+// CTA-wide sum or maximum over the main warps (barrier 1); `any` ORs a flag on the way.
+template <typename Op, int MW> __device__ __forceinline__ float distill_combine(float v, float (&red)[MW], int warp, int lane, bool& any) {
+  v = warp_reduce<Op>(v);
+  if (lane == 0) red[warp] = v;
+  unsigned r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %2, 0;\n\tbar.red.or.pred p, 1, %1, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r) : "n"(MW * 32), "r"((unsigned)any) : "memory");
+  any = r != 0;
+  float s = red[0];
+#pragma unroll
+  for (int i = 1; i < MW; ++i) s = Op::f(s, red[i]);
+  return s;
+}
 
 template <typename T> __device__ __forceinline__ void distill_put(T* o, float v, int beta) {
   *o = beta ? Elem<T>::from_f32(Elem<T>::to_f32(*o) + round_to<T>(v)) : Elem<T>::from_f32(v);
@@ -263,7 +322,7 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
   unsigned char* ring = smem_raw + (sizeof(Smem) + (size_t)2 * R * KP * kDistillListBytes + 127) / 128 * 128;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, V = p.vocab;
   const int C = (int)distill_nctas(), rank = (int)distill_ctarank();
-  const int64_t row0 = blockIdx.x / C, stride = gridDim.x / C;
+  const int rows = (int)p.rows, row0 = (int)blockIdx.x / C, stride = (int)gridDim.x / C;
   const float c = (float)(p.inv_temp * 1.4426950408889634);
   if (threadIdx.x == 0) {
     for (int s = 0; s < R; ++s) { mbar_init(sm.full + s, 1); mbar_init(sm.marked + s, 1); mbar_init(sm.stored + s, MW); }
@@ -283,10 +342,10 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
       return DistillList{reinterpret_cast<double*>(at), reinterpret_cast<float*>(at + 8 * KP), reinterpret_cast<int*>(at + 12 * KP)};
     };
     // fetch a row's vectors of this CTA; whole vectors inside the tensor only
-    auto issue = [&](int64_t row) {
+    auto issue = [&](int row) {
       if (lane == 0) {
-        const RowVecs<T> rv(L + row * V, V);
-        const int v0 = (int)((int64_t)rv.nvec * rank / C), v1 = (int)((int64_t)rv.nvec * (rank + 1) / C);
+        const RowVecs<T> rv(L + (int64_t)row * V, V);
+        const int v0 = rv.nvec * rank / C, v1 = rv.nvec * (rank + 1) / C;
         const unsigned char *a = rv.base + (size_t)v0 * 16, *b = rv.base + (size_t)v1 * 16;
         unsigned skip = 0;
         if (reinterpret_cast<uint64_t>(a) < t_begin) { a += 16; skip = 16; }
@@ -300,18 +359,18 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
     unsigned ph = 0, full_ph = 0;                               // rows of weight 0 do not pass through `full`
     int b = 0;
     DistillHead h, hn;
-    int64_t row = row0 + s * stride;
-    if (row < p.rows) {
+    int row = row0 + s * stride;
+    if (row < rows) {
       const float w0 = p.w_rows ? p.w_rows[row] : p.w_scalar;
       if (w0 != 0.f) issue(row);
       distill_prepare<T>(p, row, list_of(0), sm.seen[s], KP, lane, h);
     }
     // vectors of gradient and logits coincide: whole vectors leave by bulk copy, otherwise the slot is copied out by element
     const bool same = ((reinterpret_cast<uint64_t>(dL) ^ reinterpret_cast<uint64_t>(L)) & 15) == 0;
-    for (; row < p.rows; row += (int64_t)R * stride, b ^= 1, h = hn) {
+    for (; row < rows; row += R * stride, b ^= 1, h = hn) {
       const bool skip = h.w == 0.f;
-      const RowVecs<T> rv(L + row * V, V);
-      const int v0 = (int)((int64_t)rv.nvec * rank / C), n = (int)((int64_t)rv.nvec * (rank + 1) / C) - v0;
+      const RowVecs<T> rv(L + (int64_t)row * V, V);
+      const int v0 = rv.nvec * rank / C, n = rv.nvec * (rank + 1) / C - v0;
       const int j0 = v0 * VEC - rv.head, j1 = j0 + n * VEC;                  // row elements of this CTA: [j0, j1)
       const int ilo = j0 < 0 ? 1 : 0, ihi = j1 > V ? n - 1 : n;              // vectors [ilo, ihi) lie wholly inside the row
       const DistillList li = list_of(b);
@@ -327,10 +386,11 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
             const uint64_t a = reinterpret_cast<uint64_t>(rv.base) + (uint64_t)(v0 + i) * 16;
             const int j = j0 + i * VEC + lane;
             if (j < 0 || j >= V) sx[i * VEC + lane] = Elem<T>::from_f32(-INFINITY);
-            else if (a < t_begin || a + 16 > t_end) sx[i * VEC + lane] = L[row * V + j];
+            else if (a < t_begin || a + 16 > t_end) sx[i * VEC + lane] = L[(int64_t)row * V + j];
           }
         }
         __syncwarp();
+        // a large logit of this part: the listed ones, and one vector a lane of the rest
         float mt = -INFINITY;
         for (int k = lane; k < KP; k += 32) {
           const int id = li.idx[k];
@@ -339,43 +399,51 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
           li.x[k] = x;
           mt = fmaxf(mt, x);
         }
+        if (n > 0) {
+          float x[VEC];
+          unpack<T>(reinterpret_cast<const uint4*>(sx)[lane * n / 32], x);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) mt = fmaxf(mt, x[e]);
+        }
         mt = warp_reduce<MaxOp>(mt);
-        const float ref = mt == -INFINITY ? 0.f : mt;
+        DistillRef ref = distill_ref(mt, c);
+        if (isinf(mt)) ref = DistillRef{0.f, 0.f};
         float zt = 0.f;
-        for (int k = lane; k < KP; k += 32) zt += exp_rel(li.x[k], ref, c);
+        for (int k = lane; k < KP; k += 32) zt += distill_exp(li.x[k], ref, c);
         zt = warp_reduce<SumOp>(zt);
         if (lane == 0) {
           const double wc = (double)h.w * p.inv_temp;
-          sm.row[s] = DistillRow{mt, zt, (float)(wc * (h.psum + h.r)), (float)(wc * h.r), 0};
+          // without a usable sample the main warps look for the maximum themselves
+          if (isinf(mt)) ref.off = __int_as_float(0x7fc00000);
+          sm.row[s] = DistillRow{ref, zt, (float)(wc * (h.psum + h.r)), (float)(wc * h.r), 0};
         }
       } else if (lane == 0) {
-        sm.row[s] = DistillRow{0.f, 0.f, 0.f, 0.f, 1};
+        sm.row[s] = DistillRow{DistillRef{0.f, 0.f}, 0.f, 0.f, 0.f, 1};
       }
       __syncwarp();
       if (lane == 0) distill_arrive(sm.marked + s);
-      const int64_t next = row + (int64_t)R * stride;
-      if (next < p.rows) distill_prepare<T>(p, next, list_of(b ^ 1), sm.seen[s], KP, lane, hn);
+      const int next = row + R * stride;
+      if (next < rows) distill_prepare<T>(p, next, list_of(b ^ 1), sm.seen[s], KP, lane, hn);
       // ---- the row's gradient is in the slot: listed positions, off with it, loss ----
       if (!mbar_wait_bounded_warp(sm.stored + s, ph, kDevErrStageTimeout)) break;
       ph ^= 1u;
       if (skip) {
         if (lane == 0 && rank == 0 && p.loss_rows) p.loss_rows[row] = 0.f;
-        if (next < p.rows && hn.w != 0.f) issue(next);
+        if (next < rows && hn.w != 0.f) issue(next);
         continue;
       }
       const DistillFin f = sm.fin[s];
       const double mass = h.psum + h.r;
       if (BWD) {
-        T* dpart = dL + row * V + j0;
+        T* dpart = dL + (int64_t)row * V + j0;
         const double wc = (double)h.w * p.inv_temp;
-        const float ref = f.m == -INFINITY ? 0.f : f.m;
         const float ga = mass != 0. ? (float)(wc * mass / (double)f.z_all) : 0.f;
         for (int k = lane; k < KP; k += 32) {
           const int at = li.idx[k] - j0;
           if (li.idx[k] >= 0 && at >= 0 && at < j1 - j0) {
             // (in Accumulate mode the old value is there already, unless it is added when the element is copied out)
             const int i = at / VEC;
-            distill_put<T>(sx + at, exp_rel(li.x[k], ref, c) * ga - (float)(wc * li.p[k]), beta && same && i >= ilo && i < ihi);
+            distill_put<T>(sx + at, distill_exp(li.x[k], f.ref, c) * ga - (float)(wc * li.p[k]), beta && same && i >= ilo && i < ihi);
           }
         }
         __syncwarp();
@@ -401,15 +469,15 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
         }
       }
       if (rank == 0 && p.loss_rows) {
-        // sum p (x_k - m): differences to the maximum, so that a row of values like the type's lowest loses nothing.
-        // Listed logits of the cluster's other parts are read from memory.
+        // sum p log2 e(x_k), in the arithmetic of the exponentials.  Listed logits of the cluster's other parts are read from
+        // memory.
         double px = 0.;
         for (int k = lane; k < KP; k += 32) {
           const double pk = li.p[k];
           if (pk != 0.) {
             const int id = li.idx[k];
-            const float x = id >= j0 && id < j1 ? li.x[k] : Elem<T>::to_f32(L[row * V + id]);
-            px += pk * ((double)x - (double)f.m);
+            const float x = id >= j0 && id < j1 ? li.x[k] : Elem<T>::to_f32(L[(int64_t)row * V + id]);
+            px += pk * (((double)x - (double)f.ref.sub) * (double)c + (double)f.ref.off);
           }
         }
         px = warp_sum_f64(px);
@@ -417,8 +485,8 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
         const double lg = log(lane == 0 ? (double)f.z_all : lane == 1 ? h.r : (double)f.z_rest);
         const double la = __shfl_sync(0xffffffffu, lg, 0), lr = __shfl_sync(0xffffffffu, lg, 1), lz = __shfl_sync(0xffffffffu, lg, 2);
         if (lane == 0) {
-          double loss = mass != 0. ? h.ent - p.inv_temp * px + h.psum * la : 0.;
-          if (h.r > 0.) loss += h.r * (lr - lz + la);
+          double loss = mass != 0. ? h.ent - 0.6931471805599453 * px + h.psum * la : 0.;
+          if (h.r > 0.) loss += h.r * (lr - lz - 0.6931471805599453 * (double)f.shift_rest + la);
           p.loss_rows[row] = h.bad ? __int_as_float(0x7fc00000) : (float)loss;
         }
       }
@@ -426,24 +494,24 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
       // the slot may be filled again once the copy out has read it
       if (BWD && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
       __syncwarp();
-      if (next < p.rows && hn.w != 0.f) issue(next);
+      if (next < rows && hn.w != 0.f) issue(next);
     }
     if (BWD && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   } else {
     // ---------------- main warps ----------------
     const int t = threadIdx.x;
     int s = 0;
-    unsigned ph = 0, par = 0, rph[2] = {0, 0};
-    for (int64_t row = row0; row < p.rows; row += stride) {
+    unsigned ph = 0, par = 0, rpar = 0, rph[2] = {0, 0};
+    for (int row = row0; row < rows; row += stride) {
       // a wait that ran out is agreed on at the CTA's barrier below; until then the warp goes on with what is there
       bool gave_up = !mbar_wait_bounded_warp(sm.marked + s, ph, kDevErrStageTimeout);
       const DistillRow info = sm.row[s];
-      const RowVecs<T> rv(L + row * V, V);
-      const int v0 = (int)((int64_t)rv.nvec * rank / C), n = (int)((int64_t)rv.nvec * (rank + 1) / C) - v0;
+      const RowVecs<T> rv(L + (int64_t)row * V, V);
+      const int v0 = rv.nvec * rank / C, n = rv.nvec * (rank + 1) / C - v0;
       const int j0 = v0 * VEC - rv.head;                        // row element of this part's first vector
       // vectors [ilo, ihi) of this part lie wholly inside the row
       const int ilo = j0 < 0 ? 1 : 0, ihi = j0 + n * VEC > V ? n - 1 : n;
-      T* dpart = BWD ? dL + row * V + j0 : nullptr;
+      T* dpart = BWD ? dL + (int64_t)row * V + j0 : nullptr;
       const bool same = BWD && ((reinterpret_cast<uint64_t>(dL) ^ reinterpret_cast<uint64_t>(L)) & 15) == 0;
       if (info.skip) {
         if (BWD && !beta) {
@@ -459,128 +527,124 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
         continue;
       }
       uint4* srow = reinterpret_cast<uint4*>(ring + (size_t)s * slot_bytes);
-      // maximum and exponentials against the warp's own maximum
       constexpr int NV = HOLD ? kDistillNV : 1;
-      float a[NV][VEC];
-      float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, zq[4] = {0.f, 0.f, 0.f, 0.f};
-      float mw, ref;
-      if (HOLD) {
-        // (the row is read from shared memory twice: its raw vectors beside the exponentials would not fit the registers)
-        mw = -INFINITY;
-        if constexpr (sizeof(T) == 2) {
-          // the maximum on packed pairs: a quarter of the instructions, and the same value
-          using P2 = typename Pair16<T>::type;
-          P2 mp[2] = {Pair16<T>::neg_inf(), Pair16<T>::neg_inf()};
-#pragma unroll
-          for (int k = 0; k < NV; ++k) {
-            if (t + k * MT < n) {
-              const uint4 raw = srow[t + k * MT];
-              const P2* q = reinterpret_cast<const P2*>(&raw);
-              mp[0] = __hmax2(mp[0], __hmax2(q[0], q[1]));
-              mp[1] = __hmax2(mp[1], __hmax2(q[2], q[3]));
-            }
-          }
-          mp[0] = __hmax2(mp[0], mp[1]);
-          mw = fmaxf(Elem<T>::to_f32(mp[0].x), Elem<T>::to_f32(mp[0].y));
-        } else {
-#pragma unroll
-          for (int k = 0; k < NV; ++k) {
-            if (t + k * MT < n) {
-              float x[VEC];
-              unpack<T>(srow[t + k * MT], x);
-#pragma unroll
-              for (int e = 0; e < VEC; ++e) mq[e & 3] = fmaxf(mq[e & 3], x[e]);
-            }
-          }
-          mw = fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3]));
-        }
-        mw = warp_reduce<MaxOp>(mw);
-        ref = mw == -INFINITY ? 0.f : mw;
+      float2 a[NV][VEC / 2];
+      DistillSum rest{info.ref, 0.f, 0.f};
+      const bool sampled = info.ref.off == info.ref.off;
+      bool held = HOLD && sampled && info.ref.sub == 0.f;
+      if (held) {
+        // ordinary rows: every logit read and exponentiated once
+        float2 zq[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        const float2 c2 = make_float2(c, c), off2 = make_float2(info.ref.off, info.ref.off);
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
           if (t + k * MT < n) {
-            unpack<T>(srow[t + k * MT], a[k]);
+            float x[VEC];
+            unpack<T>(srow[t + k * MT], x);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) { a[k][e] = exp_rel(a[k][e], ref, c); zq[e & 3] += a[k][e]; }
+            for (int e = 0; e < VEC / 2; ++e) {
+              a[k][e] = fma2(make_float2(x[2 * e], x[2 * e + 1]), c2, off2);
+              a[k][e].x = exp2f_approx(a[k][e].x);
+              a[k][e].y = exp2f_approx(a[k][e].y);
+              zq[e & 1] = add2(zq[e & 1], a[k][e]);
+            }
           }
         }
-      } else {
-        for (int v = t; v < n; v += MT) {
-          unpack<T>(srow[v], a[0]);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) mq[e & 3] = fmaxf(mq[e & 3], a[0][e]);
-        }
-        mw = warp_reduce<MaxOp>(fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])));
-        ref = mw == -INFINITY ? 0.f : mw;
-        for (int v = t; v < n; v += MT) {
-          unpack<T>(srow[v], a[0]);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) zq[e & 3] += exp_rel(a[0][e], ref, c);
-        }
+        zq[0] = add2(zq[0], zq[1]);
+        rest.z = distill_combine<SumOp, MW>(zq[0].x + zq[0].y, sm.red[par], warp, lane, gave_up);
+        par ^= 1u;
+        if (gave_up) break;
+        // a logit far above the reference, all of them far below, an infinity, NaN: the CTA starts over with the true maximum
+        held = rest.z > 8.6736174e-19f && rest.z < 1.1529215e18f;           // 2^-60, 2^60
       }
-      const float zw = warp_reduce<SumOp>((zq[0] + zq[1]) + (zq[2] + zq[3]));
-      if (lane == 0) sm.red[par][warp] = make_float2(mw, zw);
-      unsigned any;
-      asm volatile(
-          "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %2, 0;\n\tbar.red.or.pred p, 1, %1, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-          : "=r"(any) : "n"(MT), "r"((unsigned)gave_up) : "memory");
-      if (any) break;
-      float2 rd = lane < MW ? sm.red[par][lane] : make_float2(-INFINITY, 0.f);
-      float m = warp_reduce<MaxOp>(rd.x);
-      float mr = m == -INFINITY ? 0.f : m;
-      float z_rest = warp_reduce<SumOp>(rd.y * exp_rel(rd.x, mr, c));
-      float m_top = info.m_top, z_top = info.z_top;
+      if (!held) {
+        float m = -INFINITY, z = 0.f;
+        for (int i = t; i < n; i += MT) {
+          float x[VEC];
+          unpack<T>(srow[i], x);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) m = fmaxf(m, x[e]);
+        }
+        m = distill_combine<MaxOp, MW>(m, sm.red[par], warp, lane, gave_up);
+        par ^= 1u;
+        if (gave_up) break;
+        rest.ref = m == -INFINITY ? DistillRef{0.f, 0.f} : distill_ref(m, c);
+        for (int i = t; i < n; i += MT) {
+          float x[VEC];
+          unpack<T>(srow[i], x);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) z += distill_exp(x[e], rest.ref, c);
+        }
+        rest.z = distill_combine<SumOp, MW>(z, sm.red[par], warp, lane, gave_up);
+        par ^= 1u;
+        if (gave_up) break;
+      }
+      const DistillRef own = rest.ref;
+      const bool empty = rest.z == 0.f;                         // nothing but -inf in this part: its reference means nothing
+      DistillSum top{sampled ? info.ref : DistillRef{0.f, 0.f}, info.z_top, 0.f};
       if (C > 1) {
         // every CTA hands its part to all of the cluster; the parts are combined in rank order everywhere
         if (warp == 0) {
-          if (lane == 0) mbar_expect_tx(sm.rec_bar + par, (unsigned)(C * sizeof(DistillRec)));
+          if (lane == 0) mbar_expect_tx(sm.rec_bar + rpar, (unsigned)(C * sizeof(DistillRec)));
           if (lane < C) {
             uint32_t dst, bar;
-            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(dst) : "r"(smem_u32(&sm.rec[par][rank])), "r"(lane));
-            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(smem_u32(&sm.rec_bar[par])), "r"(lane));
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(dst) : "r"(smem_u32(&sm.rec[rpar][rank])), "r"(lane));
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(smem_u32(&sm.rec_bar[rpar])), "r"(lane));
             asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];"
-                         ::"r"(dst), "f"(m), "f"(z_rest), "f"(m_top), "f"(z_top), "r"(bar) : "memory");
+                         ::"r"(dst), "f"(rest.ref.sub), "f"(rest.ref.off), "f"(rest.z), "f"(0.f), "r"(bar) : "memory");
+            asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];"
+                         ::"r"(dst + 16u), "f"(top.ref.sub), "f"(top.ref.off), "f"(top.z), "f"(0.f), "r"(bar) : "memory");
           }
         }
-        gave_up = !__all_sync(0xffffffffu, distill_wait_cluster(sm.rec_bar + par, rph[par]));
-        rph[par] ^= 1u;
-        const DistillRec o = lane < C ? sm.rec[par][lane] : DistillRec{-INFINITY, 0.f, -INFINITY, 0.f};
-        m = warp_reduce<MaxOp>(o.m);
-        mr = m == -INFINITY ? 0.f : m;
-        z_rest = warp_reduce<SumOp>(o.z_rest * exp_rel(o.m, mr, c));
-        m_top = warp_reduce<MaxOp>(o.m_top);
-        const float tr = m_top == -INFINITY ? 0.f : m_top;
-        z_top = warp_reduce<SumOp>(o.z_top * exp_rel(o.m_top, tr, c));
+        gave_up = !__all_sync(0xffffffffu, distill_wait_cluster(sm.rec_bar + rpar, rph[rpar]));
+        rph[rpar] ^= 1u;
+        rest = sm.rec[rpar][0].rest;
+        top = sm.rec[rpar][0].top;
+        for (int q = 1; q < C; ++q) {
+          rest = distill_add(rest, sm.rec[rpar][q].rest, c);
+          top = distill_add(top, sm.rec[rpar][q].top, c);
+        }
+        rpar ^= 1u;
       }
-      par ^= 1u;
-      // against the maximum of the whole row, listed positions included
-      const float mall = fmaxf(m, m_top), mref = mall == -INFINITY ? 0.f : mall;
-      z_rest *= exp_rel(m, mref, c);
-      const float z_all = z_rest + z_top * exp_rel(m_top, mref, c);
-      if (t == 0) sm.fin[s] = DistillFin{mall, z_all, z_rest};
+      const bool one = C == 1 && held;                          // one reference for everything
+      const DistillSum all = one ? DistillSum{own, rest.z + top.z, 0.f} : distill_add(rest, top, c);
+      if (t == 0) sm.fin[s] = DistillFin{all.ref, all.z, rest.z, one || rest.z == 0.f ? 0.f : distill_shift(all.ref, rest.ref, c)};
       if (BWD) {
-        // (P / E - r / E_rest) e, with e formed against the warp's maximum
-        const float g = info.g_mass != 0.f ? info.g_mass / z_all - (info.g_r != 0.f && z_rest > 0.f ? info.g_r / z_rest : 0.f) : 0.f;
-        if (HOLD) {
-          // a warp whose part is all -inf has no reference: its exponentials are 0
-          const float f = mw == -INFINITY && mall != -INFINITY ? g * 0.f : g * exp_rel(ref, mref, c);
+        // (P / E - r / E_rest) e, e formed against this CTA's reference
+        float g = 0.f;
+        if (info.g_mass != 0.f) {
+          g = info.g_mass / all.z;
+          float gr = info.g_r != 0.f && rest.z > 0.f ? info.g_r / rest.z : 0.f;
+          if (!one && !empty) {
+            g *= exp2f_approx(distill_shift(all.ref, own, c));
+            if (gr != 0.f) gr *= exp2f_approx(distill_shift(rest.ref, own, c));
+          }
+          g -= gr;
+        }
+        if (held) {
+          const float2 g2 = make_float2(g, g);
 #pragma unroll
           for (int k = 0; k < NV; ++k) {
             const int i = t + k * MT;
             if (i < n) {
+              float d[VEC];
 #pragma unroll
-              for (int e = 0; e < VEC; ++e) a[k][e] *= f;
-              if (beta && same && i >= ilo && i < ihi) srow[i] = pack_accumulate<T>(a[k], ld_stream(dpart + i * VEC));
-              else srow[i] = pack<T>(a[k]);
+              for (int e = 0; e < VEC / 2; ++e) {
+                const float2 v = mul2(a[k][e], g2);
+                d[2 * e] = v.x; d[2 * e + 1] = v.y;
+              }
+              if (beta && same && i >= ilo && i < ihi) srow[i] = pack_accumulate<T>(d, ld_stream(dpart + i * VEC));
+              else srow[i] = pack<T>(d);
             }
           }
         } else {
           for (int i = t; i < n; i += MT) {
-            unpack<T>(srow[i], a[0]);
+            float x[VEC];
+            unpack<T>(srow[i], x);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) a[0][e] = exp_rel(a[0][e], mref, c) * g;
-            if (beta && same && i >= ilo && i < ihi) srow[i] = pack_accumulate<T>(a[0], ld_stream(dpart + i * VEC));
-            else srow[i] = pack<T>(a[0]);
+            for (int e = 0; e < VEC; ++e) x[e] = distill_exp(x[e], empty ? all.ref : own, c) * g;
+            if (beta && same && i >= ilo && i < ihi) srow[i] = pack_accumulate<T>(x, ld_stream(dpart + i * VEC));
+            else srow[i] = pack<T>(x);
           }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // written here, read by the copy out
@@ -653,7 +717,8 @@ static int launch_distill_as(uint64_t dl, uint64_t l, const DistillParams& p, in
 template <typename T>
 static int launch_distill(uint64_t dl, uint64_t l, const DistillParams& p, cudaStream_t st) {
   constexpr int VEC = Elem<T>::VEC;
-  const int nvec = (p.vocab + 2 * VEC - 2) / VEC;               // of the worst-aligned row
+  // vectors of a row; of the worst-aligned one where rows start at different places
+  const int nvec = p.vocab % VEC == 0 && (l & 15) == 0 ? p.vocab / VEC : (p.vocab + 2 * VEC - 2) / VEC;
   // CTAs a row: as many as keep a part within 4096 vectors (64 KB, three to an SM's shared memory)
   int C = 1;
   while (C < kDistillMaxC && (nvec + C - 1) / C > 4096) C *= 2;
@@ -687,7 +752,7 @@ int cacti_b200_distill_topk_fwd_bwd(cacti_b200_dptr loss_sum, cacti_b200_dptr lo
   if ((loss_sum & 3) || (loss_rows & 3) || (t_lse & 3) || (w_rows & 3) || (status & 3)) return CACTI_B200_ERR_INVALID_VALUE;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (rows == 0 || vocab == 0) return CACTI_B200_OK;
-  if (rows > 0x7fffffffLL) return CACTI_B200_ERR_SHAPE;
+  if (rows > 0x3fffffffLL) return CACTI_B200_ERR_SHAPE;           // row indices of the kernel and a grid's stride fit 32 bits
   if (!logits || !t_values || !t_indices) return CACTI_B200_ERR_INVALID_VALUE;
   const int es = dtype == CACTI_B200_R_32F ? 4 : 2, ts = t_dtype == CACTI_B200_R_32F ? 4 : 2;
   const int is = index_dtype == CACTI_B200_R_32I ? 4 : 2;
