@@ -17,6 +17,8 @@ namespace cb {
 constexpr int kDistillMaxK = 256;
 constexpr int64_t kDistillMaxVocab = 1 << 18;
 
+int g_distill_part = 4096;     // 16-byte vectors of a row that one CTA takes at most (launch_distill)
+
 struct DistillParams {
   const void* t_values;          // teacher logits [rows, k] in t_dtype
   const void* t_indices;         // [rows, k] int32 or uint16
@@ -31,10 +33,10 @@ struct DistillParams {
   int t_dtype, idx_dtype, beta;
 };
 
-__device__ __forceinline__ double teacher_value(const DistillParams& p, int64_t i) {
-  if (p.t_dtype == CACTI_B200_R_32F) return (double)reinterpret_cast<const float*>(p.t_values)[i];
-  if (p.t_dtype == CACTI_B200_R_16F) return (double)__half2float(reinterpret_cast<const __half*>(p.t_values)[i]);
-  return (double)__bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.t_values)[i]);
+__device__ __forceinline__ float teacher_value(const DistillParams& p, int64_t i) {
+  if (p.t_dtype == CACTI_B200_R_32F) return reinterpret_cast<const float*>(p.t_values)[i];
+  if (p.t_dtype == CACTI_B200_R_16F) return __half2float(reinterpret_cast<const __half*>(p.t_values)[i]);
+  return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.t_values)[i]);
 }
 // -1: unused slot; -2: outside the vocabulary.  65535 marks an unused slot of a uint16 list where it is no index.
 __device__ __forceinline__ int teacher_index(const DistillParams& p, int64_t i) {
@@ -72,15 +74,13 @@ __device__ __forceinline__ double warp_sum_f64(double v) {
 // Roles of a CTA (a cluster of C CTAs shares a row, each a run of its vectors):
 //   list warps, one per ring slot: fetch the slot's row (bulk copy), turn the teacher's list into probabilities, take the listed
 //     student logits out of the staged row (they become -inf there), and, when the row's gradient lies in the slot, put the listed
-//     positions' gradient in, send it off (bulk copy) and write the loss.  The list of a slot's next row is prepared while the
-//     main warps work;
+//     positions' gradient in, send it off (bulk copy) and write the loss;
 //   MW main warps: maximum and exponentials of the unlisted positions, one combination of (maximum, sum) over the CTA and the
 //     cluster, then gradient = exponential times a factor, written over the staged row.
-// HOLD: a CTA's part of a row is at most MW * 32 * kDistillNV vectors: the exponentials stay in registers, one a position.
-// Otherwise they are formed again for the gradient.
-constexpr int kDistillNV = 8;                                  // vectors a main thread holds
+// NV > 0: a CTA's part of a row is at most MW * 32 * NV vectors: the exponentials stay in registers, one a position.  NV = 0: they are
+// formed again for the gradient.
 constexpr int kDistillMaxC = 8;
-constexpr int kDistillSeen = 128;                              // words of a list's index filter
+constexpr int kDistillSeen = 512;                              // words of a list's index filter
 // What exponentials are taken against: e(x) = 2^((x - sub) c + off).  Ordinarily sub = 0 and off = -(a large logit times c,
 // rounded to a whole number): one multiply-add an exponential, and two references differ by an exact power of two.  Where that
 // product is no longer a small whole number (rows near the type's largest magnitudes) sub is the row's maximum and off = 0.
@@ -91,11 +91,12 @@ struct DistillRow {              // from the list warp to the main warps
   float g_mass, g_r;             // w c P and w c r
   int skip;                      // weight 0
 };
+struct DistillOwn { double px, pown; };                        // sum of p log2 e(x) and of p over this CTA's listed positions
 // A sum of exponentials under its reference.  Listed and unlisted positions keep references of their own until the end: where
 // the list holds nearly everything, the rest is still known.
 struct alignas(16) DistillSum { DistillRef ref; float z, pad; };
-struct DistillFin { DistillRef ref; float z_all, z_rest, shift_rest; };      // back to the list warp
-struct DistillRec { DistillSum rest, top; };                   // a CTA's part of a row, to the cluster
+struct DistillFin { DistillRef ref; float z_all, z_rest; double shift_rest, px; };       // back to the list warp
+struct alignas(16) DistillRec { DistillSum rest, top; double px, pown; };  // a CTA's part of a row, to the cluster
 
 template <int MW, int R> struct alignas(16) DistillSmem {
   uint64_t full[R], marked[R], stored[R];
@@ -103,10 +104,11 @@ template <int MW, int R> struct alignas(16) DistillSmem {
   DistillRec rec[2][kDistillMaxC];
   float red[2][MW];
   DistillRow row[R];
+  DistillOwn lst[R];
   DistillFin fin[R];
-  unsigned seen[R][kDistillSeen];
+  alignas(16) unsigned seen[R][kDistillSeen];
 };
-// behind it: two lists a slot (the row at work and the next one), then the ring
+// behind it: a list a slot, then the ring
 struct DistillList {             // KP = k rounded up to 32 entries of each
   double* p;                     // scaled teacher logit, later the probability
   float* x;                      // listed student logit, where it is in this CTA's part
@@ -141,9 +143,10 @@ __device__ __forceinline__ DistillRef distill_ref(float m, float c) {
   return fabsf(a) < 4194304.f ? DistillRef{0.f, -rintf(a)} : DistillRef{m, 0.f};
 }
 // log2 of e under a over e under b; positive where b's logits are the larger ones
-__device__ __forceinline__ float distill_shift(const DistillRef& a, const DistillRef& b, float c) {
-  return (float)(((double)b.sub - (double)a.sub) * (double)c + ((double)a.off - (double)b.off));
+__device__ __forceinline__ double distill_shift64(const DistillRef& a, const DistillRef& b, float c) {
+  return ((double)b.sub - (double)a.sub) * (double)c + ((double)a.off - (double)b.off);
 }
+__device__ __forceinline__ float distill_shift(const DistillRef& a, const DistillRef& b, float c) { return (float)distill_shift64(a, b, c); }
 
 // two f32 operations an instruction
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -215,40 +218,66 @@ __device__ __forceinline__ double exp_list(double d) {
   return s * __hiloint2double(((int)n + 1023) << 20, 0);
 }
 
+// ln z to about 1e-12: the f32 logarithm and one Newton step on exp.
+__device__ __forceinline__ double log_list(double z) {
+  const float y = logf((float)z);
+  if (!(fabsf(y) < 80.f)) return log(z);                        // 0, infinities, NaN, the ends of f32's range
+  const double d = fma(z, exp_list(-(double)y), -1.);
+  return (double)y + d - 0.5 * d * d;
+}
+
+// What is fetched of a row's list ahead of its preparation: the weight, the teacher's lse and the first two entries of each lane.
+struct DistillAhead { float w, lse; int id[2]; float z[2]; };
+__device__ __forceinline__ void distill_fetch(const DistillParams& p, int64_t row, int lane, DistillAhead& f) {
+  f.w = p.w_rows ? p.w_rows[row] : p.w_scalar;
+  f.lse = p.t_lse ? p.t_lse[row] : 0.f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int k = i * 32 + lane;
+    f.id[i] = -1; f.z[i] = 0.f;
+    if (k < p.k) { f.id[i] = teacher_index(p, row * p.k + k); f.z[i] = teacher_value(p, row * p.k + k); }
+  }
+}
+
 // Prepare the list of `row`: indices and validity, probabilities, their sums.
-template <typename T>
-__device__ __forceinline__ void distill_prepare(const DistillParams& p, int64_t row, const DistillList& li, unsigned* seen, int KP, int lane, DistillHead& h) {
-  h.w = p.w_rows ? p.w_rows[row] : p.w_scalar;
+__device__ __forceinline__ void distill_prepare(const DistillParams& p, int64_t row, const DistillAhead& f, const DistillList& li,
+                                                unsigned* seen, int KP, int lane, DistillHead& h) {
+  h.w = f.w;
   h.psum = h.ent = h.r = 0.;
   h.bad = false;
   if (h.w == 0.f) return;
-  double lse_t = p.t_lse ? (double)p.t_lse[row] : 0.;
 #pragma unroll
-  for (int i = 0; i < kDistillSeen / 32; ++i) seen[i * 32 + lane] = 0u;
+  for (int i = 0; i < kDistillSeen / 128; ++i) reinterpret_cast<uint4*>(seen)[i * 32 + lane] = make_uint4(0, 0, 0, 0);
   __syncwarp();
-  // An index listed twice: of two equal ones at least one finds its bit in the filter set; only such slots are compared
-  // with the whole list.
-  bool bad = false, suspect = false;
-#pragma unroll 2
-  for (int k = lane; k < KP; k += 32) {
+  // An index listed twice: of two equal ones at least one finds its bit in the filter set; only groups of 32 slots with such a
+  // one are compared with the whole list.
+  bool bad = false;
+  unsigned suspects = 0;                                        // bit i: group i
+#pragma unroll 1
+  for (int i = 0; i * 32 < KP; ++i) {
+    const int k = i * 32 + lane;
     int id = -1;
-    double z = 0.;
-    if (k < p.k) { id = teacher_index(p, row * p.k + k); z = p.inv_temp * teacher_value(p, row * p.k + k); }
+    float z = 0.f;
+    if (i < 2) { id = i ? f.id[1] : f.id[0]; z = i ? f.z[1] : f.z[0]; }
+    else if (k < p.k) { id = teacher_index(p, row * p.k + k); z = teacher_value(p, row * p.k + k); }
     bad |= id == -2;
+    bool suspect = false;
     if (id >= 0) {
-      const unsigned hash = ((unsigned)id * 2654435761u) >> 20;                 // 12 bits
+      const unsigned hash = ((unsigned)id * 2654435761u) >> 18;                 // 14 bits
       const unsigned bit = 1u << (hash & 31);
-      suspect |= (atomicOr(seen + (hash >> 5), bit) & bit) != 0;
+      suspect = (atomicOr(seen + (hash >> 5), bit) & bit) != 0;
     }
+    if (__any_sync(0xffffffffu, suspect)) suspects |= 1u << i;
     li.idx[k] = id < 0 ? -1 : id;
-    li.p[k] = id < 0 ? -INFINITY : z;
+    li.p[k] = id < 0 ? -INFINITY : p.inv_temp * (double)z;
   }
   __syncwarp();
-  if (__any_sync(0xffffffffu, suspect)) {
+  if (suspects) {
     bool twice = false;
 #pragma unroll 1
-    for (int k = lane; k < KP; k += 32) {
-      const int own = li.idx[k];
+    for (int i = 0; i * 32 < KP; ++i) {
+      if (!((suspects >> i) & 1u)) continue;
+      const int own = li.idx[i * 32 + lane];
       int hits = 0;
 #pragma unroll 2
       for (int j = 0; j < KP; j += 4) {
@@ -271,6 +300,7 @@ __device__ __forceinline__ void distill_prepare(const DistillParams& p, int64_t 
     }
   }
   h.bad = __any_sync(0xffffffffu, bad);
+  double lse_t = (double)f.lse;
   int cnt = 0;
   if (p.t_lse) {
 #pragma unroll 1
@@ -285,7 +315,7 @@ __device__ __forceinline__ void distill_prepare(const DistillParams& p, int64_t 
     double e = 0.;
 #pragma unroll 1
     for (int k = lane; k < KP; k += 32) if (li.p[k] != -INFINITY) e += exp_list(li.p[k] - zm);
-    lse_t = zm + log(warp_sum_f64(e));
+    lse_t = zm + log_list(warp_sum_f64(e));
   }
 #pragma unroll 1
   for (int k = lane; k < KP; k += 32) {
@@ -306,10 +336,13 @@ __device__ __forceinline__ void distill_prepare(const DistillParams& p, int64_t 
   if (p.t_lse && cnt && cnt < p.vocab) h.r = fmax(0., 1. - h.psum);
 }
 
+// CTAs an SM is to hold: by registers (NV * 8 exponentials and about 30 more a thread), each scheduler's 16384 shared by its warps
+constexpr int distill_residency(int MW, int R, int NV) { return NV == 0 || MW * NV > 64 ? 1 : MW * NV > 32 ? 2 : 3; }
+
 enum { kDistillFwd = 0, kDistillBwd = 1, kDistillAcc = 2 };
 
-template <typename T, int MW, int R, bool HOLD, int MODE>
-__global__ void __launch_bounds__((MW + R) * 32)
+template <typename T, int MW, int R, int NVH, int MODE>
+__global__ void __launch_bounds__((MW + R) * 32, distill_residency(MW, R, NVH))
 distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constant__ DistillParams p, unsigned slot_bytes) {
   constexpr int VEC = Elem<T>::VEC, MT = MW * 32;
   constexpr bool BWD = MODE != kDistillFwd;
@@ -319,7 +352,7 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
   const int KP = (p.k + 31) / 32 * 32;
   unsigned char* lists = smem_raw + sizeof(Smem);
-  unsigned char* ring = smem_raw + (sizeof(Smem) + (size_t)2 * R * KP * kDistillListBytes + 127) / 128 * 128;
+  unsigned char* ring = smem_raw + (sizeof(Smem) + (size_t)R * KP * kDistillListBytes + 127) / 128 * 128;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, V = p.vocab;
   const int C = (int)distill_nctas(), rank = (int)distill_ctarank();
   const int rows = (int)p.rows, row0 = (int)blockIdx.x / C, stride = (int)gridDim.x / C;
@@ -337,10 +370,8 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
     const int s = warp - MW;
     T* sx = reinterpret_cast<T*>(ring + (size_t)s * slot_bytes);
     const uint64_t t_begin = reinterpret_cast<uint64_t>(L), t_end = t_begin + (uint64_t)p.rows * V * sizeof(T);
-    auto list_of = [&](int b) {
-      unsigned char* at = lists + (size_t)(2 * s + b) * KP * kDistillListBytes;
-      return DistillList{reinterpret_cast<double*>(at), reinterpret_cast<float*>(at + 8 * KP), reinterpret_cast<int*>(at + 12 * KP)};
-    };
+    unsigned char* at0 = lists + (size_t)s * KP * kDistillListBytes;
+    const DistillList li{reinterpret_cast<double*>(at0), reinterpret_cast<float*>(at0 + 8 * KP), reinterpret_cast<int*>(at0 + 12 * KP)};
     // fetch a row's vectors of this CTA; whole vectors inside the tensor only
     auto issue = [&](int row) {
       if (lane == 0) {
@@ -357,23 +388,22 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
       }
     };
     unsigned ph = 0, full_ph = 0;                               // rows of weight 0 do not pass through `full`
-    int b = 0;
-    DistillHead h, hn;
+    DistillHead h;
+    DistillAhead ahead;
     int row = row0 + s * stride;
     if (row < rows) {
-      const float w0 = p.w_rows ? p.w_rows[row] : p.w_scalar;
-      if (w0 != 0.f) issue(row);
-      distill_prepare<T>(p, row, list_of(0), sm.seen[s], KP, lane, h);
+      distill_fetch(p, row, lane, ahead);
+      if (ahead.w != 0.f) issue(row);
+      distill_prepare(p, row, ahead, li, sm.seen[s], KP, lane, h);
     }
     // vectors of gradient and logits coincide: whole vectors leave by bulk copy, otherwise the slot is copied out by element
     const bool same = ((reinterpret_cast<uint64_t>(dL) ^ reinterpret_cast<uint64_t>(L)) & 15) == 0;
-    for (; row < rows; row += R * stride, b ^= 1, h = hn) {
+    for (; row < rows; row += R * stride) {
       const bool skip = h.w == 0.f;
       const RowVecs<T> rv(L + (int64_t)row * V, V);
       const int v0 = rv.nvec * rank / C, n = rv.nvec * (rank + 1) / C - v0;
       const int j0 = v0 * VEC - rv.head, j1 = j0 + n * VEC;                  // row elements of this CTA: [j0, j1)
       const int ilo = j0 < 0 ? 1 : 0, ihi = j1 > V ? n - 1 : n;              // vectors [ilo, ihi) lie wholly inside the row
-      const DistillList li = list_of(b);
       if (!skip) {
         // ---- the listed logits out of the staged row ----
         if (!mbar_wait_bounded_warp(sm.full + s, full_ph, kDevErrStageTimeout)) break;
@@ -409,13 +439,29 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
         DistillRef ref = distill_ref(mt, c);
         if (isinf(mt)) ref = DistillRef{0.f, 0.f};
         float zt = 0.f;
-        for (int k = lane; k < KP; k += 32) zt += distill_exp(li.x[k], ref, c);
+        double px = 0., pown = 0.;
+        for (int k = lane; k < KP; k += 32) {
+          const float x = li.x[k];
+          const int id = li.idx[k];
+          zt += distill_exp(x, ref, c);
+          const double pk = id >= j0 && id < j1 && id >= 0 ? li.p[k] : 0.;
+          if (pk != 0.) {
+            pown += pk;
+            px += pk * (((double)x - (double)ref.sub) * (double)c + (double)ref.off);
+          }
+        }
         zt = warp_reduce<SumOp>(zt);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          px += __shfl_xor_sync(0xffffffffu, px, o);
+          pown += __shfl_xor_sync(0xffffffffu, pown, o);
+        }
         if (lane == 0) {
           const double wc = (double)h.w * p.inv_temp;
           // without a usable sample the main warps look for the maximum themselves
           if (isinf(mt)) ref.off = __int_as_float(0x7fc00000);
           sm.row[s] = DistillRow{ref, zt, (float)(wc * (h.psum + h.r)), (float)(wc * h.r), 0};
+          sm.lst[s] = DistillOwn{px, pown};
         }
       } else if (lane == 0) {
         sm.row[s] = DistillRow{DistillRef{0.f, 0.f}, 0.f, 0.f, 0.f, 1};
@@ -423,13 +469,16 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
       __syncwarp();
       if (lane == 0) distill_arrive(sm.marked + s);
       const int next = row + R * stride;
-      if (next < rows) distill_prepare<T>(p, next, list_of(b ^ 1), sm.seen[s], KP, lane, hn);
+      if (next < rows) distill_fetch(p, next, lane, ahead);      // used once this row is out of the slot
       // ---- the row's gradient is in the slot: listed positions, off with it, loss ----
       if (!mbar_wait_bounded_warp(sm.stored + s, ph, kDevErrStageTimeout)) break;
       ph ^= 1u;
       if (skip) {
         if (lane == 0 && rank == 0 && p.loss_rows) p.loss_rows[row] = 0.f;
-        if (next < rows && hn.w != 0.f) issue(next);
+        if (next < rows) {
+          if (ahead.w != 0.f) issue(next);
+          distill_prepare(p, next, ahead, li, sm.seen[s], KP, lane, h);
+        }
         continue;
       }
       const DistillFin f = sm.fin[s];
@@ -468,25 +517,13 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
           __syncwarp();
         }
       }
-      if (rank == 0 && p.loss_rows) {
-        // sum p log2 e(x_k), in the arithmetic of the exponentials.  Listed logits of the cluster's other parts are read from
-        // memory.
-        double px = 0.;
-        for (int k = lane; k < KP; k += 32) {
-          const double pk = li.p[k];
-          if (pk != 0.) {
-            const int id = li.idx[k];
-            const float x = id >= j0 && id < j1 ? li.x[k] : Elem<T>::to_f32(L[(int64_t)row * V + id]);
-            px += pk * (((double)x - (double)f.ref.sub) * (double)c + (double)f.ref.off);
-          }
-        }
-        px = warp_sum_f64(px);
+      if (row % C == rank && p.loss_rows) {                     // the CTAs of a cluster take turns
         // the three logarithms side by side
-        const double lg = log(lane == 0 ? (double)f.z_all : lane == 1 ? h.r : (double)f.z_rest);
+        const double lg = log_list(lane == 0 ? (double)f.z_all : lane == 1 ? h.r : (double)f.z_rest);
         const double la = __shfl_sync(0xffffffffu, lg, 0), lr = __shfl_sync(0xffffffffu, lg, 1), lz = __shfl_sync(0xffffffffu, lg, 2);
         if (lane == 0) {
-          double loss = mass != 0. ? h.ent - 0.6931471805599453 * px + h.psum * la : 0.;
-          if (h.r > 0.) loss += h.r * (lr - lz - 0.6931471805599453 * (double)f.shift_rest + la);
+          double loss = mass != 0. ? h.ent - 0.6931471805599453 * f.px + h.psum * la : 0.;
+          if (h.r > 0.) loss += h.r * (lr - lz - 0.6931471805599453 * f.shift_rest + la);
           p.loss_rows[row] = h.bad ? __int_as_float(0x7fc00000) : (float)loss;
         }
       }
@@ -494,7 +531,10 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
       // the slot may be filled again once the copy out has read it
       if (BWD && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
       __syncwarp();
-      if (next < rows && hn.w != 0.f) issue(next);
+      if (next < rows) {
+        if (ahead.w != 0.f) issue(next);
+        distill_prepare(p, next, ahead, li, sm.seen[s], KP, lane, h);       // while the row is on its way
+      }
     }
     if (BWD && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   } else {
@@ -527,7 +567,8 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
         continue;
       }
       uint4* srow = reinterpret_cast<uint4*>(ring + (size_t)s * slot_bytes);
-      constexpr int NV = HOLD ? kDistillNV : 1;
+      constexpr bool HOLD = NVH > 0;
+      constexpr int NV = HOLD ? NVH : 1;
       float2 a[NV][VEC / 2];
       DistillSum rest{info.ref, 0.f, 0.f};
       const bool sampled = info.ref.off == info.ref.off;
@@ -594,6 +635,8 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
                          ::"r"(dst), "f"(rest.ref.sub), "f"(rest.ref.off), "f"(rest.z), "f"(0.f), "r"(bar) : "memory");
             asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];"
                          ::"r"(dst + 16u), "f"(top.ref.sub), "f"(top.ref.off), "f"(top.z), "f"(0.f), "r"(bar) : "memory");
+            asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f64 [%0], {%1, %2}, [%3];"
+                         ::"r"(dst + 32u), "d"(sm.lst[s].px), "d"(sm.lst[s].pown), "r"(bar) : "memory");
           }
         }
         gave_up = !__all_sync(0xffffffffu, distill_wait_cluster(sm.rec_bar + rpar, rph[rpar]));
@@ -604,11 +647,22 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
           rest = distill_add(rest, sm.rec[rpar][q].rest, c);
           top = distill_add(top, sm.rec[rpar][q].top, c);
         }
-        rpar ^= 1u;
       }
       const bool one = C == 1 && held;                          // one reference for everything
       const DistillSum all = one ? DistillSum{own, rest.z + top.z, 0.f} : distill_add(rest, top, c);
-      if (t == 0) sm.fin[s] = DistillFin{all.ref, all.z, rest.z, one || rest.z == 0.f ? 0.f : distill_shift(all.ref, rest.ref, c)};
+      if (t == 0) {
+        // sum p log2 e(x) under the row's reference
+        double px = 0.;
+        if (one) px = sm.lst[s].px;
+        else if (C == 1) px = sm.lst[s].pown != 0. ? sm.lst[s].px + sm.lst[s].pown * distill_shift64(all.ref, top.ref, c) : 0.;
+        else
+          for (int q = 0; q < C; ++q) {
+            const DistillRec& o = sm.rec[rpar][q];
+            if (o.pown != 0.) px += o.px + o.pown * distill_shift64(all.ref, o.top.ref, c);
+          }
+        sm.fin[s] = DistillFin{all.ref, all.z, rest.z, one || rest.z == 0.f ? 0. : distill_shift64(all.ref, rest.ref, c), px};
+      }
+      if (C > 1) rpar ^= 1u;
       if (BWD) {
         // (P / E - r / E_rest) e, e formed against this CTA's reference
         float g = 0.f;
@@ -677,12 +731,12 @@ distill_loss_sum_kernel(float* __restrict__ loss_sum, const float* __restrict__ 
   if (threadIdx.x == 0) *loss_sum = (float)sm[0];
 }
 
-template <typename T, int MW, int R, bool HOLD>
+template <typename T, int MW, int R, int NVH>
 static int launch_distill_as(uint64_t dl, uint64_t l, const DistillParams& p, int C, unsigned slot_bytes, cudaStream_t st) {
-  const size_t lists = (size_t)2 * R * ((p.k + 31) / 32 * 32) * kDistillListBytes;
+  const size_t lists = (size_t)R * ((p.k + 31) / 32 * 32) * kDistillListBytes;
   const size_t smem = (sizeof(DistillSmem<MW, R>) + lists + 127) / 128 * 128 + (size_t)R * slot_bytes;
-  auto kern = !dl ? distill_kernel<T, MW, R, HOLD, kDistillFwd>
-                  : p.beta ? distill_kernel<T, MW, R, HOLD, kDistillAcc> : distill_kernel<T, MW, R, HOLD, kDistillBwd>;
+  auto kern = !dl ? distill_kernel<T, MW, R, NVH, kDistillFwd>
+                  : p.beta ? distill_kernel<T, MW, R, NVH, kDistillAcc> : distill_kernel<T, MW, R, NVH, kDistillBwd>;
   const int per_sm = resident_ctas(kern, (MW + R) * 32, smem);
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3((MW + R) * 32); cfg.dynamicSmemBytes = smem; cfg.stream = st;
@@ -719,15 +773,14 @@ static int launch_distill(uint64_t dl, uint64_t l, const DistillParams& p, cudaS
   constexpr int VEC = Elem<T>::VEC;
   // vectors of a row; of the worst-aligned one where rows start at different places
   const int nvec = p.vocab % VEC == 0 && (l & 15) == 0 ? p.vocab / VEC : (p.vocab + 2 * VEC - 2) / VEC;
-  // CTAs a row: as many as keep a part within 4096 vectors (64 KB, three to an SM's shared memory)
   int C = 1;
-  while (C < kDistillMaxC && (nvec + C - 1) / C > 4096) C *= 2;
-  const unsigned part = (unsigned)((nvec + C - 1) / C + 1) * 16;
-  const unsigned slot = (part + 127) / 128 * 128;
+  while (C < kDistillMaxC && (nvec + C - 1) / C > g_distill_part) C *= 2;
   const int per = (nvec + C - 1) / C;
-  if (per <= 4 * 32 * kDistillNV) return launch_distill_as<T, 4, 3, true>(dl, l, p, C, slot, st);
-  if (per <= 16 * 32 * kDistillNV) return launch_distill_as<T, 16, 3, true>(dl, l, p, C, slot, st);
-  return launch_distill_as<T, 16, 1, false>(dl, l, p, C, slot, st);
+  const unsigned slot = ((unsigned)(per + 1) * 16 + 127) / 128 * 128;
+  if (per <= 8 * 32 * 4) return launch_distill_as<T, 8, 2, 4>(dl, l, p, C, slot, st);
+  if (per <= 8 * 32 * 8) return launch_distill_as<T, 8, 2, 8>(dl, l, p, C, slot, st);
+  if (per <= 16 * 32 * 8) return launch_distill_as<T, 16, 3, 8>(dl, l, p, C, slot, st);
+  return launch_distill_as<T, 16, 1, 0>(dl, l, p, C, slot, st);
 }
 
 }  // namespace cb
