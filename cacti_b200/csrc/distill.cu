@@ -146,7 +146,9 @@ __device__ __forceinline__ DistillRef distill_ref(float m, float c) {
 __device__ __forceinline__ double distill_shift64(const DistillRef& a, const DistillRef& b, float c) {
   return ((double)b.sub - (double)a.sub) * (double)c + ((double)a.off - (double)b.off);
 }
-__device__ __forceinline__ float distill_shift(const DistillRef& a, const DistillRef& b, float c) { return (float)distill_shift64(a, b, c); }
+__device__ __forceinline__ float distill_shift(const DistillRef& a, const DistillRef& b, float c) {
+  return a.sub == b.sub ? a.off - b.off : (float)distill_shift64(a, b, c);       // whole numbers: the difference is exact
+}
 
 // two f32 operations an instruction
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -641,11 +643,34 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
         }
         gave_up = !__all_sync(0xffffffffu, distill_wait_cluster(sm.rec_bar + rpar, rph[rpar]));
         rph[rpar] ^= 1u;
-        rest = sm.rec[rpar][0].rest;
-        top = sm.rec[rpar][0].top;
-        for (int q = 1; q < C; ++q) {
-          rest = distill_add(rest, sm.rec[rpar][q].rest, c);
-          top = distill_add(top, sm.rec[rpar][q].top, c);
+        const DistillSum nothing{DistillRef{0.f, 0.f}, 0.f, 0.f};
+        const DistillSum ro = lane < C ? sm.rec[rpar][lane].rest : nothing, to = lane < C ? sm.rec[rpar][lane].top : nothing;
+        if (__all_sync(0xffffffffu, ro.ref.sub == 0.f && to.ref.sub == 0.f)) {
+          // the largest reference has the smallest offset; sums over the lanes in a fixed order
+          float ra = ro.z != 0.f ? ro.ref.off : INFINITY, ta = to.z != 0.f ? to.ref.off : INFINITY;
+#pragma unroll
+          for (int o = kDistillMaxC / 2; o > 0; o >>= 1) {
+            ra = fminf(ra, __shfl_xor_sync(0xffffffffu, ra, o));
+            ta = fminf(ta, __shfl_xor_sync(0xffffffffu, ta, o));
+          }
+          float rz = ro.z != 0.f ? ro.z * exp2f_approx(ra - ro.ref.off) : 0.f, tz = to.z != 0.f ? to.z * exp2f_approx(ta - to.ref.off) : 0.f;
+#pragma unroll
+          for (int o = kDistillMaxC / 2; o > 0; o >>= 1) {
+            rz += __shfl_xor_sync(0xffffffffu, rz, o);
+            tz += __shfl_xor_sync(0xffffffffu, tz, o);
+          }
+          rest = DistillSum{DistillRef{0.f, isinf(ra) ? 0.f : ra}, rz, 0.f};
+          top = DistillSum{DistillRef{0.f, isinf(ta) ? 0.f : ta}, tz, 0.f};
+          // (the lanes beyond the cluster's CTAs have followed lanes of their own)
+          rest.ref.off = __shfl_sync(0xffffffffu, rest.ref.off, 0); rest.z = __shfl_sync(0xffffffffu, rest.z, 0);
+          top.ref.off = __shfl_sync(0xffffffffu, top.ref.off, 0); top.z = __shfl_sync(0xffffffffu, top.z, 0);
+        } else {
+          rest = sm.rec[rpar][0].rest;
+          top = sm.rec[rpar][0].top;
+          for (int q = 1; q < C; ++q) {
+            rest = distill_add(rest, sm.rec[rpar][q].rest, c);
+            top = distill_add(top, sm.rec[rpar][q].top, c);
+          }
         }
       }
       const bool one = C == 1 && held;                          // one reference for everything
