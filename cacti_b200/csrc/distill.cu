@@ -9,7 +9,7 @@
 // The unlisted sum is formed from the unlisted exponentials themselves, never as total minus listed: in a trained student
 // the listed part is nearly everything.  What belongs to a listed entry or to a row is kept in double (a few hundred
 // operations a row): the loss is a difference of nearly equal logarithms, and r is what a sum near one leaves.
-#include "common.cuh"
+#include "row_vec.cuh"
 #include <type_traits>
 
 namespace cb {
@@ -47,23 +47,6 @@ __device__ __forceinline__ int teacher_index(const DistillParams& p, int64_t i) 
   const int v = reinterpret_cast<const uint16_t*>(p.t_indices)[i];
   return v < p.vocab ? v : (v == 65535 ? -1 : -2);
 }
-
-// ---- layout of a row in 16-byte vectors ---------------------------------------------------------------------------
-// A row may start at any element address.  Its vectors are those of memory: vector v covers the 16 bytes at (address rounded
-// down) + 16 v, its element e is row element v VEC + e - head.  The first and the last vector may hold elements of the
-// neighbouring rows ("foreign"); they are never the first bytes before, or the last after, the whole tensor: there the vector is
-// fetched element by element.
-template <typename T> struct RowVecs {
-  const unsigned char* base;     // address of vector 0
-  int head;                      // foreign elements at the start of vector 0
-  int nvec;
-  __device__ __forceinline__ RowVecs(const T* row, int V) {
-    const uint64_t a = reinterpret_cast<uint64_t>(row);
-    base = reinterpret_cast<const unsigned char*>(a & ~15ull);
-    head = (int)(a & 15) / (int)sizeof(T);
-    nvec = (head + V + Elem<T>::VEC - 1) / Elem<T>::VEC;
-  }
-};
 
 __device__ __forceinline__ double warp_sum_f64(double v) {
 #pragma unroll
@@ -150,26 +133,6 @@ __device__ __forceinline__ float distill_shift(const DistillRef& a, const Distil
   return a.sub == b.sub ? a.off - b.off : (float)distill_shift64(a, b, c);       // whole numbers: the difference is exact
 }
 
-// two f32 operations an instruction
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
-      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
-      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
-      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
-      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
 // a + b under the larger reference
 __device__ __forceinline__ DistillSum distill_add(const DistillSum& a, const DistillSum& b, float c) {
   if (a.z == 0.f) return b;

@@ -2,81 +2,260 @@
 // hands to the distillation loss instead of its whole logits tensor.
 //
 // No counterpart in the reference (its arg-max, src/librarium/llama.rs:546, is the case K = 1).  Order: larger values first,
-// equal values (+0 equals -0) by ascending index, NaN above +inf.  Floats are compared through an order-preserving map
-// to unsigned keys.
-#include "common.cuh"
+// equal values (+0 equals -0) by ascending index, NaN above +inf.
+//
+// One CTA a row, the row read twice (the second time from L2, where 148 SMs' rows fit many times over):
+//   pass 1: every thread keeps two running maxima of its positions and sums exponentials against a reference taken from the
+//           first vectors.  The K-th largest of the 2 x THREADS maxima is a lower bound t of the K-th largest logit (K positions
+//           at or above it are known); one warp finds it, or a value just below it, by bisection on counts.
+//   pass 2: positions above t, hardly more than K for ordinary rows, are collected and ranked by counting; when they are fewer
+//           than K the first positions equal to t fill the rest in index order.
+// A row with more than kTopkCap positions above t (values arranged against the kernel's order) has its exact K-th largest found by
+// bisection over the whole row instead; then at most K - 1 lie above it.  Nothing depends on the order in which positions are
+// collected.
+#include "row_vec.cuh"
 
 namespace cb {
 
 constexpr int kTopkMaxK = 256;
 constexpr int64_t kTopkMaxVocab = 1 << 18;
-constexpr int kTopkThreads = 256;
+constexpr int kTopkCap = 1024;
 
 __device__ __forceinline__ unsigned order_key(float v) {
   if (v != v) return 0xffffffffu;
   const unsigned b = __float_as_uint(v == 0.f ? 0.f : v);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float order_value(unsigned key) {                    // of a key that is no NaN's
+  return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
 
-// One CTA a row: the K-th largest key by bisection on counts, then the entries above it (at most K - 1, ranked by
-// counting) and the first entries equal to it in index order.
-template <typename T>
-__global__ void __launch_bounds__(kTopkThreads)
+// Vector i of a row; foreign elements read as -inf.
+template <typename T> __device__ __forceinline__ uint4 topk_load(const RowVecs<T>& rv, const T* row, int V, int i, int ilo, int ihi) {
+  constexpr int VEC = Elem<T>::VEC;
+  if (i >= ilo && i < ihi) return __ldg(reinterpret_cast<const uint4*>(rv.base) + i);
+  T x[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    const int j = i * VEC - rv.head + e;
+    x[e] = j >= 0 && j < V ? row[j] : Elem<T>::from_f32(-INFINITY);
+  }
+  return *reinterpret_cast<const uint4*>(x);
+}
+
+// Any element of the vector above t, or NaN?
+template <typename T> __device__ __forceinline__ bool topk_any(const uint4& v, float t) {
+  if constexpr (sizeof(T) == 2) {
+    using P2 = typename Pair16<T>::type;
+    const P2* q = reinterpret_cast<const P2*>(&v);
+    const P2 t2{Elem<T>::from_f32(t), Elem<T>::from_f32(t)};                    // exact: t is a logit
+    return (__hgtu2_mask(q[0], t2) | __hgtu2_mask(q[1], t2) | __hgtu2_mask(q[2], t2) | __hgtu2_mask(q[3], t2)) != 0u;
+  } else {
+    float x[4];
+    unpack<float>(v, x);
+    return !(x[0] <= t) || !(x[1] <= t) || !(x[2] <= t) || !(x[3] <= t);
+  }
+}
+
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1536 / THREADS)
 logits_topk_kernel(T* __restrict__ values, int* __restrict__ indices, float* __restrict__ lse, const T* __restrict__ L,
-                   int64_t rows, int V, int K, double inv_temp) {
+                   int rows, int V, int K, double inv_temp) {
+  constexpr int VEC = Elem<T>::VEC, NW = THREADS / 32, UN = 4;
+  __shared__ float s_max[2 * THREADS];
+  __shared__ unsigned long long s_cand[kTopkCap];              // key, then the complement of the index: larger is earlier
   __shared__ float s_red[33];
-  __shared__ unsigned s_key[kTopkMaxK];
-  __shared__ int s_pos[kTopkMaxK];
-  __shared__ int s_n, s_ties, s_warp[kTopkThreads / 32];
-  const int t = threadIdx.x;
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const T* x = L + row * V;
-    unsigned lo = 0u, hi = 0xffffffffu;                         // the largest key with at least K entries at or above it
-    while (lo < hi) {
-      const unsigned mid = lo + (hi - lo) / 2 + 1;
-      float n = 0.f;                                            // counts below 2^24 are exact in f32
-      for (int j = t; j < V; j += blockDim.x) n += order_key(Elem<T>::to_f32(x[j])) >= mid ? 1.f : 0.f;
-      if (block_reduce<SumOp>(n, s_red) >= (float)K) lo = mid;
-      else hi = mid - 1;
+  __shared__ int s_n, s_warp[NW];
+  __shared__ float s_t;
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  const float c = (float)(inv_temp * 1.4426950408889634);
+  for (int row = blockIdx.x; row < rows; row += gridDim.x) {
+    const T* x = L + (int64_t)row * V;
+    const RowVecs<T> rv(x, V);
+    const int nvec = rv.nvec, ilo = rv.head ? 1 : 0, ihi = nvec * VEC - rv.head > V ? nvec - 1 : nvec;
+    // ---- pass 1 ----
+    float off = 0.f;
+    if (lse) {
+      // a reference for the exponentials: the largest logit of a few vectors, times c, as a whole number
+      float m = -INFINITY;
+      if (t < 128 && t < nvec) {
+        float a[VEC];
+        unpack<T>(topk_load<T>(rv, x, V, (int)((int64_t)t * nvec / 128 < nvec ? (int64_t)t * nvec / 128 : t), ilo, ihi), a);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) m = fmaxf(m, a[e]);
+      }
+      m = block_reduce<MaxOp>(m, s_red);
+      off = fabsf(m * c) < 4194304.f ? -rintf(m * c) : 0.f;    // (otherwise the sum falls outside its range and is done again)
     }
-    if (t == 0) { s_n = 0; s_ties = 0; }
+    const float2 c2 = make_float2(c, c), off2 = make_float2(off, off);
+    float2 zq[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+    float2 mx = make_float2(-INFINITY, -INFINITY);
+    using P2 = typename Pair16<T>::type;
+    P2 mp = Pair16<T>::neg_inf();
+    auto take = [&](const uint4& v) {
+      if constexpr (sizeof(T) == 2) {
+        const P2* q = reinterpret_cast<const P2*>(&v);
+        mp = __hmax2(mp, __hmax2(__hmax2(q[0], q[1]), __hmax2(q[2], q[3])));
+      } else {
+        float a[4];
+        unpack<float>(v, a);
+        mx.x = fmaxf(mx.x, fmaxf(a[0], a[2]));
+        mx.y = fmaxf(mx.y, fmaxf(a[1], a[3]));
+      }
+      if (lse) {
+        float a[VEC];
+        unpack<T>(v, a);
+#pragma unroll
+        for (int e = 0; e < VEC / 2; ++e) {
+          float2 y = fma2(make_float2(a[2 * e], a[2 * e + 1]), c2, off2);
+          y.x = exp2f_approx(y.x);
+          y.y = exp2f_approx(y.y);
+          zq[e & 1] = add2(zq[e & 1], y);
+        }
+      }
+    };
+    int i = t;
+    for (; i + (UN - 1) * THREADS < nvec; i += UN * THREADS) {
+      uint4 v[UN];
+#pragma unroll
+      for (int u = 0; u < UN; ++u) v[u] = topk_load<T>(rv, x, V, i + u * THREADS, ilo, ihi);
+#pragma unroll
+      for (int u = 0; u < UN; ++u) take(v[u]);
+    }
+    for (; i < nvec; i += THREADS) take(topk_load<T>(rv, x, V, i, ilo, ihi));
+    if constexpr (sizeof(T) == 2) mx = make_float2(Elem<T>::to_f32(mp.x), Elem<T>::to_f32(mp.y));
+    s_max[t] = mx.x;
+    s_max[THREADS + t] = mx.y;
+    if (t == 0) s_n = 0;
     __syncthreads();
-    for (int j = t; j < V; j += blockDim.x) {
-      const unsigned key = order_key(Elem<T>::to_f32(x[j]));
-      if (key > lo) { const int at = atomicAdd(&s_n, 1); s_key[at] = key; s_pos[at] = j; }
-    }
-    __syncthreads();
-    const int n = s_n;
-    if (t < n) {
-      int rank = 0;
-      for (int i = 0; i < n; ++i) rank += s_key[i] > s_key[t] || (s_key[i] == s_key[t] && s_pos[i] < s_pos[t]);
-      values[row * K + rank] = x[s_pos[t]];
-      indices[row * K + rank] = s_pos[t];
-    }
-    for (int j0 = 0; j0 < V && s_ties < K - n; j0 += blockDim.x) {
-      const int j = j0 + t;
-      const bool tie = j < V && order_key(Elem<T>::to_f32(x[j])) == lo;
-      const unsigned b = __ballot_sync(0xffffffffu, tie);
-      if ((t & 31) == 0) s_warp[t >> 5] = __popc(b);
-      __syncthreads();
-      int at = n + s_ties + __popc(b & ((1u << (t & 31)) - 1u));
-      int total = 0;
-      for (int i = 0; i < (int)(blockDim.x >> 5); ++i) { if (i < (t >> 5)) at += s_warp[i]; total += s_warp[i]; }
-      if (tie && at < K) { values[row * K + at] = x[j]; indices[row * K + at] = j; }
-      __syncthreads();
-      if (t == 0) s_ties += total;
-      __syncthreads();
+    // ---- a lower bound of the K-th largest: warp 0 ----
+    if (warp == 0) {
+      unsigned key[2 * NW];
+      unsigned kmin = 0xffffffffu, kmax = 0u;
+#pragma unroll
+      for (int u = 0; u < 2 * NW; ++u) {
+        key[u] = order_key(s_max[u * 32 + lane]);
+        kmin = key[u] < kmin ? key[u] : kmin;
+        kmax = key[u] > kmax ? key[u] : kmax;
+      }
+      unsigned lo = __reduce_min_sync(0xffffffffu, kmin), hi = __reduce_max_sync(0xffffffffu, kmax);
+      // `lo` is always such that K of the maxima are at or above it: K <= 2 THREADS, and empty ones count as -inf
+      while (lo < hi) {
+        const unsigned mid = lo + (hi - lo) / 2 + 1;
+        int n = 0;
+#pragma unroll
+        for (int u = 0; u < 2 * NW; ++u) n += key[u] >= mid;
+        n = __reduce_add_sync(0xffffffffu, n);
+        if (n >= K) { lo = mid; if (n <= K + K / 8) break; }
+        else hi = mid - 1;
+      }
+      // a logit's own value, so that it converts to T exactly: the smallest of the maxima at or above the bound
+      unsigned up = 0xffffffffu;
+#pragma unroll
+      for (int u = 0; u < 2 * NW; ++u) up = key[u] >= lo && key[u] < up ? key[u] : up;
+      up = __reduce_min_sync(0xffffffffu, up);
+      if (lane == 0) s_t = order_value(up);
     }
     if (lse) {
-      float m = -INFINITY;
-      for (int j = t; j < V; j += blockDim.x) m = fmaxf(m, Elem<T>::to_f32(x[j]));
-      m = block_reduce<MaxOp>(m, s_red);
-      if (isinf(m)) m = 0.f;                                    // no inf - inf: the sum is then 0 or inf
-      const float c = (float)(inv_temp * 1.4426950408889634);
-      float z = 0.f;
-      for (int j = t; j < V; j += blockDim.x) z += exp2f_approx((Elem<T>::to_f32(x[j]) - m) * c);
-      z = block_reduce<SumOp>(z, s_red);
-      if (t == 0) lse[row] = (float)(log((double)z) + inv_temp * (double)m);
+      const float2 zz = add2(zq[0], zq[1]);
+      float z = block_reduce<SumOp>(zz.x + zz.y, s_red);
+      float sub = 0.f;
+      if (!(z > 8.6736174e-19f && z < 1.1529215e18f)) {         // 2^-60, 2^60: against the true maximum, differences first
+        float m = -INFINITY;
+        for (int u = t; u < 2 * THREADS; u += THREADS) m = fmaxf(m, s_max[u]);
+        m = block_reduce<MaxOp>(m, s_red);
+        sub = isinf(m) ? 0.f : m;                               // no inf - inf: the sum is then 0 or inf
+        off = 0.f;
+        z = 0.f;
+        for (int u = t; u < nvec; u += THREADS) {
+          float a[VEC];
+          unpack<T>(topk_load<T>(rv, x, V, u, ilo, ihi), a);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) z += exp2f_approx((a[e] - sub) * c);
+        }
+        z = block_reduce<SumOp>(z, s_red);
+      }
+      if (t == 0) lse[row] = (float)(log((double)z) - (double)off * 0.6931471805599453 + inv_temp * (double)sub);
+    }
+    __syncthreads();
+    // ---- pass 2 ----
+    float bound = s_t;
+    int n = 0;
+    for (int attempt = 0; attempt < 2; ++attempt) {
+      auto collect = [&](const uint4& v, int at) {
+        if (topk_any<T>(v, bound)) {
+          float a[VEC];
+          unpack<T>(v, a);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            if (!(a[e] <= bound)) {
+              const int slot = atomicAdd(&s_n, 1);
+              const unsigned j = (unsigned)(at * VEC - rv.head + e);
+              if (slot < kTopkCap) s_cand[slot] = ((unsigned long long)order_key(a[e]) << 32) | (0xffffffffu - j);
+            }
+          }
+        }
+      };
+      int u0 = t;
+      for (; u0 + (UN - 1) * THREADS < nvec; u0 += UN * THREADS) {
+        uint4 v[UN];
+#pragma unroll
+        for (int u = 0; u < UN; ++u) v[u] = topk_load<T>(rv, x, V, u0 + u * THREADS, ilo, ihi);
+#pragma unroll
+        for (int u = 0; u < UN; ++u) collect(v[u], u0 + u * THREADS);
+      }
+      for (; u0 < nvec; u0 += THREADS) collect(topk_load<T>(rv, x, V, u0, ilo, ihi), u0);
+      __syncthreads();
+      n = s_n;
+      if (n <= kTopkCap) break;
+      // the exact K-th largest: at most K - 1 positions are above it
+      unsigned lo = order_key(bound), hi = 0xffffffffu;
+      while (lo < hi) {
+        const unsigned mid = lo + (hi - lo) / 2 + 1;
+        float cnt = 0.f;                                        // counts below 2^24 are exact in f32
+        for (int u = t; u < nvec; u += THREADS) {
+          float a[VEC];
+          unpack<T>(topk_load<T>(rv, x, V, u, ilo, ihi), a);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            const int j = u * VEC - rv.head + e;
+            cnt += j >= 0 && j < V && order_key(a[e]) >= mid ? 1.f : 0.f;
+          }
+        }
+        if (block_reduce<SumOp>(cnt, s_red) >= (float)K) lo = mid;
+        else hi = mid - 1;
+      }
+      // K NaNs or more: the bound is NaN, nothing is above it and its positions are the ties
+      bound = lo == 0xffffffffu ? __int_as_float(0x7fc00000) : order_value(lo);
+      if (t == 0) s_n = 0;
+      __syncthreads();
+      if (bound != bound) { n = 0; break; }
+    }
+    // ---- rank: a warp a candidate, counting the larger ones ----
+    for (int q = warp; q < n; q += NW) {
+      const unsigned long long own = s_cand[q];
+      int rank = 0;
+      for (int u = 0; u < n; u += 32) rank += __popc(__ballot_sync(0xffffffffu, u + lane < n && s_cand[u + lane] > own));
+      if (lane == 0 && rank < K) {
+        const int j = (int)(0xffffffffu - (unsigned)own);
+        values[(int64_t)row * K + rank] = x[j];
+        indices[(int64_t)row * K + rank] = j;
+      }
+    }
+    // ---- the first positions equal to the bound, in index order ----
+    for (int j0 = 0, have = n; have < K && j0 < V; j0 += THREADS) {
+      const int j = j0 + t;
+      const float a = j < V ? Elem<T>::to_f32(x[j]) : 0.f;
+      const bool tie = j < V && (a == bound || (bound != bound && a != a));
+      const unsigned b = __ballot_sync(0xffffffffu, tie);
+      if (lane == 0) s_warp[warp] = __popc(b);
+      __syncthreads();
+      int at = have + __popc(b & ((1u << lane) - 1u)), total = 0;
+#pragma unroll
+      for (int u = 0; u < NW; ++u) { if (u < warp) at += s_warp[u]; total += s_warp[u]; }
+      if (tie && at < K) { values[(int64_t)row * K + at] = x[j]; indices[(int64_t)row * K + at] = j; }
+      have += total;
+      __syncthreads();
     }
     __syncthreads();
   }
@@ -85,10 +264,17 @@ logits_topk_kernel(T* __restrict__ values, int* __restrict__ indices, float* __r
 template <typename T>
 static int launch_topk(uint64_t values, uint64_t indices, uint64_t lse, uint64_t logits, int64_t rows, int64_t vocab, int64_t k,
                        double inv_temp, cudaStream_t st) {
-  const int64_t cap = (int64_t)kNumSMs * 8;
-  logits_topk_kernel<T><<<(unsigned)(rows < cap ? rows : cap), kTopkThreads, 0, st>>>(
-      reinterpret_cast<T*>(values), reinterpret_cast<int*>(indices), reinterpret_cast<float*>(lse),
-      reinterpret_cast<const T*>(logits), rows, (int)vocab, (int)k, inv_temp);
+  T* v = reinterpret_cast<T*>(values);
+  int* ix = reinterpret_cast<int*>(indices);
+  float* ls = reinterpret_cast<float*>(lse);
+  const T* l = reinterpret_cast<const T*>(logits);
+  // few rows: 1024 threads bring a row's bytes sooner; otherwise CTAs of 256, so that the passes of several rows overlap on an SM
+  if (rows <= kNumSMs) {
+    logits_topk_kernel<T, 1024><<<(unsigned)rows, 1024, 0, st>>>(v, ix, ls, l, (int)rows, (int)vocab, (int)k, inv_temp);
+  } else {
+    const int64_t cap = (int64_t)kNumSMs * 6;
+    logits_topk_kernel<T, 256><<<(unsigned)(rows < cap ? rows : cap), 256, 0, st>>>(v, ix, ls, l, (int)rows, (int)vocab, (int)k, inv_temp);
+  }
   return check_launch();
 }
 
@@ -101,7 +287,7 @@ int cacti_b200_logits_topk(cacti_b200_dptr values, cacti_b200_dptr indices, cact
   if (rows < 0 || vocab < 0 || k < 0) return CACTI_B200_ERR_INVALID_VALUE;
   if (!(temperature >= 1e-4f && temperature <= 1e4f)) return CACTI_B200_ERR_INVALID_VALUE;
   if (dtype != CACTI_B200_R_32F && dtype != CACTI_B200_R_16F && dtype != CACTI_B200_R_16BF) return CACTI_B200_ERR_DTYPE;
-  if (vocab > kTopkMaxVocab || k > kTopkMaxK || k < 1 || k > vocab || rows > 0x7fffffffLL) return CACTI_B200_ERR_SHAPE;
+  if (vocab > kTopkMaxVocab || k > kTopkMaxK || k < 1 || k > vocab || rows > 0x3fffffffLL) return CACTI_B200_ERR_SHAPE;
   if (rows == 0) return CACTI_B200_OK;
   const int es = dtype == CACTI_B200_R_32F ? 4 : 2;
   if (!values || !indices || !logits || values % es || logits % es || (indices & 3) || (lse & 3)) return CACTI_B200_ERR_INVALID_VALUE;
