@@ -30,17 +30,30 @@ __device__ __forceinline__ float order_value(unsigned key) {                    
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-// Vector i of a row; foreign elements read as -inf.
-template <typename T> __device__ __forceinline__ uint4 topk_load(const RowVecs<T>& rv, const T* row, int V, int i, int ilo, int ihi) {
+// f(vector, index) for every whole vector of the row, UN at a time, all their loads first; f1(j) for the elements of the vectors at
+// its edges that belong to it, one a thread.
+template <typename T, int THREADS, int UN, typename F, typename F1>
+__device__ __forceinline__ void topk_sweep(const RowVecs<T>& rv, int V, int t, F&& f, F1&& f1) {
   constexpr int VEC = Elem<T>::VEC;
-  if (i >= ilo && i < ihi) return __ldg(reinterpret_cast<const uint4*>(rv.base) + i);
-  T x[VEC];
+  const int ilo = rv.head ? 1 : 0, ihi = rv.nvec * VEC - rv.head > V ? rv.nvec - 1 : rv.nvec;
+  const uint4* p = reinterpret_cast<const uint4*>(rv.base);
+  int i = ilo + t;
+#pragma unroll 1
+  for (; i + (UN - 1) * THREADS < ihi; i += UN * THREADS) {
+    uint4 v[UN];
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) {
-    const int j = i * VEC - rv.head + e;
-    x[e] = j >= 0 && j < V ? row[j] : Elem<T>::from_f32(-INFINITY);
+    for (int u = 0; u < UN; ++u) v[u] = __ldg(p + i + u * THREADS);
+#pragma unroll
+    for (int u = 0; u < UN; ++u) f(v[u], i + u * THREADS);
   }
-  return *reinterpret_cast<const uint4*>(x);
+#pragma unroll 1
+  for (; i < ihi; i += THREADS) f(__ldg(p + i), i);
+  if (t < 2 * VEC) {
+    // vector 0, and the last one where it is another
+    const bool tail = t >= VEC;
+    const int v = tail ? rv.nvec - 1 : 0, j = v * VEC - rv.head + (tail ? t - VEC : t);
+    if ((v < ilo || v >= ihi) && !(tail && v == 0) && j >= 0 && j < V) f1(j);
+  }
 }
 
 // Any element of the vector above t, or NaN?
@@ -56,33 +69,30 @@ template <typename T> __device__ __forceinline__ bool topk_any(const uint4& v, f
     return !(x[0] <= t) || !(x[1] <= t) || !(x[2] <= t) || !(x[3] <= t);
   }
 }
-
 template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1536 / THREADS)
 logits_topk_kernel(T* __restrict__ values, int* __restrict__ indices, float* __restrict__ lse, const T* __restrict__ L,
                    int rows, int V, int K, double inv_temp) {
-  constexpr int VEC = Elem<T>::VEC, NW = THREADS / 32, UN = 4;
+  constexpr int VEC = Elem<T>::VEC, NW = THREADS / 32;
   __shared__ float s_max[2 * THREADS];
   __shared__ unsigned long long s_cand[kTopkCap];              // key, then the complement of the index: larger is earlier
   __shared__ float s_red[33];
-  __shared__ int s_n, s_warp[NW];
+  __shared__ int s_n, s_hits, s_warp[NW];
+  __shared__ int s_hit[kTopkCap];                              // vectors that hold a candidate
   __shared__ float s_t;
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
   const float c = (float)(inv_temp * 1.4426950408889634);
   for (int row = blockIdx.x; row < rows; row += gridDim.x) {
     const T* x = L + (int64_t)row * V;
     const RowVecs<T> rv(x, V);
-    const int nvec = rv.nvec, ilo = rv.head ? 1 : 0, ihi = nvec * VEC - rv.head > V ? nvec - 1 : nvec;
     // ---- pass 1 ----
     float off = 0.f;
     if (lse) {
-      // a reference for the exponentials: the largest logit of a few vectors, times c, as a whole number
+      // a reference for the exponentials: the largest of 1024 logits, times c, as a whole number
       float m = -INFINITY;
-      if (t < 128 && t < nvec) {
-        float a[VEC];
-        unpack<T>(topk_load<T>(rv, x, V, (int)((int64_t)t * nvec / 128 < nvec ? (int64_t)t * nvec / 128 : t), ilo, ihi), a);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) m = fmaxf(m, a[e]);
+      for (int u = t; u < 1024; u += THREADS) {
+        const int64_t j = (int64_t)u * V / 1024;
+        m = fmaxf(m, Elem<T>::to_f32(x[j]));
       }
       m = block_reduce<MaxOp>(m, s_red);
       off = fabsf(m * c) < 4194304.f ? -rintf(m * c) : 0.f;    // (otherwise the sum falls outside its range and is done again)
@@ -92,7 +102,12 @@ logits_topk_kernel(T* __restrict__ values, int* __restrict__ indices, float* __r
     float2 mx = make_float2(-INFINITY, -INFINITY);
     using P2 = typename Pair16<T>::type;
     P2 mp = Pair16<T>::neg_inf();
-    auto take = [&](const uint4& v) {
+    auto take1 = [&](int j) {
+      const float a = Elem<T>::to_f32(x[j]);
+      mx.x = fmaxf(mx.x, a);
+      if (lse) zq[0].x += exp2f_approx(fmaf(a, c, off));
+    };
+    auto take = [&](const uint4& v, int) {
       if constexpr (sizeof(T) == 2) {
         const P2* q = reinterpret_cast<const P2*>(&v);
         mp = __hmax2(mp, __hmax2(__hmax2(q[0], q[1]), __hmax2(q[2], q[3])));
@@ -114,19 +129,11 @@ logits_topk_kernel(T* __restrict__ values, int* __restrict__ indices, float* __r
         }
       }
     };
-    int i = t;
-    for (; i + (UN - 1) * THREADS < nvec; i += UN * THREADS) {
-      uint4 v[UN];
-#pragma unroll
-      for (int u = 0; u < UN; ++u) v[u] = topk_load<T>(rv, x, V, i + u * THREADS, ilo, ihi);
-#pragma unroll
-      for (int u = 0; u < UN; ++u) take(v[u]);
-    }
-    for (; i < nvec; i += THREADS) take(topk_load<T>(rv, x, V, i, ilo, ihi));
-    if constexpr (sizeof(T) == 2) mx = make_float2(Elem<T>::to_f32(mp.x), Elem<T>::to_f32(mp.y));
+    topk_sweep<T, THREADS, 4>(rv, V, t, take, take1);
+    if constexpr (sizeof(T) == 2) mx = make_float2(fmaxf(mx.x, Elem<T>::to_f32(mp.x)), Elem<T>::to_f32(mp.y));
     s_max[t] = mx.x;
     s_max[THREADS + t] = mx.y;
-    if (t == 0) s_n = 0;
+    if (t == 0) { s_n = 0; s_hits = 0; }
     __syncthreads();
     // ---- a lower bound of the K-th largest: warp 0 ----
     if (warp == 0) {
@@ -167,12 +174,12 @@ logits_topk_kernel(T* __restrict__ values, int* __restrict__ indices, float* __r
         sub = isinf(m) ? 0.f : m;                               // no inf - inf: the sum is then 0 or inf
         off = 0.f;
         z = 0.f;
-        for (int u = t; u < nvec; u += THREADS) {
+        topk_sweep<T, THREADS, 1>(rv, V, t, [&](const uint4& v, int) {
           float a[VEC];
-          unpack<T>(topk_load<T>(rv, x, V, u, ilo, ihi), a);
+          unpack<T>(v, a);
 #pragma unroll
           for (int e = 0; e < VEC; ++e) z += exp2f_approx((a[e] - sub) * c);
-        }
+        }, [&](int j) { z += exp2f_approx((Elem<T>::to_f32(x[j]) - sub) * c); });
         z = block_reduce<SumOp>(z, s_red);
       }
       if (t == 0) lse[row] = (float)(log((double)z) - (double)off * 0.6931471805599453 + inv_temp * (double)sub);
@@ -182,52 +189,43 @@ logits_topk_kernel(T* __restrict__ values, int* __restrict__ indices, float* __r
     float bound = s_t;
     int n = 0;
     for (int attempt = 0; attempt < 2; ++attempt) {
-      auto collect = [&](const uint4& v, int at) {
-        if (topk_any<T>(v, bound)) {
-          float a[VEC];
-          unpack<T>(v, a);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            if (!(a[e] <= bound)) {
-              const int slot = atomicAdd(&s_n, 1);
-              const unsigned j = (unsigned)(at * VEC - rv.head + e);
-              if (slot < kTopkCap) s_cand[slot] = ((unsigned long long)order_key(a[e]) << 32) | (0xffffffffu - j);
-            }
-          }
+      // vectors that hold such a position first: the elements are looked at one a thread afterwards
+      auto push = [&](int j) {
+        const float a = Elem<T>::to_f32(x[j]);
+        if (!(a <= bound)) {
+          const int slot = atomicAdd(&s_n, 1);
+          if (slot < kTopkCap) s_cand[slot] = ((unsigned long long)order_key(a) << 32) | (0xffffffffu - (unsigned)j);
         }
       };
-      int u0 = t;
-      for (; u0 + (UN - 1) * THREADS < nvec; u0 += UN * THREADS) {
-        uint4 v[UN];
-#pragma unroll
-        for (int u = 0; u < UN; ++u) v[u] = topk_load<T>(rv, x, V, u0 + u * THREADS, ilo, ihi);
-#pragma unroll
-        for (int u = 0; u < UN; ++u) collect(v[u], u0 + u * THREADS);
-      }
-      for (; u0 < nvec; u0 += THREADS) collect(topk_load<T>(rv, x, V, u0, ilo, ihi), u0);
+      topk_sweep<T, THREADS, 4>(rv, V, t, [&](const uint4& v, int at) {
+        if (topk_any<T>(v, bound)) {
+          const int slot = atomicAdd(&s_hits, 1);
+          if (slot < kTopkCap) s_hit[slot] = at;
+        }
+      }, push);
       __syncthreads();
-      n = s_n;
+      const int hits = s_hits;
+      for (int q = t; q < (hits < kTopkCap ? hits : 0) * VEC; q += THREADS) push(s_hit[q / VEC] * VEC - rv.head + q % VEC);
+      __syncthreads();
+      n = hits > kTopkCap ? hits : s_n;
       if (n <= kTopkCap) break;
       // the exact K-th largest: at most K - 1 positions are above it
       unsigned lo = order_key(bound), hi = 0xffffffffu;
       while (lo < hi) {
         const unsigned mid = lo + (hi - lo) / 2 + 1;
         float cnt = 0.f;                                        // counts below 2^24 are exact in f32
-        for (int u = t; u < nvec; u += THREADS) {
+        topk_sweep<T, THREADS, 1>(rv, V, t, [&](const uint4& v, int) {
           float a[VEC];
-          unpack<T>(topk_load<T>(rv, x, V, u, ilo, ihi), a);
+          unpack<T>(v, a);
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const int j = u * VEC - rv.head + e;
-            cnt += j >= 0 && j < V && order_key(a[e]) >= mid ? 1.f : 0.f;
-          }
-        }
+          for (int e = 0; e < VEC; ++e) cnt += order_key(a[e]) >= mid ? 1.f : 0.f;
+        }, [&](int j) { cnt += order_key(Elem<T>::to_f32(x[j])) >= mid ? 1.f : 0.f; });
         if (block_reduce<SumOp>(cnt, s_red) >= (float)K) lo = mid;
         else hi = mid - 1;
       }
       // K NaNs or more: the bound is NaN, nothing is above it and its positions are the ties
       bound = lo == 0xffffffffu ? __int_as_float(0x7fc00000) : order_value(lo);
-      if (t == 0) s_n = 0;
+      if (t == 0) { s_n = 0; s_hits = 0; }
       __syncthreads();
       if (bound != bound) { n = 0; break; }
     }
