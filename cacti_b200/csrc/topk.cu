@@ -4,15 +4,16 @@
 // No counterpart in the reference (its arg-max, src/librarium/llama.rs:546, is the case K = 1).  Order: larger values first,
 // equal values (+0 equals -0) by ascending index, NaN above +inf.
 //
-// One CTA a row, the row read twice (the second time from L2, where 148 SMs' rows fit many times over):
-//   pass 1: every thread keeps two running maxima of its positions and sums exponentials against a reference taken from the
-//           first vectors.  The K-th largest of the 2 x THREADS maxima is a lower bound t of the K-th largest logit (K positions
-//           at or above it are known); one warp finds it, or a value just below it, by bisection on counts.
-//   pass 2: positions above t, hardly more than K for ordinary rows, are collected and ranked by counting; when they are fewer
-//           than K the first positions equal to t fill the rest in index order.
-// A row with more than kTopkCap positions above t (values arranged against the kernel's order) has its exact K-th largest found by
-// bisection over the whole row instead; then at most K - 1 lie above it.  Nothing depends on the order in which positions are
-// collected.
+// One CTA a row, the row read twice (the second time from L2):
+//   pass 1: 512 groups of positions (by thread and lane of a pair) each keep a running maximum, and every warp sums exponentials
+//           against a reference from its first vectors.  The K-th largest of the 512 maxima is a lower bound t of the K-th largest
+//           logit (K positions at or above it are known); one warp finds it, or a value just below it, by bisection on counts.
+//   pass 2: vectors with a position at or above t are put aside, then these positions, hardly more than K for ordinary rows, are
+//           collected and ranked by counting.
+// More than kTopkCap of them: with many equal to t (few distinct values, masks) only those above t are collected, and the first
+// positions equal to t fill the rest in index order.  More than kTopkCap above t (values arranged against the kernel's order): the
+// exact K-th largest is found by bisection over the whole row, and at most K - 1 lie above that.  Nothing depends on the order in
+// which positions are collected.
 #include "row_vec.cuh"
 
 namespace cb {
@@ -20,6 +21,7 @@ namespace cb {
 constexpr int kTopkMaxK = 256;
 constexpr int64_t kTopkMaxVocab = 1 << 18;
 constexpr int kTopkCap = 1024;
+constexpr int kTopkGroups = 512;
 
 __device__ __forceinline__ unsigned order_key(float v) {
   if (v != v) return 0xffffffffu;
@@ -56,6 +58,21 @@ __device__ __forceinline__ void topk_sweep(const RowVecs<T>& rv, int V, int t, F
   }
 }
 
+// The largest value of T below t; NaN below -inf, with which every value compares as not less or equal.
+template <typename T> __device__ __forceinline__ float topk_below(float t) {
+  if (t == 0.f) t = 0.f;                                       // of -0 and +0 alike: the smallest negative number
+  if (t == -INFINITY) return __int_as_float(0x7fc00000);
+  if constexpr (sizeof(T) == 2) {
+    const T v = Elem<T>::from_f32(t);
+    unsigned short b = *reinterpret_cast<const unsigned short*>(&v);
+    b = b == 0 ? 0x8001 : (b & 0x8000u) ? b + 1 : b - 1;
+    return Elem<T>::to_f32(*reinterpret_cast<const T*>(&b));
+  } else {
+    const unsigned b = __float_as_uint(t);
+    return __uint_as_float(b == 0 ? 0x80000001u : (b & 0x80000000u) ? b + 1 : b - 1);
+  }
+}
+
 // Any element of the vector above t, or NaN?
 template <typename T> __device__ __forceinline__ bool topk_any(const uint4& v, float t) {
   if constexpr (sizeof(T) == 2) {
@@ -74,11 +91,14 @@ __global__ void __launch_bounds__(THREADS, 1536 / THREADS)
 logits_topk_kernel(T* __restrict__ values, int* __restrict__ indices, float* __restrict__ lse, const T* __restrict__ L,
                    int rows, int V, int K, double inv_temp) {
   constexpr int VEC = Elem<T>::VEC, NW = THREADS / 32;
-  __shared__ float s_max[2 * THREADS];
-  __shared__ unsigned long long s_cand[kTopkCap];              // key, then the complement of the index: larger is earlier
+  __shared__ float s_max[kTopkGroups];
+  __shared__ uint4 s_hit[kTopkCap];                            // vectors that hold a candidate ...
+  __shared__ int s_hit_at[kTopkCap];                           // ... and their indices
+  // candidates: key, then the complement of the index (18 bits; larger is earlier), then 1 for -0
+  __shared__ alignas(16) unsigned long long s_cand[kTopkCap + 8];
   __shared__ float s_red[33];
+  __shared__ float2 s_z[NW];                                   // a warp's sum of exponentials and its reference
   __shared__ int s_n, s_hits, s_warp[NW];
-  __shared__ int s_hit[kTopkCap];                              // vectors that hold a candidate
   __shared__ float s_t;
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
   const float c = (float)(inv_temp * 1.4426950408889634);
@@ -88,13 +108,13 @@ logits_topk_kernel(T* __restrict__ values, int* __restrict__ indices, float* __r
     // ---- pass 1 ----
     float off = 0.f;
     if (lse) {
-      // a reference for the exponentials: the largest of 1024 logits, times c, as a whole number
+      // the warp's reference for the exponentials: the largest of its first logits, times c, as a whole number
       float m = -INFINITY;
-      for (int u = t; u < 1024; u += THREADS) {
-        const int64_t j = (int64_t)u * V / 1024;
-        m = fmaxf(m, Elem<T>::to_f32(x[j]));
+      for (int e = 0; e < 4; ++e) {
+        const int j = warp * 32 * VEC + e * 32 + lane;
+        if (j < V) m = fmaxf(m, Elem<T>::to_f32(x[j]));
       }
-      m = block_reduce<MaxOp>(m, s_red);
+      m = warp_reduce<MaxOp>(m);
       off = fabsf(m * c) < 4194304.f ? -rintf(m * c) : 0.f;    // (otherwise the sum falls outside its range and is done again)
     }
     const float2 c2 = make_float2(c, c), off2 = make_float2(off, off);
@@ -130,49 +150,71 @@ logits_topk_kernel(T* __restrict__ values, int* __restrict__ indices, float* __r
       }
     };
     topk_sweep<T, THREADS, 4>(rv, V, t, take, take1);
-    if constexpr (sizeof(T) == 2) mx = make_float2(fmaxf(mx.x, Elem<T>::to_f32(mp.x)), Elem<T>::to_f32(mp.y));
-    s_max[t] = mx.x;
-    s_max[THREADS + t] = mx.y;
+    if constexpr (sizeof(T) == 2) mx = make_float2(fmaxf(mx.x, Elem<T>::to_f32(mp.x)), fmaxf(mx.y, Elem<T>::to_f32(mp.y)));
+    if constexpr (THREADS == 256) { s_max[t] = mx.x; s_max[256 + t] = mx.y; }
+    else {
+      float m = fmaxf(mx.x, mx.y);
+      if constexpr (THREADS == 1024) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      if (THREADS == 512 || (t & 1) == 0) s_max[THREADS == 512 ? t : t >> 1] = m;
+    }
+    if (lse) {
+      const float2 zz = add2(zq[0], zq[1]);
+      const float z = warp_reduce<SumOp>(zz.x + zz.y);
+      if (lane == 0) s_z[warp] = make_float2(z, off);
+    }
     if (t == 0) { s_n = 0; s_hits = 0; }
     __syncthreads();
-    // ---- a lower bound of the K-th largest: warp 0 ----
     if (warp == 0) {
-      unsigned key[2 * NW];
+      // ---- a lower bound of the K-th largest: three thresholds a step, their counts in one word ----
+      constexpr int PER = kTopkGroups / 32;
+      unsigned key[PER];
       unsigned kmin = 0xffffffffu, kmax = 0u;
 #pragma unroll
-      for (int u = 0; u < 2 * NW; ++u) {
+      for (int u = 0; u < PER; ++u) {
         key[u] = order_key(s_max[u * 32 + lane]);
         kmin = key[u] < kmin ? key[u] : kmin;
         kmax = key[u] > kmax ? key[u] : kmax;
       }
       unsigned lo = __reduce_min_sync(0xffffffffu, kmin), hi = __reduce_max_sync(0xffffffffu, kmax);
-      // `lo` is always such that K of the maxima are at or above it: K <= 2 THREADS, and empty ones count as -inf
+      // K of the maxima are always at or above `lo` (K <= 512, and empty groups count as -inf), fewer above `hi`
       while (lo < hi) {
-        const unsigned mid = lo + (hi - lo) / 2 + 1;
-        int n = 0;
+        const unsigned d = hi - lo;
+        const unsigned m1 = lo + d / 4 + 1 <= hi ? lo + d / 4 + 1 : hi, m2 = lo + d / 2 + 1 <= hi ? lo + d / 2 + 1 : hi;
+        const unsigned m3 = lo + d / 2 + d / 4 + 1 <= hi ? lo + d / 2 + d / 4 + 1 : hi;
+        unsigned n = 0;
 #pragma unroll
-        for (int u = 0; u < 2 * NW; ++u) n += key[u] >= mid;
-        n = __reduce_add_sync(0xffffffffu, n);
-        if (n >= K) { lo = mid; if (n <= K + K / 8) break; }
-        else hi = mid - 1;
+        for (int u = 0; u < PER; ++u) n += (key[u] >= m1 ? 1u : 0u) + (key[u] >= m2 ? 1u << 10 : 0u) + (key[u] >= m3 ? 1u << 20 : 0u);
+        n = __reduce_add_sync(0xffffffffu, n);                  // at most 512 each: no carries
+        const int n1 = (int)(n & 1023u), n2 = (int)((n >> 10) & 1023u), n3 = (int)(n >> 20);
+        int at;
+        if (n3 >= K) { lo = m3; at = n3; }
+        else if (n2 >= K) { lo = m2; hi = m3 - 1; at = n2; }
+        else if (n1 >= K) { lo = m1; hi = m2 - 1; at = n1; }
+        else { hi = m1 - 1; continue; }
+        if (at <= K + K / 8) break;
       }
       // a logit's own value, so that it converts to T exactly: the smallest of the maxima at or above the bound
       unsigned up = 0xffffffffu;
 #pragma unroll
-      for (int u = 0; u < 2 * NW; ++u) up = key[u] >= lo && key[u] < up ? key[u] : up;
+      for (int u = 0; u < PER; ++u) up = key[u] >= lo && key[u] < up ? key[u] : up;
       up = __reduce_min_sync(0xffffffffu, up);
       if (lane == 0) s_t = order_value(up);
     }
+    float z = 0.f, zoff = INFINITY;
     if (lse) {
-      const float2 zz = add2(zq[0], zq[1]);
-      float z = block_reduce<SumOp>(zz.x + zz.y, s_red);
+      // the warps' sums under the largest reference (the smallest offset), every thread the same
+      for (int u = 0; u < NW; ++u) if (s_z[u].x != 0.f) zoff = fminf(zoff, s_z[u].y);
+      for (int u = 0; u < NW; ++u) if (s_z[u].x != 0.f) z += s_z[u].x * exp2f_approx(zoff - s_z[u].y);
+    }
+    __syncthreads();
+    if (lse) {
       float sub = 0.f;
       if (!(z > 8.6736174e-19f && z < 1.1529215e18f)) {         // 2^-60, 2^60: against the true maximum, differences first
         float m = -INFINITY;
-        for (int u = t; u < 2 * THREADS; u += THREADS) m = fmaxf(m, s_max[u]);
+        for (int u = t; u < kTopkGroups; u += THREADS) m = fmaxf(m, s_max[u]);
         m = block_reduce<MaxOp>(m, s_red);
         sub = isinf(m) ? 0.f : m;                               // no inf - inf: the sum is then 0 or inf
-        off = 0.f;
+        zoff = 0.f;
         z = 0.f;
         topk_sweep<T, THREADS, 1>(rv, V, t, [&](const uint4& v, int) {
           float a[VEC];
@@ -182,33 +224,37 @@ logits_topk_kernel(T* __restrict__ values, int* __restrict__ indices, float* __r
         }, [&](int j) { z += exp2f_approx((Elem<T>::to_f32(x[j]) - sub) * c); });
         z = block_reduce<SumOp>(z, s_red);
       }
-      if (t == 0) lse[row] = (float)(log((double)z) - (double)off * 0.6931471805599453 + inv_temp * (double)sub);
+      if (t == THREADS - 32) lse[row] = (float)(log((double)z) - (double)zoff * 0.6931471805599453 + inv_temp * (double)sub);
     }
-    __syncthreads();
     // ---- pass 2 ----
-    float bound = s_t;
+    float bound = s_t, above = topk_below<T>(bound);           // collected: what is not less than or equal to `above`
     int n = 0;
-    for (int attempt = 0; attempt < 2; ++attempt) {
-      // vectors that hold such a position first: the elements are looked at one a thread afterwards
-      auto push = [&](int j) {
-        const float a = Elem<T>::to_f32(x[j]);
-        if (!(a <= bound)) {
+    for (int attempt = 0; attempt < 3; ++attempt) {
+      auto push = [&](float a, int j) {
+        if (!(a <= above)) {
           const int slot = atomicAdd(&s_n, 1);
-          if (slot < kTopkCap) s_cand[slot] = ((unsigned long long)order_key(a) << 32) | (0xffffffffu - (unsigned)j);
+          if (slot < kTopkCap)
+            s_cand[slot] = ((unsigned long long)order_key(a) << 32) | ((0x3ffffu - (unsigned)j) << 1) | (a == 0.f && signbit(a) ? 1u : 0u);
         }
       };
       topk_sweep<T, THREADS, 4>(rv, V, t, [&](const uint4& v, int at) {
-        if (topk_any<T>(v, bound)) {
+        if (topk_any<T>(v, above)) {
           const int slot = atomicAdd(&s_hits, 1);
-          if (slot < kTopkCap) s_hit[slot] = at;
+          if (slot < kTopkCap) { s_hit[slot] = v; s_hit_at[slot] = at; }
         }
-      }, push);
+      }, [&](int j) { push(Elem<T>::to_f32(x[j]), j); });
       __syncthreads();
       const int hits = s_hits;
-      for (int q = t; q < (hits < kTopkCap ? hits : 0) * VEC; q += THREADS) push(s_hit[q / VEC] * VEC - rv.head + q % VEC);
+      for (int q = t; q < (hits < kTopkCap ? hits : 0) * VEC; q += THREADS)
+        push(Elem<T>::to_f32(reinterpret_cast<const T*>(s_hit)[q]), s_hit_at[q / VEC] * VEC - rv.head + q % VEC);
       __syncthreads();
       n = hits > kTopkCap ? hits : s_n;
       if (n <= kTopkCap) break;
+      __syncthreads();                                          // everyone has read the counts
+      if (t == 0) { s_n = 0; s_hits = 0; }
+      __syncthreads();
+      above = bound;
+      if (attempt == 0) continue;                               // the same bound, without its equals
       // the exact K-th largest: at most K - 1 positions are above it
       unsigned lo = order_key(bound), hi = 0xffffffffu;
       while (lo < hi) {
@@ -225,19 +271,26 @@ logits_topk_kernel(T* __restrict__ values, int* __restrict__ indices, float* __r
       }
       // K NaNs or more: the bound is NaN, nothing is above it and its positions are the ties
       bound = lo == 0xffffffffu ? __int_as_float(0x7fc00000) : order_value(lo);
-      if (t == 0) { s_n = 0; s_hits = 0; }
-      __syncthreads();
+      above = bound;
       if (bound != bound) { n = 0; break; }
     }
-    // ---- rank: a warp a candidate, counting the larger ones ----
-    for (int q = warp; q < n; q += NW) {
-      const unsigned long long own = s_cand[q];
+    // ---- rank: the number of larger candidates; a candidate's comparisons shared by `parts` neighbouring lanes ----
+    const int parts = n * 4 <= THREADS ? 4 : n * 2 <= THREADS ? 2 : 1;
+    for (int q0 = 0; q0 < n * parts; q0 += THREADS) {           // whole warps take part in the shuffles
+      const int q = (q0 + t) / parts, part = t & (parts - 1);
+      const unsigned long long own = q < n ? s_cand[q] : ~0ull;
       int rank = 0;
-      for (int u = 0; u < n; u += 32) rank += __popc(__ballot_sync(0xffffffffu, u + lane < n && s_cand[u + lane] > own));
-      if (lane == 0 && rank < K) {
-        const int j = (int)(0xffffffffu - (unsigned)own);
-        values[(int64_t)row * K + rank] = x[j];
-        indices[(int64_t)row * K + rank] = j;
+      for (int u = part * 2; u < n; u += 2 * parts) {
+        const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(s_cand + u);
+        rank += (o.x > own ? 1 : 0) + (u + 1 < n && o.y > own ? 1 : 0);
+      }
+      if (parts > 1) rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+      if (parts > 2) rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+      if (q < n && part == 0 && rank < K) {
+        const unsigned key = (unsigned)(own >> 32);
+        const float v = key == 0xffffffffu ? __int_as_float(0x7fc00000) : (own & 1ull) ? -0.f : order_value(key);
+        values[(int64_t)row * K + rank] = Elem<T>::from_f32(v);
+        indices[(int64_t)row * K + rank] = (int)(0x3ffffu - (((unsigned)own >> 1) & 0x3ffffu));
       }
     }
     // ---- the first positions equal to the bound, in index order ----
@@ -266,13 +319,16 @@ static int launch_topk(uint64_t values, uint64_t indices, uint64_t lse, uint64_t
   int* ix = reinterpret_cast<int*>(indices);
   float* ls = reinterpret_cast<float*>(lse);
   const T* l = reinterpret_cast<const T*>(logits);
-  // few rows: 1024 threads bring a row's bytes sooner; otherwise CTAs of 256, so that the passes of several rows overlap on an SM
-  if (rows <= kNumSMs) {
-    logits_topk_kernel<T, 1024><<<(unsigned)rows, 1024, 0, st>>>(v, ix, ls, l, (int)rows, (int)vocab, (int)k, inv_temp);
-  } else {
-    const int64_t cap = (int64_t)kNumSMs * 6;
-    logits_topk_kernel<T, 256><<<(unsigned)(rows < cap ? rows : cap), 256, 0, st>>>(v, ix, ls, l, (int)rows, (int)vocab, (int)k, inv_temp);
-  }
+  // The rows at work have to stay in the 126 MB of L2 between their two passes, and a CTA's serial steps have to be covered by
+  // others on its SM: six CTAs an SM for short rows, three for longer ones, one for the longest; one also for few rows, where 1024
+  // threads bring a row's bytes sooner.
+  const int64_t bytes = vocab * (int64_t)sizeof(T);
+  const int64_t per_sm = rows <= kNumSMs || bytes > 200 * 1024 ? 1 : bytes > 80 * 1024 ? 3 : 6;
+  const int64_t cap = (int64_t)kNumSMs * per_sm;
+  const unsigned grid = (unsigned)(rows < cap ? rows : cap);
+  if (per_sm == 1) logits_topk_kernel<T, 1024><<<grid, 1024, 0, st>>>(v, ix, ls, l, (int)rows, (int)vocab, (int)k, inv_temp);
+  else if (per_sm == 3) logits_topk_kernel<T, 512><<<grid, 512, 0, st>>>(v, ix, ls, l, (int)rows, (int)vocab, (int)k, inv_temp);
+  else logits_topk_kernel<T, 256><<<grid, 256, 0, st>>>(v, ix, ls, l, (int)rows, (int)vocab, (int)k, inv_temp);
   return check_launch();
 }
 
