@@ -5,9 +5,9 @@
 // equal values (+0 equals -0) by ascending index, NaN above +inf.
 //
 // One CTA a row, the row read twice (the second time from L2):
-//   pass 1: 512 groups of positions (by thread and lane of a pair) each keep a running maximum, and every warp sums exponentials
-//           against a reference from its first vectors.  The K-th largest of the 512 maxima is a lower bound t of the K-th largest
-//           logit (K positions at or above it are known); one warp finds it, or a value just below it, by bisection on counts.
+//   pass 1: 512 groups of positions (by thread and lane of a pair) each keep a running maximum, and every warp sums exponentials.
+//           The K-th largest of the 512 maxima is a lower bound t of the K-th largest logit (K positions at or above it are known);
+//           one warp finds it, or a value just below it, by bisection on counts.
 //   pass 2: vectors with a position at or above t are put aside, then these positions, hardly more than K for ordinary rows, are
 //           collected and ranked by counting.
 // More than kTopkCap of them: with many equal to t (few distinct values, masks) only those above t are collected, and the first
@@ -97,27 +97,20 @@ logits_topk_kernel(T* __restrict__ values, int* __restrict__ indices, float* __r
   // candidates: key, then the complement of the index (18 bits; larger is earlier), then 1 for -0
   __shared__ alignas(16) unsigned long long s_cand[kTopkCap + 8];
   __shared__ float s_red[33];
-  __shared__ float2 s_z[NW];                                   // a warp's sum of exponentials and its reference
+  __shared__ float s_z[NW];                                    // a warp's sum of exponentials
   __shared__ int s_n, s_hits, s_warp[NW];
   __shared__ float s_t;
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
   const float c = (float)(inv_temp * 1.4426950408889634);
+  // exponentials are 2^(x c + off): off is a whole number, so it changes no bit of a sum that stays in range, and what suited the row
+  // before is a good guess; a sum out of range is formed again, the same way, with an off of its own
+  float off = 0.f;
   for (int row = blockIdx.x; row < rows; row += gridDim.x) {
     const T* x = L + (int64_t)row * V;
     const RowVecs<T> rv(x, V);
     // ---- pass 1 ----
-    float off = 0.f;
-    if (lse) {
-      // the warp's reference for the exponentials: the largest of its first logits, times c, as a whole number
-      float m = -INFINITY;
-      for (int e = 0; e < 4; ++e) {
-        const int j = warp * 32 * VEC + e * 32 + lane;
-        if (j < V) m = fmaxf(m, Elem<T>::to_f32(x[j]));
-      }
-      m = warp_reduce<MaxOp>(m);
-      off = fabsf(m * c) < 4194304.f ? -rintf(m * c) : 0.f;    // (otherwise the sum falls outside its range and is done again)
-    }
-    const float2 c2 = make_float2(c, c), off2 = make_float2(off, off);
+    const float2 c2 = make_float2(c, c);
+    float2 off2 = make_float2(off, off);
     float2 zq[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
     float2 mx = make_float2(-INFINITY, -INFINITY);
     using P2 = typename Pair16<T>::type;
@@ -149,21 +142,36 @@ logits_topk_kernel(T* __restrict__ values, int* __restrict__ indices, float* __r
         }
       }
     };
-    topk_sweep<T, THREADS, 4>(rv, V, t, take, take1);
-    if constexpr (sizeof(T) == 2) mx = make_float2(fmaxf(mx.x, Elem<T>::to_f32(mp.x)), fmaxf(mx.y, Elem<T>::to_f32(mp.y)));
-    if constexpr (THREADS == 256) { s_max[t] = mx.x; s_max[256 + t] = mx.y; }
-    else {
-      float m = fmaxf(mx.x, mx.y);
-      if constexpr (THREADS == 1024) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-      if (THREADS == 512 || (t & 1) == 0) s_max[THREADS == 512 ? t : t >> 1] = m;
+    float z = 0.f;
+    for (int attempt = 0;; ++attempt) {
+      topk_sweep<T, THREADS, 4>(rv, V, t, take, take1);
+      if constexpr (sizeof(T) == 2) mx = make_float2(fmaxf(mx.x, Elem<T>::to_f32(mp.x)), fmaxf(mx.y, Elem<T>::to_f32(mp.y)));
+      if constexpr (THREADS == 256) { s_max[t] = mx.x; s_max[256 + t] = mx.y; }
+      else {
+        float m = fmaxf(mx.x, mx.y);
+        if constexpr (THREADS == 1024) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        if (THREADS == 512 || (t & 1) == 0) s_max[THREADS == 512 ? t : t >> 1] = m;
+      }
+      if (lse) {
+        const float2 zz = add2(zq[0], zq[1]);
+        const float zw = warp_reduce<SumOp>(zz.x + zz.y);
+        if (lane == 0) s_z[warp] = zw;
+      }
+      if (t == 0) { s_n = 0; s_hits = 0; }
+      __syncthreads();
+      if (!lse) break;
+      z = 0.f;
+      for (int u = 0; u < NW; ++u) z += s_z[u];
+      if (attempt || (z > 8.6736174e-19f && z < 1.1529215e18f)) break;            // 2^-60, 2^60
+      float m = -INFINITY;
+      for (int u = t; u < kTopkGroups; u += THREADS) m = fmaxf(m, s_max[u]);
+      m = block_reduce<MaxOp>(m, s_red);
+      if (!(fabsf(m * c) < 4194304.f)) break;                    // infinite, or near the type's largest magnitudes: below
+      off = -rintf(m * c);
+      off2 = make_float2(off, off);
+      zq[0] = zq[1] = make_float2(0.f, 0.f);
+      __syncthreads();
     }
-    if (lse) {
-      const float2 zz = add2(zq[0], zq[1]);
-      const float z = warp_reduce<SumOp>(zz.x + zz.y);
-      if (lane == 0) s_z[warp] = make_float2(z, off);
-    }
-    if (t == 0) { s_n = 0; s_hits = 0; }
-    __syncthreads();
     if (warp == 0) {
       // ---- a lower bound of the K-th largest: three thresholds a step, their counts in one word ----
       constexpr int PER = kTopkGroups / 32;
@@ -200,21 +208,16 @@ logits_topk_kernel(T* __restrict__ values, int* __restrict__ indices, float* __r
       up = __reduce_min_sync(0xffffffffu, up);
       if (lane == 0) s_t = order_value(up);
     }
-    float z = 0.f, zoff = INFINITY;
-    if (lse) {
-      // the warps' sums under the largest reference (the smallest offset), every thread the same
-      for (int u = 0; u < NW; ++u) if (s_z[u].x != 0.f) zoff = fminf(zoff, s_z[u].y);
-      for (int u = 0; u < NW; ++u) if (s_z[u].x != 0.f) z += s_z[u].x * exp2f_approx(zoff - s_z[u].y);
-    }
     __syncthreads();
     if (lse) {
       float sub = 0.f;
-      if (!(z > 8.6736174e-19f && z < 1.1529215e18f)) {         // 2^-60, 2^60: against the true maximum, differences first
+      double ln_off = (double)off * 0.6931471805599453;
+      if (!(z > 8.6736174e-19f && z < 1.1529215e18f)) {         // still: against the true maximum, differences first
         float m = -INFINITY;
         for (int u = t; u < kTopkGroups; u += THREADS) m = fmaxf(m, s_max[u]);
         m = block_reduce<MaxOp>(m, s_red);
         sub = isinf(m) ? 0.f : m;                               // no inf - inf: the sum is then 0 or inf
-        zoff = 0.f;
+        ln_off = 0.;
         z = 0.f;
         topk_sweep<T, THREADS, 1>(rv, V, t, [&](const uint4& v, int) {
           float a[VEC];
@@ -224,7 +227,7 @@ logits_topk_kernel(T* __restrict__ values, int* __restrict__ indices, float* __r
         }, [&](int j) { z += exp2f_approx((Elem<T>::to_f32(x[j]) - sub) * c); });
         z = block_reduce<SumOp>(z, s_red);
       }
-      if (t == THREADS - 32) lse[row] = (float)(log((double)z) - (double)zoff * 0.6931471805599453 + inv_temp * (double)sub);
+      if (t == THREADS - 32) lse[row] = (float)(log((double)z) - ln_off + inv_temp * (double)sub);
     }
     // ---- pass 2 ----
     float bound = s_t, above = topk_below<T>(bound);           // collected: what is not less than or equal to `above`
@@ -274,24 +277,45 @@ logits_topk_kernel(T* __restrict__ values, int* __restrict__ indices, float* __r
       above = bound;
       if (bound != bound) { n = 0; break; }
     }
-    // ---- rank: the number of larger candidates; a candidate's comparisons shared by `parts` neighbouring lanes ----
-    const int parts = n * 4 <= THREADS ? 4 : n * 2 <= THREADS ? 2 : 1;
-    for (int q0 = 0; q0 < n * parts; q0 += THREADS) {           // whole warps take part in the shuffles
-      const int q = (q0 + t) / parts, part = t & (parts - 1);
-      const unsigned long long own = q < n ? s_cand[q] : ~0ull;
-      int rank = 0;
-      for (int u = part * 2; u < n; u += 2 * parts) {
-        const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(s_cand + u);
-        rank += (o.x > own ? 1 : 0) + (u + 1 < n && o.y > own ? 1 : 0);
+    // ---- the candidates in order ----
+    auto put = [&](unsigned long long cand, int rank) {
+      const unsigned key = (unsigned)(cand >> 32);
+      const float v = key == 0xffffffffu ? __int_as_float(0x7fc00000) : (cand & 1ull) ? -0.f : order_value(key);
+      values[(int64_t)row * K + rank] = Elem<T>::from_f32(v);
+      indices[(int64_t)row * K + rank] = (int)(0x3ffffu - (((unsigned)cand >> 1) & 0x3ffffu));
+    };
+    if (n <= 160) {
+      // few: a candidate's rank is the number of larger ones, its comparisons shared by `parts` neighbouring lanes (n^2 of them:
+      // above about 160 sorting is cheaper)
+      const int parts = n * 4 <= THREADS ? 4 : n * 2 <= THREADS ? 2 : 1;
+      for (int q0 = 0; q0 < n * parts; q0 += THREADS) {         // whole warps take part in the shuffles
+        const int q = (q0 + t) / parts, part = t & (parts - 1);
+        const unsigned long long own = q < n ? s_cand[q] : ~0ull;
+        int rank = 0;
+        for (int u = part * 2; u < n; u += 2 * parts) {
+          const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(s_cand + u);
+          rank += (o.x > own ? 1 : 0) + (u + 1 < n && o.y > own ? 1 : 0);
+        }
+        if (parts > 1) rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+        if (parts > 2) rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+        if (q < n && part == 0 && rank < K) put(own, rank);
       }
-      if (parts > 1) rank += __shfl_xor_sync(0xffffffffu, rank, 1);
-      if (parts > 2) rank += __shfl_xor_sync(0xffffffffu, rank, 2);
-      if (q < n && part == 0 && rank < K) {
-        const unsigned key = (unsigned)(own >> 32);
-        const float v = key == 0xffffffffu ? __int_as_float(0x7fc00000) : (own & 1ull) ? -0.f : order_value(key);
-        values[(int64_t)row * K + rank] = Elem<T>::from_f32(v);
-        indices[(int64_t)row * K + rank] = (int)(0x3ffffu - (((unsigned)own >> 1) & 0x3ffffu));
+    } else {
+      // a bitonic sort, largest first; 0 is below every candidate
+      const int size = n <= 256 ? 256 : n <= 512 ? 512 : 1024;
+      for (int q = n + t; q < size; q += THREADS) s_cand[q] = 0ull;
+      __syncthreads();
+      for (int len = 2; len <= size; len *= 2) {
+        for (int gap = len / 2; gap > 0; gap /= 2) {
+          for (int q = t; q < size / 2; q += THREADS) {
+            const int i = 2 * q - (q & (gap - 1)), j = i + gap;
+            const unsigned long long a = s_cand[i], b = s_cand[j];
+            if ((a < b) == ((i & len) == 0)) { s_cand[i] = b; s_cand[j] = a; }
+          }
+          __syncthreads();
+        }
       }
+      for (int q = t; q < (n < K ? n : K); q += THREADS) put(s_cand[q], q);
     }
     // ---- the first positions equal to the bound, in index order ----
     for (int j0 = 0, have = n; have < K && j0 < V; j0 += THREADS) {
