@@ -140,8 +140,8 @@ template <bool SAVE> constexpr size_t ffn_fwd_smem() {
 }
 
 // PAIR: a cluster of two CTAs computes 256 tokens x 128 columns of h (a 256 x 256 accumulator).
-// Otherwise one CTA computes 128 tokens x 64 columns (a 128 x 128 accumulator): for few tokens, where the block is bound
-// by reading the weights and 64-column tiles spread them over twice as many SMs.
+// Otherwise one CTA computes 128 tokens x 64 columns (a 128 x 128 accumulator): for few tokens, where the block is bound by reading
+// the weights and 64-column tiles spread them over twice as many SMs (the rule is in ffn_fwd_run).
 template <typename T, bool PAIR, bool SAVE>
 __device__ __forceinline__ void ffn_fwd_body(const FfnMaps& maps, T* __restrict__ H, T* __restrict__ G, T* __restrict__ U, const FfnFwdParams& p) {
   constexpr int HALF = PAIR ? 128 : 64, STAGES = ffn_fwd_stages<SAVE>(), TM = PAIR ? 256 : 128;
@@ -277,15 +277,54 @@ ffn_fwd_kernel(const __grid_constant__ FfnMaps maps, T* __restrict__ H, T* __res
   ffn_fwd_body<T, false, SAVE>(maps, H, G, U, p);
 }
 
-// A packed matrix as an operand; repacked into the workspace when TMA cannot address it.
-static int ffn_operand(Operand& o, uint64_t ptr, int64_t rows, int64_t cols, uint64_t ws, size_t ws_bytes, size_t& off, cudaStream_t st) {
-  o = Operand{ptr, rows, cols, cols, 0, 0, 0, 0};
-  if (tma_ok(o, 1, 1)) return CACTI_B200_OK;
-  const size_t need = packed_bytes(rows, cols, 1);
-  if (!ws || (ws & 255) || off + need > ws_bytes) return CACTI_B200_ERR_WORKSPACE;
-  const int rc = repack_operand(o, 1, 1, ws + off, st);
-  off += need;
-  return rc;
+// Up to three packed matrices [rows][cols] to rows of cols_pad (a multiple of 64) with zeros behind the data, for operands that TMA
+// cannot address.  One 16-byte vector a thread: five aligned 4-byte loads, shifted where the row starts at an odd element.
+struct FfnPack { const unsigned char* src[3]; uint4* dst[3]; unsigned first[4]; unsigned rows[3]; };   // first: vector counts, running
+__global__ void __launch_bounds__(256) ffn_pack_kernel(const FfnPack p, unsigned cols, unsigned vpr /* vectors per padded row */) {
+  const unsigned i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= p.first[3]) return;
+  const int m = i >= p.first[2] ? 2 : i >= p.first[1] ? 1 : 0;
+  const unsigned v = i - p.first[m], row = v / vpr, c = (v - row * vpr) * 8;
+  const uint64_t begin = reinterpret_cast<uint64_t>(p.src[m]), end = begin + (uint64_t)p.rows[m] * cols * 2;
+  const uint64_t a = begin + ((uint64_t)row * cols + c) * 2, base = a & ~3ull;
+  uint32_t o[4] = {0, 0, 0, 0};
+  if (c + 8 <= cols && base >= begin && base + 20 <= end) {
+    const uint32_t* s = reinterpret_cast<const uint32_t*>(base);
+    uint32_t w[5];
+#pragma unroll
+    for (int k = 0; k < 5; ++k) w[k] = __ldg(s + k);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] = (a & 2) ? __funnelshift_r(w[k], w[k + 1], 16) : w[k];
+  } else {                                                      // a row's end, the matrix's ends
+    for (unsigned k = 0; k < 8; ++k)
+      if (c + k < cols) o[k >> 1] |= (uint32_t)reinterpret_cast<const unsigned short*>(a)[k] << (16 * (k & 1));
+  }
+  p.dst[m][v] = make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+// Packed matrices as operands; those that TMA cannot address are repacked into the workspace, in one launch.
+static int ffn_operands(Operand (&o)[3], const uint64_t (&ptr)[3], const int64_t (&rows)[3], int64_t cols, uint64_t ws, size_t ws_bytes,
+                        size_t off, cudaStream_t st) {
+  FfnPack p{};
+  const int64_t cp = packed_cols(cols), vpr = cp / 8;
+  unsigned n = 0;
+  for (int i = 0; i < 3; ++i) {
+    o[i] = Operand{ptr[i], rows[i], cols, cols, 0, 0, 0, 0};
+    p.first[i] = n;
+    if (tma_ok(o[i], 1, 1)) continue;
+    const size_t need = packed_bytes(rows[i], cols, 1);
+    if (!ws || (ws & 255) || off + need > ws_bytes) return CACTI_B200_ERR_WORKSPACE;
+    p.src[i] = reinterpret_cast<const unsigned char*>(ptr[i]);
+    p.dst[i] = reinterpret_cast<uint4*>(ws + off);
+    p.rows[i] = (unsigned)rows[i];
+    n += (unsigned)(rows[i] * vpr);
+    o[i].ptr = ws + off; o[i].ld = cp; o[i].map_cols = cp;
+    off += need;
+  }
+  p.first[3] = n;
+  if (!n) return CACTI_B200_OK;
+  ffn_pack_kernel<<<(n + 255) / 256, 256, 0, st>>>(p, (unsigned)cols, (unsigned)vpr);
+  return check_launch();
 }
 
 // Sizes whose tile, k-block and vector counts fit 32-bit indices (any that fit the device's memory do).
@@ -305,13 +344,16 @@ template <typename T>
 static int ffn_fwd_run(uint64_t h, uint64_t gate, uint64_t up, uint64_t x, uint64_t wg, uint64_t wu, int64_t tokens, int64_t D,
                        int64_t F, uint64_t ws, size_t ws_bytes, cudaStream_t st) {
   const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
-  Operand ox, og, ou;
-  size_t off = 0;
-  int rc = ffn_operand(ox, x, tokens, D, ws, ws_bytes, off, st);
-  if (!rc) rc = ffn_operand(og, wg, F, D, ws, ws_bytes, off, st);
-  if (!rc) rc = ffn_operand(ou, wu, F, D, ws, ws_bytes, off, st);
+  Operand op[3];
+  int rc = ffn_operands(op, {x, wg, wu}, {tokens, F, F}, D, ws, ws_bytes, 0, st);
   if (rc) return rc;
-  const bool save = gate != 0, pair = tokens > kBM;
+  // Two-SM tiles of 256 tokens x 128 columns, or one-SM tiles of 128 x 64, whichever needs less time: waves of the persistent grid
+  // times a tile's cost per wave.  The costs are the matmul kernels' (gemm.cu): 0.93 of 256 columns against 1.3 of 128; measured here
+  // at 333 x 1160 x 3080: one-SM 147 tiles in one wave 13.5 us, two-SM 50 tiles 17.5 us; at 2048 x 3200 x 8640: 250 us against 187 us.
+  auto waves = [](int64_t tiles, int64_t workers) { return (double)((tiles + workers - 1) / workers); };
+  const double cost2 = waves((tokens + 255) / 256 * ((F + 127) / 128), kNumSMs / 2) * 256 * 0.93;
+  const double cost1 = waves((tokens + 127) / 128 * ((F + 63) / 64), kNumSMs) * 128 * 1.3;
+  const bool save = gate != 0, pair = tokens > kBM && cost2 <= cost1;
   const int tm = pair ? 256 : 128, half = pair ? 128 : 64;
   FfnFwdParams p;
   p.M = (int)tokens; p.N = (int)F; p.nkb = (int)((D + kBK - 1) / kBK);
@@ -321,9 +363,9 @@ static int ffn_fwd_run(uint64_t h, uint64_t gate, uint64_t up, uint64_t x, uint6
   p.a_rows = pair || tokens >= 128 ? 128 : (int)((tokens + 7) / 8 * 8);
   p.out_tma = ffn_rows_aligned(h, F) && (!save || (ffn_rows_aligned(gate, F) && ffn_rows_aligned(up, F)));
   FfnMaps maps;
-  rc = encode_operand(&maps.a[0], ox, 1, 1, 64, p.a_rows, bf16);
-  if (!rc) rc = encode_operand(&maps.b[0], og, 1, 1, 64, half, bf16);
-  if (!rc) rc = encode_operand(&maps.b[1], ou, 1, 1, 64, half, bf16);
+  rc = encode_operand(&maps.a[0], op[0], 1, 1, 64, p.a_rows, bf16);
+  if (!rc) rc = encode_operand(&maps.b[0], op[1], 1, 1, 64, half, bf16);
+  if (!rc) rc = encode_operand(&maps.b[1], op[2], 1, 1, 64, half, bf16);
   maps.a[1] = maps.ak[0] = maps.ak[1] = maps.a[0]; maps.b[2] = maps.b[0];
   for (int i = 0; i < 3; ++i) {
     maps.c[i] = maps.a[0];
@@ -422,28 +464,37 @@ __device__ __forceinline__ FfnItem ffn_item(const FfnBwdParams& p, int t) {
   return it;
 }
 
-// Epilogue of a range of dx's contraction: the f32 accumulator to its place in the partial sums.
-template <int BN>
-__device__ __forceinline__ void ffn_partial_tile(float* __restrict__ part, int M, int N, uint32_t tmem_base, int acc, int row, int tn,
-                                                 int q, int lane, uint32_t tempty_addr) {
+// Epilogues by rows: 64 accumulator columns at a time to f32 staging (one thread a row, 16-byte chunks placed by row so that neither
+// side conflicts), then one row at a time to memory, consecutive lanes consecutive columns.  emit(row, column, value).
+template <int BN, typename F>
+__device__ __forceinline__ void ffn_tile_rows(int M, int N, uint32_t tmem_base, int acc, int row0, int tn, int q, int lane, unsigned char* mybuf,
+                                              uint32_t tempty_addr, F&& emit) {
 #pragma unroll 1
-  for (int c = 0; c < BN / 32; ++c) {
-    const int col0 = tn * BN + c * 32;
+  for (int c = 0; c < BN / 64; ++c) {
+    const int col0 = tn * BN + c * 64;
     if (col0 >= N) break;                // warp-uniform
-    uint32_t v[32];
-    tc_ld32(tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN + c * 32), v);
-    tc_ld_wait();
-    if (row < M) {
-      float* out = part + (long long)row * N + col0;
-      if ((N & 3) == 0) {                // col0 + 4 i + 3 < N whenever col0 + 4 i < N
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (col0 + 4 * i < N) __stcg(reinterpret_cast<uint4*>(out) + i, make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]));
-      } else {
+    for (int hh = 0; hh < 2; ++hh) {
+      uint32_t v[32];
+      tc_ld32(tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN + c * 64 + hh * 32), v);
+      tc_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) if (col0 + i < N) __stcg(out + i, __uint_as_float(v[i]));
+      for (int k = 0; k < 8; ++k)
+        *reinterpret_cast<uint4*>(mybuf + lane * 256 + (((hh * 8 + k) ^ (lane & 15)) << 4)) = make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+    }
+    __syncwarp();
+#pragma unroll 4
+    for (int r = 0; r < 32; ++r) {
+      if (row0 + r < M) {
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          const int j = hh * 32 + lane;
+          if (col0 + j < N)
+            emit(row0 + r, col0 + j, *reinterpret_cast<const float*>(mybuf + r * 256 + (((j >> 2) ^ (r & 15)) << 4) + (j & 3) * 4));
+        }
       }
     }
+    __syncwarp();
   }
   tc_fence_before();
   __syncwarp();
@@ -602,11 +653,21 @@ ffn_bwd_kernel(const __grid_constant__ FfnMaps maps, T* __restrict__ dX, T* __re
       const int row0 = it.tm * 256 + (int)rank * kBM + q * 32;
       const uint32_t te = map_to_rank(smem_u32(tempty + acc), 0);
       const GemmParams& g = p.pr[it.prod].g;
-      if (it.prod == 0 && p.splits > 1)
-        ffn_partial_tile<BN>(p.part + (long long)it.split * g.M * g.N, g.M, g.N, tmem_base, acc, row0 + lane, it.tn, q, lane, te);
-      else
-        epilogue_tile<T, BN>(g, maps.c[it.prod + it.part], it.prod == 0 ? dX : it.part ? dWu : dWg, tmem_base, acc, row0, it.tn, 0, 0, q,
-                             lane, cstage + (size_t)(warp - 2) * 8192, te, cbar + (warp - 2), cpar);
+      unsigned char* stage = cstage + (size_t)(warp - 2) * 8192;
+      T* out = it.prod == 0 ? dX : it.part ? dWu : dWg;
+      if ((it.prod == 0 && p.splits > 1) || !g.c_tma) {
+        // a range's partial sums, or a result whose rows TMA cannot address
+        float* part = it.prod == 0 && p.splits > 1 ? p.part + (long long)it.split * g.M * g.N : nullptr;
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");     // the staging has been read
+        __syncwarp();
+        ffn_tile_rows<BN>(g.M, g.N, tmem_base, acc, row0, it.tn, q, lane, stage, te, [&](int r, int j, float v) {
+          const long long at = (long long)r * g.N + j;
+          if (part) __stcg(part + at, v);
+          else out[at] = Elem<T>::from_f32(g.beta != 0.f ? v + Elem<T>::to_f32(out[at]) : v);
+        });
+      } else {
+        epilogue_tile<T, BN>(g, maps.c[it.prod + it.part], out, tmem_base, acc, row0, it.tn, 0, 0, q, lane, stage, te, cbar + (warp - 2), cpar);
+      }
     }
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
@@ -686,7 +747,7 @@ static int ffn_bwd_run(uint64_t dx, uint64_t dwg, uint64_t dwu, uint64_t dh, uin
   unsigned* counter = reinterpret_cast<unsigned*>(ws);
   size_t off = 256 + 2 * b.dpart + b.part;
   if (!ws || (ws & 255) || ws_bytes < off) return CACTI_B200_ERR_WORKSPACE;
-  Operand ox, og, ou;
+  Operand op[3];
   for (const auto& [ptr, rows] : {std::pair<uint64_t, int64_t>{x, tokens}, {wg, F}, {wu, F}}) {     // before anything is launched
     if (!ffn_rows_aligned(ptr, D)) off += packed_bytes(rows, D, 1);
   }
@@ -700,9 +761,7 @@ static int ffn_bwd_run(uint64_t dx, uint64_t dwg, uint64_t dwu, uint64_t dh, uin
                                                reinterpret_cast<const T*>(dh), reinterpret_cast<const T*>(gate),
                                                reinterpret_cast<const T*>(up), nvec, (unsigned)F, vpr, counter);
   int rc = check_launch();
-  if (!rc) rc = ffn_operand(ox, x, tokens, D, ws, ws_bytes, off, st);
-  if (!rc) rc = ffn_operand(og, wg, F, D, ws, ws_bytes, off, st);
-  if (!rc) rc = ffn_operand(ou, wu, F, D, ws, ws_bytes, off, st);
+  if (!rc) rc = ffn_operands(op, {x, wg, wu}, {tokens, F, F}, D, ws, ws_bytes, off, st);
   if (rc) return rc;
   FfnMaps maps;
   for (int i = 0; i < 2 && !rc; ++i) {
@@ -710,9 +769,9 @@ static int ffn_bwd_run(uint64_t dx, uint64_t dwg, uint64_t dwu, uint64_t dh, uin
     rc = encode_operand(&maps.a[i], o, 1, 1, 64, 64, bf16);
     if (!rc) rc = encode_operand(&maps.ak[i], o, 1, 1, 64, kBM, bf16);
   }
-  if (!rc) rc = encode_operand(&maps.b[0], og, 1, 1, 64, 64, bf16);
-  if (!rc) rc = encode_operand(&maps.b[1], ou, 1, 1, 64, 64, bf16);
-  if (!rc) rc = encode_operand(&maps.b[2], ox, 1, 1, 64, 64, bf16);
+  if (!rc) rc = encode_operand(&maps.b[0], op[1], 1, 1, 64, 64, bf16);
+  if (!rc) rc = encode_operand(&maps.b[1], op[2], 1, 1, 64, 64, bf16);
+  if (!rc) rc = encode_operand(&maps.b[2], op[0], 1, 1, 64, 64, bf16);
   if (rc) return rc;
   for (auto& m : maps.c) m = maps.a[0];
   FfnBwdParams p;

@@ -33,7 +33,8 @@ def _ptr(t) -> int:
 
 
 def _stream():
-    return torch.cuda.current_stream().cuda_stream
+    # the handle of torch.cuda.current_stream() without the Stream object around it (3 us of a call's host time)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _ws(nbytes: int, device) -> torch.Tensor:
