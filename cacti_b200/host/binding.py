@@ -38,6 +38,12 @@ def lib():
             "cbh_thunk_swiglu_fwd": (C.c_int, [_p, C.c_int, _i64, _i64, _i64, _i64, C.c_int]),
             "cbh_thunk_swiglu_bwd": (C.c_int, [_p, C.c_int, C.c_int, _i64, _i64, _i64, _i64, _i64, _i64, C.c_int]),
             "cbh_thunk_softmax_nll": (C.c_int, [_p, C.c_int, _i64, _i64, _i64, _i64, C.c_int, C.c_float, _i64, _i64, C.c_int, _i64]),
+            "cbh_thunk_distill_topk": (C.c_int, [_p, C.c_int, _i64, _i64, _i64, _i64, C.c_int, _i64, C.c_int, _i64, _i64, C.c_float,
+                                                 C.c_float, _i64, _i64, C.c_int, _i64]),
+            "cbh_thunk_logits_topk": (C.c_int, [_p, C.c_int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, C.c_float, C.c_int]),
+            "cbh_thunk_gated_ffn_fwd": (C.c_int, [_p, C.c_int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, C.c_int]),
+            "cbh_thunk_gated_ffn_bwd": (C.c_int, [_p, C.c_int, C.c_int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                                                  _i64, _i64, C.c_int]),
             "cbh_thunk_gather_rows": (C.c_int, [_p, C.c_int, _i64, _i64, _i64, C.c_int, _i64, _i64, _i64, C.c_int, _i64]),
             "cbh_thunk_scatter_add_rows": (C.c_int, [_p, C.c_int, _i64, _i64, _i64, C.c_int, _i64, _i64, _i64, C.c_int, _i64]),
             "cbh_thunk_block_pad": (C.c_int, [_p, C.c_int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, C.c_int]),

@@ -486,6 +486,55 @@ int thunk_softmax_nll(PCtx& p, Mode m_dlogits, int64_t loss_sum, int64_t dlogits
                                         p.stream());
 }
 
+int thunk_distill_topk(PCtx& p, Mode m_dlogits, int64_t loss_sum, int64_t dlogits, int64_t logits, int64_t t_values, int t_dtype,
+                       int64_t t_indices, int index_dtype, int64_t t_lse, int64_t k, float temperature, float w, int64_t rows,
+                       int64_t vocab, int dtype, int64_t status) {
+  if (m_dlogits == kInitialize) return CACTI_B200_ERR_INVALID_VALUE;
+  Binding b(p);
+  const uint64_t dl = b.in(logits), dv = b.in(t_values), di = b.in(t_indices), de = t_lse >= 0 ? b.in(t_lse) : 0;
+  const uint64_t dsum = b.opt_out(loss_sum, kApply), dd = b.opt_out(dlogits, m_dlogits), dst = b.opt_out(status, kAccumulate);
+  const size_t wsb = cacti_b200_distill_topk_workspace_bytes(rows);
+  const uint64_t ws = b.temp(wsb);
+  if (!b.ok) return -1;
+  return cacti_b200_distill_topk_fwd_bwd(dsum, 0, dd, dl, dv, t_dtype, di, index_dtype, de, k, temperature, 0, w, rows, vocab, dtype,
+                                         beta_of(m_dlogits), dst, ws, wsb, p.stream());
+}
+
+int thunk_logits_topk(PCtx& p, Mode m, int64_t values, int64_t indices, int64_t lse, int64_t logits, int64_t rows, int64_t vocab, int64_t k,
+                      float temperature, int dtype) {
+  if (m != kApply) return CACTI_B200_ERR_INVALID_VALUE;
+  Binding b(p);
+  const uint64_t dl = b.in(logits), dv = b.out(values, kApply), di = b.out(indices, kApply), de = b.opt_out(lse, kApply);
+  if (!b.ok) return -1;
+  return cacti_b200_logits_topk(dv, di, de, dl, rows, vocab, k, temperature, dtype, p.stream());
+}
+
+int thunk_gated_ffn_fwd(PCtx& p, Mode m, int64_t h, int64_t gate, int64_t up, int64_t x, int64_t w_gate, int64_t w_up, int64_t tokens,
+                        int64_t d_model, int64_t d_ffn, int dtype) {
+  if (m != kApply) return CACTI_B200_ERR_INVALID_VALUE;
+  Binding b(p);
+  const uint64_t dx = b.in(x), dg = b.in(w_gate), du = b.in(w_up), dh = b.out(h, kApply);
+  const uint64_t og = b.opt_out(gate, kApply), ou = b.opt_out(up, kApply);
+  // cells start 256-byte aligned
+  const size_t wsb = cacti_b200_gated_ffn_fwd_workspace_bytes(tokens, d_model, d_ffn, 1);
+  const uint64_t ws = b.temp(wsb);
+  if (!b.ok) return -1;
+  return cacti_b200_gated_ffn_fwd(dh, og, ou, dx, dg, du, tokens, d_model, d_ffn, dtype, ws, wsb, p.stream());
+}
+
+int thunk_gated_ffn_bwd(PCtx& p, Mode m_dx, Mode m_dw, int64_t dx, int64_t dw_gate, int64_t dw_up, int64_t dh, int64_t x, int64_t w_gate,
+                        int64_t w_up, int64_t gate, int64_t up, int64_t tokens, int64_t d_model, int64_t d_ffn, int dtype) {
+  if (m_dx == kInitialize || m_dw == kInitialize) return CACTI_B200_ERR_INVALID_VALUE;
+  Binding b(p);
+  const uint64_t ddh = b.in(dh), dxx = b.in(x), dg = b.in(w_gate), du = b.in(w_up), sg = b.in(gate), su = b.in(up);
+  const uint64_t ox = b.out(dx, m_dx), og = b.out(dw_gate, m_dw), ou = b.out(dw_up, m_dw);
+  const size_t wsb = cacti_b200_gated_ffn_bwd_workspace_bytes(tokens, d_model, d_ffn, 1);
+  const uint64_t ws = b.temp(wsb);
+  if (!b.ok) return -1;
+  return cacti_b200_gated_ffn_bwd(ox, og, ou, ddh, dxx, dg, du, sg, su, tokens, d_model, d_ffn, dtype, beta_of(m_dx), beta_of(m_dw), ws,
+                                  wsb, p.stream());
+}
+
 int thunk_gather_rows(PCtx& p, Mode m, int64_t out, int64_t table, int64_t tokens, int token_dtype, int64_t n, int64_t vocab,
                       int64_t cols, int dtype, int64_t status) {
   if (m != kApply) return CACTI_B200_ERR_INVALID_VALUE;
@@ -659,6 +708,25 @@ int cbh_thunk_swiglu_bwd(void* c, int m_dgate, int m_dup, int64_t dgate, int64_t
 int cbh_thunk_softmax_nll(void* c, int m_dlogits, int64_t loss_sum, int64_t dlogits, int64_t logits, int64_t targets, int target_dtype,
                           float w, int64_t rows, int64_t vocab, int dtype, int64_t status) {
   return cbh::thunk_softmax_nll(CBH_P, CBH_M(m_dlogits), loss_sum, dlogits, logits, targets, target_dtype, w, rows, vocab, dtype, status);
+}
+int cbh_thunk_distill_topk(void* c, int m_dlogits, int64_t loss_sum, int64_t dlogits, int64_t logits, int64_t t_values, int t_dtype,
+                           int64_t t_indices, int index_dtype, int64_t t_lse, int64_t k, float temperature, float w, int64_t rows,
+                           int64_t vocab, int dtype, int64_t status) {
+  return cbh::thunk_distill_topk(CBH_P, CBH_M(m_dlogits), loss_sum, dlogits, logits, t_values, t_dtype, t_indices, index_dtype, t_lse, k,
+                                 temperature, w, rows, vocab, dtype, status);
+}
+int cbh_thunk_logits_topk(void* c, int mode, int64_t values, int64_t indices, int64_t lse, int64_t logits, int64_t rows, int64_t vocab,
+                          int64_t k, float temperature, int dtype) {
+  return cbh::thunk_logits_topk(CBH_P, CBH_M(mode), values, indices, lse, logits, rows, vocab, k, temperature, dtype);
+}
+int cbh_thunk_gated_ffn_fwd(void* c, int mode, int64_t h, int64_t gate, int64_t up, int64_t x, int64_t w_gate, int64_t w_up, int64_t tokens,
+                            int64_t d_model, int64_t d_ffn, int dtype) {
+  return cbh::thunk_gated_ffn_fwd(CBH_P, CBH_M(mode), h, gate, up, x, w_gate, w_up, tokens, d_model, d_ffn, dtype);
+}
+int cbh_thunk_gated_ffn_bwd(void* c, int m_dx, int m_dw, int64_t dx, int64_t dw_gate, int64_t dw_up, int64_t dh, int64_t x, int64_t w_gate,
+                            int64_t w_up, int64_t gate, int64_t up, int64_t tokens, int64_t d_model, int64_t d_ffn, int dtype) {
+  return cbh::thunk_gated_ffn_bwd(CBH_P, CBH_M(m_dx), CBH_M(m_dw), dx, dw_gate, dw_up, dh, x, w_gate, w_up, gate, up, tokens, d_model, d_ffn,
+                                  dtype);
 }
 int cbh_thunk_gather_rows(void* c, int mode, int64_t out, int64_t table, int64_t tokens, int token_dtype, int64_t n, int64_t vocab,
                           int64_t cols, int dtype, int64_t status) {

@@ -156,6 +156,13 @@ int thunk_swiglu_bwd(PCtx& p, Mode m_dgate, Mode m_dup, int64_t dgate, int64_t d
 // loss_sum (f32[1]) and dlogits; status: u32 cell the caller zeroed; the per-row workspace is a temporary cell
 int thunk_softmax_nll(PCtx& p, Mode m_dlogits, int64_t loss_sum, int64_t dlogits, int64_t logits, int64_t targets, int target_dtype,
                       float w, int64_t rows, int64_t vocab, int dtype, int64_t status);
+// distillation: t_lse may be -1 (renormalise over the list); the per-row workspace is a temporary cell
+int thunk_distill_topk(PCtx& p, Mode m_dlogits, int64_t loss_sum, int64_t dlogits, int64_t logits, int64_t t_values, int t_dtype,
+                       int64_t t_indices, int index_dtype, int64_t t_lse, int64_t k, float temperature, float w, int64_t rows,
+                       int64_t vocab, int dtype, int64_t status);
+// the teacher's side: values, indices and (or -1) lse
+int thunk_logits_topk(PCtx& p, Mode m, int64_t values, int64_t indices, int64_t lse, int64_t logits, int64_t rows, int64_t vocab, int64_t k,
+                      float temperature, int dtype);
 int thunk_gather_rows(PCtx& p, Mode m, int64_t out, int64_t table, int64_t tokens, int token_dtype, int64_t n, int64_t vocab,
                       int64_t cols, int dtype, int64_t status);
 int thunk_scatter_add_rows(PCtx& p, Mode m, int64_t dtable, int64_t dy, int64_t tokens, int token_dtype, int64_t n, int64_t vocab,
@@ -172,6 +179,11 @@ int thunk_attention_bwd_prep(PCtx& p, Mode m, int64_t prob, int64_t ds, int64_t 
 // three outputs (dq, dk, dv); P and dS never exist as cells
 int thunk_attention_bwd(PCtx& p, Mode m, int64_t dq, int64_t dk, int64_t dv, int64_t q, int64_t k, int64_t v, int64_t dctx, int64_t ctx,
                         int64_t stats, int64_t batch, int64_t seq, int64_t heads, int64_t hd, float alpha, int dtype);
+// gated feed-forward block; gate and up may both be -1 (nothing kept for the adjoint).  Workspaces are temporary cells.
+int thunk_gated_ffn_fwd(PCtx& p, Mode m, int64_t h, int64_t gate, int64_t up, int64_t x, int64_t w_gate, int64_t w_up, int64_t tokens,
+                        int64_t d_model, int64_t d_ffn, int dtype);
+int thunk_gated_ffn_bwd(PCtx& p, Mode m_dx, Mode m_dw, int64_t dx, int64_t dw_gate, int64_t dw_up, int64_t dh, int64_t x, int64_t w_gate,
+                        int64_t w_up, int64_t gate, int64_t up, int64_t tokens, int64_t d_model, int64_t d_ffn, int dtype);
 // Initialize mode only: master, grad1_avg, grad2_avg are read and overwritten, param_out rewritten (AdamW32::step,
 // src/librarium/adamw.rs:46-61)
 int thunk_adamw32_step(PCtx& p, Mode m, int64_t master, int64_t grad1_avg, int64_t grad2_avg, int64_t param_out, int64_t grad, int64_t n,

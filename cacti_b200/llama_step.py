@@ -14,6 +14,11 @@ arithmetic step is a `cacti_b200_*` call.  Differences from the reference graph,
     not computed (the masked softmax never reads them) and products with the exact zeros of P and dS are skipped;
     every value that is used is bit-identical to the full product.  The softmax zero-fills the masked tails of P
     and dS only as far as those matmuls read (CACTI_B200_MASK_CAUSAL_TRIM).
+  * `ffn="fused"` runs each layer's gate and up projections, the activation and the product as one kernel and their adjoint as one
+    product launch (cacti_b200_gated_ffn_fwd / _bwd: fewer roundings than the reference's thunks, so not its bits); the default keeps
+    the separate thunks;
+  * `forward_backward(teacher=...)` takes the distillation loss against a teacher's listed logits instead of, or beside, the
+    cross-entropy; `teacher_topk` is the teacher's forward pass that makes them.  The reference has neither;
   * by default attention runs fused (cacti_b200_attention_fwd / _bwd_prep): scores and probabilities stay on chip in
     the forward, and the backward rebuilds P and dS per tile instead of reading stored scores, materialises them once
     and multiplies them with the three hinted block matmuls.  `attention="fused-bwd"` keeps P and dS on chip in the
@@ -92,6 +97,17 @@ def stacked(*ts):
     return torch.as_strided(t0, (len(ts), t0.shape[0], 1, t0.shape[1]), (t0.numel(), t0.shape[1], t0.shape[1], 1))
 
 
+@dataclass
+class Teacher:
+    """A teacher's listed logits for the tokens of a step (what TrainStep.teacher_topk of the teacher's own step returns):
+    `weight` of the loss is the distillation loss against them, 1 - weight the cross-entropy of the targets."""
+    values: torch.Tensor                    # [tokens, k]
+    indices: torch.Tensor                   # int32 [tokens, k], -1: unused
+    lse: torch.Tensor | None = None         # f32 [tokens]: the unlisted words form one bucket; None: renormalise over the list
+    temperature: float = 1.0
+    weight: float = 1.0
+
+
 def zeros_like_params(P):
     out = {k: torch.zeros_like(v) for k, v in P.items() if k != "layers"}
     out["layers"] = [{k: torch.zeros_like(v) for k, v in L.items()} for L in P["layers"]]
@@ -112,7 +128,8 @@ class TrainStep:
     gradients are complete, and with i = cfg.layers as soon as the output head's gradients are (the hook a
     data-parallel reducer attaches to; the embedding gradient is complete when the call returns)."""
 
-    def __init__(self, cfg: LlamaShape, params, batch: int, loss_tokens: int | None = None, attention: str = "auto"):
+    def __init__(self, cfg: LlamaShape, params, batch: int, loss_tokens: int | None = None, attention: str = "auto",
+                 ffn: str = "unfused"):
         self.cfg, self.P, self.B = cfg, params, batch
         # "fused": attention_fwd / attention_bwd_prep (scores never reach HBM); "unfused": the reference's op sequence,
         # block matmul - softmax - block matmul; "auto": fused when the shape allows it
@@ -123,6 +140,10 @@ class TrainStep:
             raise ValueError("fused attention needs seq % 128 == 0, head_dim <= 128 and head_dim % 4 == 0")
         self.fused = can_fuse if attention == "auto" else attention in ("fused", "fused-bwd")
         self.fused_bwd = attention == "fused-bwd"       # the backward keeps P and dS on chip as well
+        # "fused": gated_ffn_fwd / _bwd (f32 up to h's one rounding); "unfused": two matmuls and swiglu, rounding as the reference
+        if ffn not in ("unfused", "fused"):
+            raise ValueError(f"ffn={ffn!r}")
+        self.ffn_fused = ffn == "fused"
         dev = params["embed"].device
         self.dev = dev
         self.T = batch * cfg.seq
@@ -135,6 +156,10 @@ class TrainStep:
         self.gemm_ws = torch.empty(nb, dtype=torch.uint8, device=dev)
         # dense matmuls: partial sums of the k-split schedule (all operands here are TMA-addressable, nothing is repacked)
         self.mm_ws = ops.gemm_workspace(0, 0, 0, dev)
+        self.ffn_ws = None
+        if self.ffn_fused:
+            nb = L.cacti_b200_gated_ffn_bwd_workspace_bytes(self.T, cfg.d_model, cfg.ffn, 0)
+            self.ffn_ws = torch.empty(nb, dtype=torch.uint8, device=dev)
         self.norm_ws = ops.rmsnorm_workspace(self.T, cfg.d_model, dev)
         self.status = torch.zeros(1, dtype=torch.int32, device=dev)
         self.launches = 0
@@ -158,7 +183,15 @@ class TrainStep:
         b4 = b if b.dim() == 4 else b.view(1, b.shape[0], 1, b.shape[1])
         return ops.block_gemm(a4, b4, ta, tb, workspace=self.gemm_ws, c=c)
 
-    def forward_backward(self, tokens, targets, grads, on_layer_done=None):
+    def teacher_topk(self, tokens, k, temperature=1.0, weight=1.0):
+        """A forward pass reduced to each token's k largest logits and their log-sum-exp: the Teacher of a student's step."""
+        logits = self._forward(tokens, None)[-1]
+        values, indices, lse = ops.logits_topk(logits, k, temperature)
+        self.launches += 1
+        return Teacher(values, indices, lse, temperature, weight)
+
+    def _forward(self, tokens, saved):
+        """(nf, x, logits); what the backward needs is appended to `saved` layer by layer (None: nothing is kept)."""
         cfg, P, B, T = self.cfg, self.P, self.B, self.T
         S, H, hd, D = cfg.seq, cfg.heads, cfg.head_dim, cfg.d_model
         alpha = 1.0 / math.sqrt(hd)
@@ -168,7 +201,6 @@ class TrainStep:
         self.launches = 0
         x, _ = ops.gather_rows(P["embed"], tokens, status=self.status)
         self.launches += 1
-        saved = []
         branch = None                                     # output of the previous MLP, not yet added to the stream
         for Lw in P["layers"]:
             # each residual add is fused into the norm that follows it (one pass instead of two over [T, D])
@@ -202,19 +234,47 @@ class TrainStep:
                 del p
                 self.launches += 1
             n2, x_mid = ops.add_rmsnorm_fwd(x, self._mm(ctx, Lw["o"], False, True), Lw["post_norm"], cfg.eps)
-            up = self._mm(n2, Lw["up"], False, True)
-            gate = self._mm(n2, Lw["gate"], False, True)
-            h = ops.swiglu_fwd(gate, up)
+            if self.ffn_fused:
+                h, gate, up = ops.gated_ffn_fwd(n2, Lw["gate"], Lw["up"], save=saved is not None)
+            else:
+                up = self._mm(n2, Lw["up"], False, True)
+                gate = self._mm(n2, Lw["gate"], False, True)
+                h = ops.swiglu_fwd(gate, up)
             branch = self._mm(h, Lw["down"], False, True)
             self.launches += 5
-            saved.append((x, n1, q, k, v, sc, ctx, x_mid, n2, up, gate, h))
+            if saved is not None:
+                saved.append((x, n1, q, k, v, sc, ctx, x_mid, n2, up, gate, h))
             x = x_mid
         nf, x = ops.add_rmsnorm_fwd(x, branch, P["head_norm"], cfg.eps)
         del branch
         logits = self._mm(nf, P["lm_head"], False, True)
-        loss, _, dlogits, _ = ops.softmax_nll_fwd_bwd(logits, targets, w_scalar=1.0 / self.loss_tokens, want_rows=False,
-                                                       status=self.status)
-        self.launches += 3
+        self.launches += 1
+        return nf, x, logits
+
+    def _loss(self, logits, targets, teacher):
+        """(loss f32[1], dlogits): the mean cross-entropy, the distillation loss, or their weighted sum."""
+        hard = 1.0 if teacher is None else 1.0 - teacher.weight
+        loss = dlogits = None
+        if hard != 0.0:
+            loss, _, dlogits, _ = ops.softmax_nll_fwd_bwd(logits, targets, w_scalar=hard / self.loss_tokens, want_rows=False,
+                                                           status=self.status)
+            self.launches += 2
+        if teacher is not None:
+            soft, _, dlogits, _ = ops.distill_topk_fwd_bwd(logits, teacher.values, teacher.indices, teacher.lse, teacher.temperature,
+                                                            w_scalar=teacher.weight / self.loss_tokens, want_rows=False,
+                                                            dlogits=dlogits, beta=int(dlogits is not None), status=self.status)
+            loss = soft if loss is None else ops.add(loss, soft)
+            self.launches += 2
+        return loss, dlogits
+
+    def forward_backward(self, tokens, targets, grads, on_layer_done=None, teacher: Teacher | None = None):
+        cfg, P, B, T = self.cfg, self.P, self.B, self.T
+        S, H, hd, D = cfg.seq, cfg.heads, cfg.head_dim, cfg.d_model
+        alpha = 1.0 / math.sqrt(hd)
+        mask = (H, S, 0, True)
+        saved = []
+        nf, x, logits = self._forward(tokens, saved)
+        loss, dlogits = self._loss(logits, targets, teacher)
         del logits
         # ---------------------------------------------------------------- backward
         self._mm(dlogits, nf, True, False, c=grads["lm_head"])
@@ -230,13 +290,19 @@ class TrainStep:
             # MLP branch: x_out = x_mid + h Wdown^T
             self._mm(dx, h, True, False, c=G["down"])
             dh = self._mm(dx, Lw["down"], False, False)
-            dgate, dup = ops.swiglu_bwd(gate, up, dh)
-            del dh, h
-            self._mm(dup, n2, True, False, c=G["up"])
-            self._mm(dgate, n2, True, False, c=G["gate"])
-            dn2 = self._mm(dup, Lw["up"], False, False)
-            self._mm(dgate, Lw["gate"], False, False, c=dn2, beta=1.0)
-            del dgate, dup, up, gate
+            if self.ffn_fused:
+                dn2, _, _ = ops.gated_ffn_bwd(dh, n2, Lw["gate"], Lw["up"], gate, up, dw_gate=G["gate"], dw_up=G["up"],
+                                              workspace=self.ffn_ws)
+                self.launches += 1
+                del dh, h, up, gate
+            else:
+                dgate, dup = ops.swiglu_bwd(gate, up, dh)
+                del dh, h
+                self._mm(dup, n2, True, False, c=G["up"])
+                self._mm(dgate, n2, True, False, c=G["gate"])
+                dn2 = self._mm(dup, Lw["up"], False, False)
+                self._mm(dgate, Lw["gate"], False, False, c=dn2, beta=1.0)
+                del dgate, dup, up, gate
             ops.rmsnorm_bwd(x_mid, Lw["post_norm"], dn2, cfg.eps, dx=dx, dgamma=G["post_norm"], beta_dx=1,
                             workspace=self.norm_ws)                                  # dx += adjoint through the norm
             del dn2
