@@ -765,9 +765,13 @@ static int launch_distill(uint64_t dl, uint64_t l, const DistillParams& p, cudaS
   while (C < kDistillMaxC && (nvec + C - 1) / C > g_distill_part) C *= 2;
   const int per = (nvec + C - 1) / C;
   const unsigned slot = ((unsigned)(per + 1) * 16 + 127) / 128 * 128;
-  if (per <= 8 * 32 * 4) return launch_distill_as<T, 8, 2, 4>(dl, l, p, C, slot, st);
+  // Warps and vectors a thread, by a row's (or part's) length: few warps that hold much, as long as two or three CTAs share an SM or
+  // one has the registers to itself.  Measured, us, k 64: 8192 x 32000 f16 with 12 x 11: 204, 16 x 8 (spills): 221, 9 x 15: 226,
+  // 8 x 16: 266, 24 x 6: 288; 8192 x 16000 with 8 x 8 on two CTAs: 133, 6 x 11: 179; 16384 x 8000 with 4 x 8 on three CTAs: 149,
+  // 8 x 4: 177.
+  if (per <= 4 * 32 * 8) return launch_distill_as<T, 4, 2, 8>(dl, l, p, C, slot, st);
   if (per <= 8 * 32 * 8) return launch_distill_as<T, 8, 2, 8>(dl, l, p, C, slot, st);
-  if (per <= 16 * 32 * 8) return launch_distill_as<T, 16, 3, 8>(dl, l, p, C, slot, st);
+  if (per <= 12 * 32 * 11) return launch_distill_as<T, 12, 3, 11>(dl, l, p, C, slot, st);
   return launch_distill_as<T, 16, 1, 0>(dl, l, p, C, slot, st);
 }
 

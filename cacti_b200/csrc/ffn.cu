@@ -277,6 +277,55 @@ ffn_fwd_kernel(const __grid_constant__ FfnMaps maps, T* __restrict__ H, T* __res
   ffn_fwd_body<T, false, SAVE>(maps, H, G, U, p);
 }
 
+static bool ffn_rows_aligned(uint64_t ptr, int64_t cols) { return ((ptr | (uint64_t)(cols * 2)) & 15) == 0; }
+
+// ---- forward, one token -------------------------------------------------------------------------------------------------
+// Bound by reading the weights once.  A warp takes an output column at a time: its gate row and its up row in 16-byte vectors,
+// eight loads ahead, against the token in shared memory (f32, so that it is converted once); sums in f32, joined over the lanes in a
+// fixed order.  3200 x 8640 f16: 18.7 us = 5.9 TB/s, 0.91 of the measured copy rate; the tensor-core kernel takes 22.1 us.  For two
+// tokens it is the other way round (22.7 against 22.1 us): the multiply-adds no longer hide.
+constexpr int kFfnVecElems = 24576;                            // the token has to fit
+template <typename T>
+__global__ void __launch_bounds__(512, 2)
+ffn_fwd_vec_kernel(T* __restrict__ H, T* __restrict__ G, T* __restrict__ U, const T* __restrict__ X, const T* __restrict__ Wg,
+                   const T* __restrict__ Wu, int D, int F) {
+  extern __shared__ float sx[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nvec = D / 8;
+  for (int i = threadIdx.x; i < D; i += 512) sx[i] = Elem<T>::to_f32(X[i]);
+  __syncthreads();
+  for (int f = blockIdx.x * 16 + warp; f < F; f += gridDim.x * 16) {
+    const uint4* wg = reinterpret_cast<const uint4*>(Wg + (long long)f * D);
+    const uint4* wu = reinterpret_cast<const uint4*>(Wu + (long long)f * D);
+    float g = 0.f, u = 0.f;
+    auto take = [&](const uint4& a, const uint4& b, int v) {
+      float ga[8], ub[8];
+      unpack<T>(a, ga);
+      unpack<T>(b, ub);
+      const float4 x0 = *reinterpret_cast<const float4*>(sx + v * 8), x1 = *reinterpret_cast<const float4*>(sx + v * 8 + 4);
+      const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) { g = fmaf(ga[e], x[e], g); u = fmaf(ub[e], x[e], u); }
+    };
+    int v = lane;
+#pragma unroll 1
+    for (; v + 96 < nvec; v += 128) {
+      uint4 a[4], b[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { a[i] = ld_stream(wg + v + 32 * i); b[i] = ld_stream(wu + v + 32 * i); }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) take(a[i], b[i], v + 32 * i);
+    }
+#pragma unroll 1
+    for (; v < nvec; v += 32) take(ld_stream(wg + v), ld_stream(wu + v), v);
+    g = warp_reduce<SumOp>(g);
+    u = warp_reduce<SumOp>(u);
+    if (lane == 0) {
+      H[f] = Elem<T>::from_f32(g * sigmoid_f32(g) * u);
+      if (G) { G[f] = Elem<T>::from_f32(g); U[f] = Elem<T>::from_f32(u); }
+    }
+  }
+}
+
 // Up to three packed matrices [rows][cols] to rows of cols_pad (a multiple of 64) with zeros behind the data, for operands that TMA
 // cannot address.  One 16-byte vector a thread: five aligned 4-byte loads, shifted where the row starts at an odd element.
 struct FfnPack { const unsigned char* src[3]; uint4* dst[3]; unsigned first[4]; unsigned rows[3]; };   // first: vector counts, running
@@ -333,7 +382,6 @@ static bool ffn_sizes_ok(int64_t tokens, int64_t D, int64_t F) {
   return D > 0 && F > 0 && tokens <= kMax && D <= kMax && F <= kMax && tokens * (F + 64) < kElems && tokens * D < kElems && F * D < kElems;
 }
 
-static bool ffn_rows_aligned(uint64_t ptr, int64_t cols) { return ((ptr | (uint64_t)(cols * 2)) & 15) == 0; }
 
 static uint32_t ffn_idesc(bool bf16, int a_mn, int b_mn, int n, int m) {
   return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
@@ -344,6 +392,16 @@ template <typename T>
 static int ffn_fwd_run(uint64_t h, uint64_t gate, uint64_t up, uint64_t x, uint64_t wg, uint64_t wu, int64_t tokens, int64_t D,
                        int64_t F, uint64_t ws, size_t ws_bytes, cudaStream_t st) {
   const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+  if (tokens == 1 && D <= kFfnVecElems && ffn_rows_aligned(wg, D) && ffn_rows_aligned(wu, D)) {
+    auto kern = ffn_fwd_vec_kernel<T>;
+    static bool attr_set[kMaxDevices] = {};
+    ensure_dynamic_smem(kern, kFfnVecElems * sizeof(float), attr_set);
+    const int64_t blocks = (F + 15) / 16;
+    kern<<<(unsigned)(blocks < 2 * kNumSMs ? blocks : 2 * kNumSMs), 512, (size_t)D * sizeof(float), st>>>(
+        reinterpret_cast<T*>(h), reinterpret_cast<T*>(gate), reinterpret_cast<T*>(up), reinterpret_cast<const T*>(x),
+        reinterpret_cast<const T*>(wg), reinterpret_cast<const T*>(wu), (int)D, (int)F);
+    return check_launch();
+  }
   Operand op[3];
   int rc = ffn_operands(op, {x, wg, wu}, {tokens, F, F}, D, ws, ws_bytes, 0, st);
   if (rc) return rc;
