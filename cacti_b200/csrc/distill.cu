@@ -70,24 +70,25 @@ constexpr int kDistillSeen = 512;                              // words of a lis
 struct DistillRef { float sub, off; };
 struct DistillRow {              // from the list warp to the main warps
   DistillRef ref;                // from the listed logits and a sample of the others; off = NaN: none to be had
-  float z_top;                   // sum of the listed exponentials (of this CTA's vectors)
-  float g_mass, g_r;             // w c P and w c r
   int skip;                      // weight 0
+  double z_top;                  // sum of the listed exponentials (of this CTA's vectors)
+  double g_mass, g_r;            // w c P and w c r
+  double px, pown;               // sum of p log2 e(x) and of p over this CTA's listed positions
 };
-struct DistillOwn { double px, pown; };                        // sum of p log2 e(x) and of p over this CTA's listed positions
 // A sum of exponentials under its reference.  Listed and unlisted positions keep references of their own until the end: where
-// the list holds nearly everything, the rest is still known.
-struct alignas(16) DistillSum { DistillRef ref; float z, pad; };
-struct DistillFin { DistillRef ref; float z_all, z_rest; double shift_rest, px; };       // back to the list warp
+// the list holds nearly everything, the rest is still known.  f64 from a warp's sum on, and the listed exponentials are exact to 1e-10:
+// near the teacher both the loss and the gradient are small differences, in which the errors of single exponentials average out or
+// are multiplied by a difference, but an error of the whole sum is not.
+struct alignas(16) DistillSum { DistillRef ref; double z; };
+struct DistillFin { DistillRef ref; double z_all, z_rest, shift_rest, px; };             // back to the list warp
 struct alignas(16) DistillRec { DistillSum rest, top; double px, pown; };  // a CTA's part of a row, to the cluster
 
 template <int MW, int R> struct alignas(16) DistillSmem {
   uint64_t full[R], marked[R], stored[R];
   uint64_t rec_bar[2];
   DistillRec rec[2][kDistillMaxC];
-  float red[2][MW];
+  double red[2][MW];
   DistillRow row[R];
-  DistillOwn lst[R];
   DistillFin fin[R];
   alignas(16) unsigned seen[R][kDistillSeen];
 };
@@ -129,31 +130,36 @@ __device__ __forceinline__ DistillRef distill_ref(float m, float c) {
 __device__ __forceinline__ double distill_shift64(const DistillRef& a, const DistillRef& b, float c) {
   return ((double)b.sub - (double)a.sub) * (double)c + ((double)a.off - (double)b.off);
 }
-__device__ __forceinline__ float distill_shift(const DistillRef& a, const DistillRef& b, float c) {
-  return a.sub == b.sub ? a.off - b.off : (float)distill_shift64(a, b, c);       // whole numbers: the difference is exact
+// 2^s, exact for whole numbers
+__device__ __forceinline__ double distill_pow2(double s) {
+  return s == rint(s) && fabs(s) < 1000. ? __hiloint2double(((int)s + 1023) << 20, 0) : exp2(s);
 }
-
 // a + b under the larger reference
 __device__ __forceinline__ DistillSum distill_add(const DistillSum& a, const DistillSum& b, float c) {
-  if (a.z == 0.f) return b;
-  if (b.z == 0.f) return a;
-  const float s = distill_shift(a.ref, b.ref, c);
-  if (s > 0.f) return DistillSum{b.ref, fmaf(a.z, exp2f_approx(-s), b.z), 0.f};
-  return DistillSum{a.ref, fmaf(b.z, exp2f_approx(s), a.z), 0.f};
+  if (a.z == 0.) return b;
+  if (b.z == 0.) return a;
+  const double s = distill_shift64(a.ref, b.ref, c);
+  if (s > 0.) return DistillSum{b.ref, a.z * distill_pow2(-s) + b.z};
+  return DistillSum{a.ref, b.z * distill_pow2(s) + a.z};
 }
+
 // CTA-wide sum or maximum over the main warps (barrier 1); `any` ORs a flag on the way.
-template <typename Op, int MW> __device__ __forceinline__ float distill_combine(float v, float (&red)[MW], int warp, int lane, bool& any) {
-  v = warp_reduce<Op>(v);
+// CTA-wide sum (f64) or maximum over the main warps, on barrier 1; `any` ORs a flag on the way.
+struct SumOp64 { static __device__ __forceinline__ double f(double a, double b) { return a + b; } };
+struct MaxOp64 { static __device__ __forceinline__ double f(double a, double b) { return fmax(a, b); } };
+template <typename Op, int MW> __device__ __forceinline__ double distill_combine(double v, double (&red)[MW], int warp, int lane, bool& any) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = Op::f(v, __shfl_xor_sync(0xffffffffu, v, o));
   if (lane == 0) red[warp] = v;
   unsigned r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %2, 0;\n\tbar.red.or.pred p, 1, %1, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(r) : "n"(MW * 32), "r"((unsigned)any) : "memory");
   any = r != 0;
-  float s = red[0];
+  double s[2] = {red[0], red[1]};
 #pragma unroll
-  for (int i = 1; i < MW; ++i) s = Op::f(s, red[i]);
-  return s;
+  for (int i = 2; i < MW; ++i) s[i & 1] = Op::f(s[i & 1], red[i]);
+  return Op::f(s[0], s[1]);
 }
 
 template <typename T> __device__ __forceinline__ void distill_put(T* o, float v, int beta) {
@@ -369,6 +375,7 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
       const int v0 = rv.nvec * rank / C, n = rv.nvec * (rank + 1) / C - v0;
       const int j0 = v0 * VEC - rv.head, j1 = j0 + n * VEC;                  // row elements of this CTA: [j0, j1)
       const int ilo = j0 < 0 ? 1 : 0, ihi = j1 > V ? n - 1 : n;              // vectors [ilo, ihi) lie wholly inside the row
+      DistillRef ref{0.f, 0.f};                                 // of the listed exponentials
       if (!skip) {
         // ---- the listed logits out of the staged row ----
         if (!mbar_wait_bounded_warp(sm.full + s, full_ph, kDevErrStageTimeout)) break;
@@ -401,35 +408,30 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
           for (int e = 0; e < VEC; ++e) mt = fmaxf(mt, x[e]);
         }
         mt = warp_reduce<MaxOp>(mt);
-        DistillRef ref = distill_ref(mt, c);
-        if (isinf(mt)) ref = DistillRef{0.f, 0.f};
-        float zt = 0.f;
-        double px = 0., pown = 0.;
+        ref = isinf(mt) ? DistillRef{0.f, 0.f} : distill_ref(mt, c);
+        double zt = 0., px = 0., pown = 0.;
         for (int k = lane; k < KP; k += 32) {
           const float x = li.x[k];
           const int id = li.idx[k];
-          zt += distill_exp(x, ref, c);
+          const double arg = ((double)x - (double)ref.sub) * (double)c + (double)ref.off, ek = exp_list(arg * 0.6931471805599453);
+          zt += ek;
+          li.x[k] = (float)ek;                                  // from here on the exponential
           const double pk = id >= j0 && id < j1 && id >= 0 ? li.p[k] : 0.;
-          if (pk != 0.) {
-            pown += pk;
-            px += pk * (((double)x - (double)ref.sub) * (double)c + (double)ref.off);
-          }
+          if (pk != 0.) { pown += pk; px += pk * arg; }
         }
-        zt = warp_reduce<SumOp>(zt);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
+          zt += __shfl_xor_sync(0xffffffffu, zt, o);
           px += __shfl_xor_sync(0xffffffffu, px, o);
           pown += __shfl_xor_sync(0xffffffffu, pown, o);
         }
         if (lane == 0) {
           const double wc = (double)h.w * p.inv_temp;
           // without a usable sample the main warps look for the maximum themselves
-          if (isinf(mt)) ref.off = __int_as_float(0x7fc00000);
-          sm.row[s] = DistillRow{ref, zt, (float)(wc * (h.psum + h.r)), (float)(wc * h.r), 0};
-          sm.lst[s] = DistillOwn{px, pown};
+          sm.row[s] = DistillRow{DistillRef{ref.sub, isinf(mt) ? __int_as_float(0x7fc00000) : ref.off}, 0, zt, wc * (h.psum + h.r), wc * h.r, px, pown};
         }
       } else if (lane == 0) {
-        sm.row[s] = DistillRow{DistillRef{0.f, 0.f}, 0.f, 0.f, 0.f, 1};
+        sm.row[s] = DistillRow{DistillRef{0.f, 0.f}, 1, 0., 0., 0., 0., 0.};
       }
       __syncwarp();
       if (lane == 0) distill_arrive(sm.marked + s);
@@ -451,13 +453,13 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
       if (BWD) {
         T* dpart = dL + (int64_t)row * V + j0;
         const double wc = (double)h.w * p.inv_temp;
-        const float ga = mass != 0. ? (float)(wc * mass / (double)f.z_all) : 0.f;
+        const double ga = mass != 0. ? wc * mass / f.z_all * distill_pow2(distill_shift64(f.ref, ref, c)) : 0.;
         for (int k = lane; k < KP; k += 32) {
           const int at = li.idx[k] - j0;
           if (li.idx[k] >= 0 && at >= 0 && at < j1 - j0) {
             // (in Accumulate mode the old value is there already, unless it is added when the element is copied out)
             const int i = at / VEC;
-            distill_put<T>(sx + at, distill_exp(li.x[k], f.ref, c) * ga - (float)(wc * li.p[k]), beta && same && i >= ilo && i < ihi);
+            distill_put<T>(sx + at, (float)(ga * (double)li.x[k] - wc * li.p[k]), beta && same && i >= ilo && i < ihi);
           }
         }
         __syncwarp();
@@ -484,7 +486,7 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
       }
       if (row % C == rank && p.loss_rows) {                     // the CTAs of a cluster take turns
         // the three logarithms side by side
-        const double lg = log_list(lane == 0 ? (double)f.z_all : lane == 1 ? h.r : (double)f.z_rest);
+        const double lg = log_list(lane == 0 ? f.z_all : lane == 1 ? h.r : f.z_rest);
         const double la = __shfl_sync(0xffffffffu, lg, 0), lr = __shfl_sync(0xffffffffu, lg, 1), lz = __shfl_sync(0xffffffffu, lg, 2);
         if (lane == 0) {
           double loss = mass != 0. ? h.ent - 0.6931471805599453 * f.px + h.psum * la : 0.;
@@ -510,7 +512,7 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
     for (int row = row0; row < rows; row += stride) {
       // a wait that ran out is agreed on at the CTA's barrier below; until then the warp goes on with what is there
       bool gave_up = !mbar_wait_bounded_warp(sm.marked + s, ph, kDevErrStageTimeout);
-      const DistillRow info = sm.row[s];
+      const struct { DistillRef ref; int skip; } info{sm.row[s].ref, sm.row[s].skip};
       const RowVecs<T> rv(L + (int64_t)row * V, V);
       const int v0 = rv.nvec * rank / C, n = rv.nvec * (rank + 1) / C - v0;
       const int j0 = v0 * VEC - rv.head;                        // row element of this part's first vector
@@ -535,7 +537,7 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
       constexpr bool HOLD = NVH > 0;
       constexpr int NV = HOLD ? NVH : 1;
       float2 a[NV][VEC / 2];
-      DistillSum rest{info.ref, 0.f, 0.f};
+      DistillSum rest{info.ref, 0.};
       const bool sampled = info.ref.off == info.ref.off;
       bool held = HOLD && sampled && info.ref.sub == 0.f;
       if (held) {
@@ -557,11 +559,11 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
           }
         }
         zq[0] = add2(zq[0], zq[1]);
-        rest.z = distill_combine<SumOp, MW>(zq[0].x + zq[0].y, sm.red[par], warp, lane, gave_up);
+        rest.z = distill_combine<SumOp64, MW>((double)zq[0].x + (double)zq[0].y, sm.red[par], warp, lane, gave_up);
         par ^= 1u;
         if (gave_up) break;
         // a logit far above the reference, all of them far below, an infinity, NaN: the CTA starts over with the true maximum
-        held = rest.z > 8.6736174e-19f && rest.z < 1.1529215e18f;           // 2^-60, 2^60
+        held = rest.z > 8.6736174e-19 && rest.z < 1.1529215e18;             // 2^-60, 2^60
       }
       if (!held) {
         float m = -INFINITY, z = 0.f;
@@ -571,7 +573,7 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
 #pragma unroll
           for (int e = 0; e < VEC; ++e) m = fmaxf(m, x[e]);
         }
-        m = distill_combine<MaxOp, MW>(m, sm.red[par], warp, lane, gave_up);
+        m = (float)distill_combine<MaxOp64, MW>((double)m, sm.red[par], warp, lane, gave_up);
         par ^= 1u;
         if (gave_up) break;
         rest.ref = m == -INFINITY ? DistillRef{0.f, 0.f} : distill_ref(m, c);
@@ -581,13 +583,13 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
 #pragma unroll
           for (int e = 0; e < VEC; ++e) z += distill_exp(x[e], rest.ref, c);
         }
-        rest.z = distill_combine<SumOp, MW>(z, sm.red[par], warp, lane, gave_up);
+        rest.z = distill_combine<SumOp64, MW>((double)z, sm.red[par], warp, lane, gave_up);
         par ^= 1u;
         if (gave_up) break;
       }
       const DistillRef own = rest.ref;
-      const bool empty = rest.z == 0.f;                         // nothing but -inf in this part: its reference means nothing
-      DistillSum top{sampled ? info.ref : DistillRef{0.f, 0.f}, info.z_top, 0.f};
+      const bool empty = rest.z == 0.;                          // nothing but -inf in this part: its reference means nothing
+      DistillSum top{sampled ? info.ref : DistillRef{0.f, 0.f}, sm.row[s].z_top};
       if (C > 1) {
         // every CTA hands its part to all of the cluster; the parts are combined in rank order everywhere
         if (warp == 0) {
@@ -596,37 +598,37 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
             uint32_t dst, bar;
             asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(dst) : "r"(smem_u32(&sm.rec[rpar][rank])), "r"(lane));
             asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(smem_u32(&sm.rec_bar[rpar])), "r"(lane));
-            asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];"
-                         ::"r"(dst), "f"(rest.ref.sub), "f"(rest.ref.off), "f"(rest.z), "f"(0.f), "r"(bar) : "memory");
-            asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];"
-                         ::"r"(dst + 16u), "f"(top.ref.sub), "f"(top.ref.off), "f"(top.z), "f"(0.f), "r"(bar) : "memory");
-            asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f64 [%0], {%1, %2}, [%3];"
-                         ::"r"(dst + 32u), "d"(sm.lst[s].px), "d"(sm.lst[s].pown), "r"(bar) : "memory");
+            auto send = [&](uint32_t at, double lo, double hi) {
+              asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f64 [%0], {%1, %2}, [%3];"
+                           ::"r"(dst + at), "d"(lo), "d"(hi), "r"(bar) : "memory");
+            };
+            auto refs = [](const DistillRef& r) { return __hiloint2double(__float_as_int(r.off), __float_as_int(r.sub)); };
+            send(0u, refs(rest.ref), rest.z);
+            send(16u, refs(top.ref), top.z);
+            send(32u, sm.row[s].px, sm.row[s].pown);
           }
         }
         gave_up = !__all_sync(0xffffffffu, distill_wait_cluster(sm.rec_bar + rpar, rph[rpar]));
         rph[rpar] ^= 1u;
-        const DistillSum nothing{DistillRef{0.f, 0.f}, 0.f, 0.f};
+        const DistillSum nothing{DistillRef{0.f, 0.f}, 0.};
         const DistillSum ro = lane < C ? sm.rec[rpar][lane].rest : nothing, to = lane < C ? sm.rec[rpar][lane].top : nothing;
         if (__all_sync(0xffffffffu, ro.ref.sub == 0.f && to.ref.sub == 0.f)) {
           // the largest reference has the smallest offset; sums over the lanes in a fixed order
-          float ra = ro.z != 0.f ? ro.ref.off : INFINITY, ta = to.z != 0.f ? to.ref.off : INFINITY;
+          float ra = ro.z != 0. ? ro.ref.off : INFINITY, ta = to.z != 0. ? to.ref.off : INFINITY;
 #pragma unroll
           for (int o = kDistillMaxC / 2; o > 0; o >>= 1) {
             ra = fminf(ra, __shfl_xor_sync(0xffffffffu, ra, o));
             ta = fminf(ta, __shfl_xor_sync(0xffffffffu, ta, o));
           }
-          float rz = ro.z != 0.f ? ro.z * exp2f_approx(ra - ro.ref.off) : 0.f, tz = to.z != 0.f ? to.z * exp2f_approx(ta - to.ref.off) : 0.f;
+          double rz = ro.z != 0. ? ro.z * distill_pow2((double)(ra - ro.ref.off)) : 0., tz = to.z != 0. ? to.z * distill_pow2((double)(ta - to.ref.off)) : 0.;
 #pragma unroll
           for (int o = kDistillMaxC / 2; o > 0; o >>= 1) {
             rz += __shfl_xor_sync(0xffffffffu, rz, o);
             tz += __shfl_xor_sync(0xffffffffu, tz, o);
           }
-          rest = DistillSum{DistillRef{0.f, isinf(ra) ? 0.f : ra}, rz, 0.f};
-          top = DistillSum{DistillRef{0.f, isinf(ta) ? 0.f : ta}, tz, 0.f};
           // (the lanes beyond the cluster's CTAs have followed lanes of their own)
-          rest.ref.off = __shfl_sync(0xffffffffu, rest.ref.off, 0); rest.z = __shfl_sync(0xffffffffu, rest.z, 0);
-          top.ref.off = __shfl_sync(0xffffffffu, top.ref.off, 0); top.z = __shfl_sync(0xffffffffu, top.z, 0);
+          rest = DistillSum{DistillRef{0.f, __shfl_sync(0xffffffffu, isinf(ra) ? 0.f : ra, 0)}, __shfl_sync(0xffffffffu, rz, 0)};
+          top = DistillSum{DistillRef{0.f, __shfl_sync(0xffffffffu, isinf(ta) ? 0.f : ta, 0)}, __shfl_sync(0xffffffffu, tz, 0)};
         } else {
           rest = sm.rec[rpar][0].rest;
           top = sm.rec[rpar][0].top;
@@ -637,32 +639,30 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
         }
       }
       const bool one = C == 1 && held;                          // one reference for everything
-      const DistillSum all = one ? DistillSum{own, rest.z + top.z, 0.f} : distill_add(rest, top, c);
+      const DistillSum all = one ? DistillSum{own, rest.z + top.z} : distill_add(rest, top, c);
       if (t == 0) {
         // sum p log2 e(x) under the row's reference
         double px = 0.;
-        if (one) px = sm.lst[s].px;
-        else if (C == 1) px = sm.lst[s].pown != 0. ? sm.lst[s].px + sm.lst[s].pown * distill_shift64(all.ref, top.ref, c) : 0.;
+        if (one) px = sm.row[s].px;
+        else if (C == 1) px = sm.row[s].pown != 0. ? sm.row[s].px + sm.row[s].pown * distill_shift64(all.ref, top.ref, c) : 0.;
         else
           for (int q = 0; q < C; ++q) {
             const DistillRec& o = sm.rec[rpar][q];
             if (o.pown != 0.) px += o.px + o.pown * distill_shift64(all.ref, o.top.ref, c);
           }
-        sm.fin[s] = DistillFin{all.ref, all.z, rest.z, one || rest.z == 0.f ? 0. : distill_shift64(all.ref, rest.ref, c), px};
+        sm.fin[s] = DistillFin{all.ref, all.z, rest.z, one || rest.z == 0. ? 0. : distill_shift64(all.ref, rest.ref, c), px};
       }
       if (C > 1) rpar ^= 1u;
       if (BWD) {
         // (P / E - r / E_rest) e, e formed against this CTA's reference
-        float g = 0.f;
-        if (info.g_mass != 0.f) {
-          g = info.g_mass / all.z;
-          float gr = info.g_r != 0.f && rest.z > 0.f ? info.g_r / rest.z : 0.f;
-          if (!one && !empty) {
-            g *= exp2f_approx(distill_shift(all.ref, own, c));
-            if (gr != 0.f) gr *= exp2f_approx(distill_shift(rest.ref, own, c));
-          }
-          g -= gr;
+        const double num = lane == 0 ? sm.row[s].g_mass : sm.row[s].g_r, den = lane == 0 ? all.z : rest.z;
+        double ga = num != 0. && (lane == 0 || den > 0.) ? num / den : 0., gr = __shfl_sync(0xffffffffu, ga, 1);      // one division
+        ga = __shfl_sync(0xffffffffu, ga, 0);
+        if (!one && !empty) {
+          if (ga != 0.) ga *= distill_pow2(distill_shift64(all.ref, own, c));
+          if (gr != 0.) gr *= distill_pow2(distill_shift64(rest.ref, own, c));
         }
+        const float g = (float)(ga - gr);
         if (held) {
           const float2 g2 = make_float2(g, g);
 #pragma unroll

@@ -284,6 +284,26 @@ def test_masked_and_extreme_rows(cuda, dtype, tail, vocab):
             assert per_row[i] == ref[0][i]
 
 
+@pytest.mark.parametrize("tau,vocab,k,noise", [(1.5, 50001, 17, 0.05), (4.0, 32000, 64, 0.05), (1.0, 8000, 128, 0.2), (2.0, 131072, 100, 0.02)])
+def test_a_student_near_its_teacher(cuda, tau, vocab, k, noise):
+    """Loss and gradient are then small differences of large terms.  What does not cancel: the error of the sum over the unlisted
+    positions, times the difference of its share from the teacher's; the sum is made of f32 sums of at most 128 terms whose roundings
+    (2^-24, growing with the square root of the number of terms) average over more than 100 threads: below 2^-25; and
+    the temperature's rounding to f32, 2^-24 of the difference of the mean logits.  Single exponentials are good to 2^-22, the listed
+    ones to 2^-24."""
+    z = _logits(64, vocab, torch.float32, 11, std=1.5)
+    g = torch.Generator(device="cuda").manual_seed(12)
+    x = z + noise * torch.randn(64, vocab, device="cuda", generator=g)
+    tv, ti, _ = ops.logits_topk(z, k, temperature=tau)
+    lse = torch.logsumexp(z.double() / tau, 1).float()
+    w = torch.ones(64, device="cuda")
+    loss, rows, grad, _ = ops.distill_topk_fwd_bwd(x, tv, ti, lse, tau, w)
+    rl, rg, mag, A, P, r = _ref(x, tv, ti, lse, tau, w)
+    assert (rl < 0.05).all()
+    assert ((rows.double() - rl).abs() <= 2.0 ** -22 * rl + noise * 2.0 ** -24 * 8).all(), ((rows.double() - rl).abs() / rl).max()
+    assert ((grad.double() - rg).abs() <= 2.0 ** -21 * rg.abs() + 2.0 ** -23 * mag * noise * 8 + 2.0 ** -24 * mag).all()
+
+
 def test_gradient_against_differences(cuda):
     """Central differences of the loss in 64 bits of torch autograd-free form: the formula's gradient is the loss's."""
     torch.manual_seed(0)
