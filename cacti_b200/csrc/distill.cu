@@ -144,22 +144,37 @@ __device__ __forceinline__ DistillSum distill_add(const DistillSum& a, const Dis
 }
 
 // CTA-wide sum or maximum over the main warps (barrier 1); `any` ORs a flag on the way.
-// CTA-wide sum (f64) or maximum over the main warps, on barrier 1; `any` ORs a flag on the way.
-struct SumOp64 { static __device__ __forceinline__ double f(double a, double b) { return a + b; } };
-struct MaxOp64 { static __device__ __forceinline__ double f(double a, double b) { return fmax(a, b); } };
-template <typename Op, int MW> __device__ __forceinline__ double distill_combine(double v, double (&red)[MW], int warp, int lane, bool& any) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = Op::f(v, __shfl_xor_sync(0xffffffffu, v, o));
-  if (lane == 0) red[warp] = v;
+// CTA-wide sum or maximum over the main warps, on barrier 1; `any` ORs a flag on the way.  A sum is f32 inside a warp and f64 from there on:
+// the roundings of the warps' sums average out (below 2^-25 of the sum), those of a last f32 addition would not.
+template <int MW> __device__ __forceinline__ bool distill_meet(bool any) {
   unsigned r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %2, 0;\n\tbar.red.or.pred p, 1, %1, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(r) : "n"(MW * 32), "r"((unsigned)any) : "memory");
-  any = r != 0;
+  return r != 0;
+}
+template <int MW> __device__ __forceinline__ double distill_sum(float z, double (&red)[MW], int warp, int lane, bool& any) {
+  z = warp_reduce<SumOp>(z);
+  if (lane == 0) red[warp] = (double)z;
+  any = distill_meet<MW>(any);
   double s[2] = {red[0], red[1]};
 #pragma unroll
-  for (int i = 2; i < MW; ++i) s[i & 1] = Op::f(s[i & 1], red[i]);
-  return Op::f(s[0], s[1]);
+  for (int i = 2; i < MW; ++i) s[i & 1] += red[i];
+  return s[0] + s[1];
+}
+template <int MW> __device__ __forceinline__ float distill_max(float m, double (&red)[MW], int warp, int lane, bool& any) {
+  m = warp_reduce<MaxOp>(m);
+  if (lane == 0) red[warp] = (double)m;
+  any = distill_meet<MW>(any);
+#pragma unroll
+  for (int i = 0; i < MW; ++i) m = fmaxf(m, (float)red[i]);
+  return m;
+}
+// a / b to about 1e-11: the hardware's reciprocal estimate (20 bits) and one Newton step.  NaN where b is 0 or infinite.
+__device__ __forceinline__ double quotient(double a, double b) {
+  double r;
+  asm("rcp.approx.ftz.f64 %0, %1;" : "=d"(r) : "d"(b));
+  return a * fma(r, fma(-b, r, 1.), r);
 }
 
 template <typename T> __device__ __forceinline__ void distill_put(T* o, float v, int beta) {
@@ -453,7 +468,7 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
       if (BWD) {
         T* dpart = dL + (int64_t)row * V + j0;
         const double wc = (double)h.w * p.inv_temp;
-        const double ga = mass != 0. ? wc * mass / f.z_all * distill_pow2(distill_shift64(f.ref, ref, c)) : 0.;
+        const double ga = mass != 0. ? quotient(wc * mass, f.z_all) * (f.ref.off == ref.off && f.ref.sub == ref.sub ? 1. : distill_pow2(distill_shift64(f.ref, ref, c))) : 0.;
         for (int k = lane; k < KP; k += 32) {
           const int at = li.idx[k] - j0;
           if (li.idx[k] >= 0 && at >= 0 && at < j1 - j0) {
@@ -559,7 +574,7 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
           }
         }
         zq[0] = add2(zq[0], zq[1]);
-        rest.z = distill_combine<SumOp64, MW>((double)zq[0].x + (double)zq[0].y, sm.red[par], warp, lane, gave_up);
+        rest.z = distill_sum<MW>(zq[0].x + zq[0].y, sm.red[par], warp, lane, gave_up);
         par ^= 1u;
         if (gave_up) break;
         // a logit far above the reference, all of them far below, an infinity, NaN: the CTA starts over with the true maximum
@@ -573,7 +588,7 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
 #pragma unroll
           for (int e = 0; e < VEC; ++e) m = fmaxf(m, x[e]);
         }
-        m = (float)distill_combine<MaxOp64, MW>((double)m, sm.red[par], warp, lane, gave_up);
+        m = distill_max<MW>(m, sm.red[par], warp, lane, gave_up);
         par ^= 1u;
         if (gave_up) break;
         rest.ref = m == -INFINITY ? DistillRef{0.f, 0.f} : distill_ref(m, c);
@@ -583,7 +598,7 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
 #pragma unroll
           for (int e = 0; e < VEC; ++e) z += distill_exp(x[e], rest.ref, c);
         }
-        rest.z = distill_combine<SumOp64, MW>((double)z, sm.red[par], warp, lane, gave_up);
+        rest.z = distill_sum<MW>(z, sm.red[par], warp, lane, gave_up);
         par ^= 1u;
         if (gave_up) break;
       }
@@ -656,7 +671,7 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
       if (BWD) {
         // (P / E - r / E_rest) e, e formed against this CTA's reference
         const double num = lane == 0 ? sm.row[s].g_mass : sm.row[s].g_r, den = lane == 0 ? all.z : rest.z;
-        double ga = num != 0. && (lane == 0 || den > 0.) ? num / den : 0., gr = __shfl_sync(0xffffffffu, ga, 1);      // one division
+        double ga = num != 0. && (lane == 0 || den > 0.) ? quotient(num, den) : 0., gr = __shfl_sync(0xffffffffu, ga, 1);      // one division
         ga = __shfl_sync(0xffffffffu, ga, 0);
         if (!one && !empty) {
           if (ga != 0.) ga *= distill_pow2(distill_shift64(all.ref, own, c));
