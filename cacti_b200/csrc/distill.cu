@@ -143,7 +143,6 @@ __device__ __forceinline__ DistillSum distill_add(const DistillSum& a, const Dis
   return DistillSum{a.ref, b.z * distill_pow2(s) + a.z};
 }
 
-// CTA-wide sum or maximum over the main warps (barrier 1); `any` ORs a flag on the way.
 // CTA-wide sum or maximum over the main warps, on barrier 1; `any` ORs a flag on the way.  A sum is f32 inside a warp and f64 from there on:
 // the roundings of the warps' sums average out (below 2^-25 of the sum), those of a last f32 addition would not.
 template <int MW> __device__ __forceinline__ bool distill_meet(bool any) {
@@ -524,9 +523,11 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
     const int t = threadIdx.x;
     int s = 0;
     unsigned ph = 0, par = 0, rpar = 0, rph[2] = {0, 0};
+    // A wait that ran out: the warp goes on with what is there up to the CTA's next barrier, in this row or behind the last one, where
+    // all leave together.  (Held over several rows, the flag costs registers: 8192 x 32000 f16 took 240 us instead of 218.)
+    bool gave_up = false, agreed = false;
     for (int row = row0; row < rows; row += stride) {
-      // a wait that ran out is agreed on at the CTA's barrier below; until then the warp goes on with what is there
-      bool gave_up = !mbar_wait_bounded_warp(sm.marked + s, ph, kDevErrStageTimeout);
+      gave_up = !mbar_wait_bounded_warp(sm.marked + s, ph, kDevErrStageTimeout);
       const struct { DistillRef ref; int skip; } info{sm.row[s].ref, sm.row[s].skip};
       const RowVecs<T> rv(L + (int64_t)row * V, V);
       const int v0 = rv.nvec * rank / C, n = rv.nvec * (rank + 1) / C - v0;
@@ -576,7 +577,7 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
         zq[0] = add2(zq[0], zq[1]);
         rest.z = distill_sum<MW>(zq[0].x + zq[0].y, sm.red[par], warp, lane, gave_up);
         par ^= 1u;
-        if (gave_up) break;
+        if (gave_up) { agreed = true; break; }
         // a logit far above the reference, all of them far below, an infinity, NaN: the CTA starts over with the true maximum
         held = rest.z > 8.6736174e-19 && rest.z < 1.1529215e18;             // 2^-60, 2^60
       }
@@ -590,7 +591,7 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
         }
         m = distill_max<MW>(m, sm.red[par], warp, lane, gave_up);
         par ^= 1u;
-        if (gave_up) break;
+        if (gave_up) { agreed = true; break; }
         rest.ref = m == -INFINITY ? DistillRef{0.f, 0.f} : distill_ref(m, c);
         for (int i = t; i < n; i += MT) {
           float x[VEC];
@@ -600,7 +601,7 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
         }
         rest.z = distill_sum<MW>(z, sm.red[par], warp, lane, gave_up);
         par ^= 1u;
-        if (gave_up) break;
+        if (gave_up) { agreed = true; break; }
       }
       const DistillRef own = rest.ref;
       const bool empty = rest.z == 0.;                          // nothing but -inf in this part: its reference means nothing
@@ -711,6 +712,7 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
       if (++s == R) { s = 0; ph ^= 1u; }
       if (gave_up) break;
     }
+    if (!agreed) (void)distill_meet<MW>(gave_up);
   }
   __syncwarp();
   // no CTA leaves while another may still write into its records

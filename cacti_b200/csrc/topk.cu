@@ -102,10 +102,11 @@ logits_topk_kernel(T* __restrict__ values, int* __restrict__ indices, float* __r
   __shared__ float s_t;
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
   const float c = (float)(inv_temp * 1.4426950408889634);
-  // exponentials are 2^(x c + off): off is a whole number, so it changes no bit of a sum that stays in range, and what suited the row
-  // before is a good guess; a sum out of range is formed again, the same way, with an off of its own
-  float off = 0.f;
   for (int row = blockIdx.x; row < rows; row += gridDim.x) {
+    // exponentials are 2^(x c + off), off a whole number: 0, and where the sum leaves its range it is formed once more with the off
+    // that suits the row's maximum.  (The off of the row before would spare rows of large logits that second sum, but a row's last bits
+    // would then depend on its neighbours.)
+    float off = 0.f;
     const T* x = L + (int64_t)row * V;
     const RowVecs<T> rv(x, V);
     // ---- pass 1 ----

@@ -272,8 +272,10 @@ def distill_topk_fwd_bwd(logits, t_values, t_indices, t_lse=None, temperature=1.
     with _on(dev):
         loss_sum = torch.empty(1, dtype=torch.float32, device=dev) if want_sum else None
         loss_rows = torch.empty(rows, dtype=torch.float32, device=dev) if want_rows else None
-        if loss_sum is not None and (rows == 0 or vocab == 0):
-            loss_sum.zero_()
+        if rows == 0 or vocab == 0:
+            for out in (loss_sum, loss_rows):
+                if out is not None:
+                    out.zero_()
         if want_grad and dlogits is None:
             dlogits = torch.empty_like(logits)
         status = torch.zeros(1, dtype=torch.int32, device=dev) if status is None else status

@@ -322,6 +322,35 @@ def test_gradient_against_differences(cuda):
             assert ((grad[:, j].double() - num).abs() <= 1e-9 + 2.0 ** -18).all()
 
 
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("vocab", [2992, 4099, 50000, 120000])
+def test_a_row_of_the_teacher_does_not_depend_on_its_neighbours(cuda, dtype, vocab):
+    # rows of large and of small logits in turn before copies of one row, enough rows that each block takes several
+    rows = 2000 if vocab < 10000 else 1000
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    one = torch.randn(vocab, device="cuda", generator=g) * 3
+    x = one.repeat(rows, 1)
+    other = torch.rand(rows, device="cuda", generator=g) < 0.5
+    x[other] += (torch.rand(int(other.sum()), 1, device="cuda", generator=g) - 0.5) * 200
+    v, i, lse = ops.logits_topk(x.to(DT[dtype]), 20)
+    same = ~other
+    first = int(same.nonzero()[0])
+    assert torch.equal(lse[same], lse[first].expand(int(same.sum())))
+    assert torch.equal(v[same], v[first].expand(int(same.sum()), 20)) and torch.equal(i[same], i[first].expand(int(same.sum()), 20))
+    ref = torch.logsumexp(x.to(DT[dtype]).double(), 1)
+    # exponentials at up to 2^60 or re-referenced: 2^-22 (1 + 60) of the sum, one rounding of the result
+    assert ((lse.double() - ref).abs() <= 61 * 2.0 ** -22 + (vocab / 256 + 24) * 2.0 ** -24 + ref.abs() * 2.0 ** -24).all()
+
+
+def test_an_empty_vocabulary_has_zero_losses(cuda):
+    x = torch.empty(5, 0, device="cuda", dtype=torch.float16)
+    tv = torch.zeros(5, 2, device="cuda", dtype=torch.float16)
+    ti = torch.full((5, 2), -1, device="cuda", dtype=torch.int32)
+    torch.full((5,), 7.0, device="cuda")                        # what an allocation may find in its memory
+    total, loss, d, status = ops.distill_topk_fwd_bwd(x, tv, ti)
+    assert loss.tolist() == [0.0] * 5 and total.item() == 0.0 and d.shape == (5, 0) and status.item() == 0
+
+
 def test_streams_graphs_and_empty_calls(cuda):
     x, z = _logits(40, 4000, torch.bfloat16, 1), _logits(40, 4000, torch.bfloat16, 2)
     want = ops.distill_topk_fwd_bwd(x, *ops.logits_topk(z, 30), want_rows=False)
