@@ -244,7 +244,9 @@ int cacti_b200_logits_topk(cacti_b200_dptr values, cacti_b200_dptr indices, cact
  * whose used logits are all -inf) has loss 0 and gradient 0.  Any other index outside [0, vocab), and an index listed
  * twice (every slot but the first), writes CACTI_B200_ERR_INDEX_RANGE to *status; the slot is left out and the row's loss
  * is NaN.  A row of weight 0 is not read: loss 0, gradient 0 (beta 1: dlogits unchanged).
- * Statistics, listed probabilities and the loss are kept in f64 except for the f32 sums of the exponentials.
+ * The teacher's probabilities, the listed exponentials, the row's sums and the loss are kept in f64; the exponentials of unlisted
+ * positions are f32, and so are their sums up to 32 threads' (f64 from there on).  Results are the same in every
+ * run and do not depend on what the other rows hold.
  * 1 <= k <= 256, vocab <= 262144 (else CACTI_B200_ERR_SHAPE), temperature in [1e-4, 1e4].  dlogits must not overlap
  * logits. */
 size_t cacti_b200_distill_topk_workspace_bytes(int64_t rows);
@@ -368,7 +370,7 @@ int cacti_b200_gemm_strided_batched_tri(cacti_b200_dptr c, cacti_b200_dptr a, ca
  *   dx = T(dg w_gate + du w_up + beta_dx dx),  dw_gate = T(dg^T x + beta_dw dw_gate),  dw_up = T(du^T x + beta_dw dw_up)
  * (sums in f32, one rounding; the old value is added in f32 before it, as in cacti_b200_gemm).  tokens = 0 is legal: the
  * adjoint then writes zero weight gradients (beta_dw = 0).  d_model = 0 or d_ffn = 0 is CACTI_B200_ERR_SHAPE.
- * Outputs may not overlap inputs or one another.  Workspaces: 256-byte aligned; `aligned` = 1 asks for what suffices when
+ * Outputs may not overlap inputs or one another.  Workspaces: 256-byte aligned, one for each call at work at a time; `aligned` = 1 asks for what suffices when
  * d_model is a multiple of 8 and x, w_gate and w_up are 16-byte aligned (operands that are not are repacked), 0 for any. */
 size_t cacti_b200_gated_ffn_fwd_workspace_bytes(int64_t tokens, int64_t d_model, int64_t d_ffn, int aligned);
 int cacti_b200_gated_ffn_fwd(cacti_b200_dptr h, cacti_b200_dptr gate, cacti_b200_dptr up, cacti_b200_dptr x,
