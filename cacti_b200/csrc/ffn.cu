@@ -560,6 +560,8 @@ __device__ __forceinline__ void ffn_tile_rows(int M, int N, uint32_t tmem_base, 
     }
     __syncwarp();
   }
+  // the staging's next writer may be a TMA load (the old values of an accumulating tile): after these ordinary accesses
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   tc_fence_before();
   __syncwarp();
   if (lane == 0) mbar_arrive_cluster(tempty_addr);

@@ -126,6 +126,26 @@ def test_both_directions_at_larger_sizes(cuda, dtype, t, d, f):
     _check_bwd(ops.gated_ffn_bwd(dh, x, wg, wu, out[1], out[2]), dh, x, wg, wu, out[1], out[2])
 
 
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("t,d,f,dx_off", [(16, 3200, 8640, 0), (77, 1024, 2048, 0), (300, 640, 8640, 1)])
+def test_partial_sums_and_accumulating_tiles_in_one_staging(cuda, dtype, t, d, f, dx_off):
+    """Few tokens cut dx's contraction (and a dx at an odd address cannot leave by TMA): its tiles leave the staging by ordinary
+    accesses, and the same warps then load old weight gradients into it by TMA.  More items than workers, so that one warp does both.
+    Added to zeros the weight gradients are those of Apply mode, bit for bit; added to ones, one rounding of the f32 sum away."""
+    x, wg, wu, dh = _inputs(t, d, f, DT[dtype], 6)
+    _, gate, up = ops.gated_ffn_fwd(x, wg, wu, save=True)
+    want = ops.gated_ffn_bwd(dh, x, wg, wu, gate, up)
+    for _ in range(3):
+        dx, _ = _at_offset(torch.zeros_like(x), dx_off)
+        zeros = ops.gated_ffn_bwd(dh, x, wg, wu, gate, up, dx=dx, dw_gate=torch.zeros_like(wg), dw_up=torch.zeros_like(wu), beta_dw=1)
+        assert all(torch.equal(a, b) for a, b in zip(zeros, want))
+        old = (None, torch.ones_like(wg), torch.full_like(wu, -2.0))
+        dx, _ = _at_offset(torch.zeros_like(x), dx_off)
+        out = ops.gated_ffn_bwd(dh, x, wg, wu, gate, up, dx=dx, dw_gate=old[1].clone(), dw_up=old[2].clone(), beta_dw=1)
+        assert torch.equal(out[0], want[0])
+        _check_bwd(out, dh, x, wg, wu, gate, up, old, "added")
+
+
 def test_gradient_against_differences(cuda):
     """The backward's formulas are the forward's derivative: central differences of sum(dh * h) in 64 bits."""
     t, d, f, eps = 3, 16, 24, 1e-5
