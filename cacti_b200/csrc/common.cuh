@@ -4,6 +4,7 @@
 #include <cuda_fp16.h>
 #include <cuda_bf16.h>
 #include <stdint.h>
+#include <mutex>
 #include "../../include/cacti_b200.h"
 
 namespace cb {
@@ -356,22 +357,39 @@ template <typename F> inline int dispatch_dtype(int dtype, F&& f) {
 // or below g_pref threads, else nv_max vectors per thread and up to 512 threads.
 constexpr size_t kMaxDynSmem = 200 * 1024;      // of the 227 KB a CTA may use
 
+// Raise a kernel's dynamic shared memory limit to at least `smem`.  The limit belongs to the device's copy of the function,
+// whichever host thread sets it, so what was set last is kept for the whole process and never lowered: a thread whose
+// call needs less must not take away from one whose call needs more.
+struct SmemLimit { const void* k; int dev; size_t s; };
+constexpr int kMaxSmemLimits = 1024;             // kernels x devices; beyond it no call lowers a limit that is in the table
+inline void raise_dynamic_smem(const void* kern, int dev, size_t smem) {
+  static std::mutex mu;
+  static SmemLimit table[kMaxSmemLimits];
+  static int used = 0;
+  std::lock_guard<std::mutex> hold(mu);
+  int i = 0;
+  for (; i < used; ++i) if (table[i].k == kern && table[i].dev == dev) break;
+  if (i < used && table[i].s >= smem) return;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return;   // the launch reports it
+  if (i == used && used < kMaxSmemLimits) table[used++] = SmemLimit{kern, dev, 0};
+  if (i < used) table[i].s = smem;
+}
+
 // CTAs of `kern` that fit on one SM with this block size and dynamic shared memory; also raises the
 // kernel's dynamic shared memory limit when needed (never lowers it).  Cached per (kernel, config).
 template <typename K> inline int resident_ctas(K kern, int threads, size_t smem) {
   struct Key { const void* k; int dev; int t; size_t s; int n; };
-  struct Lim { const void* k; int dev; size_t s; };
   static thread_local Key cache[128];
-  static thread_local Lim lim[128];
+  static thread_local SmemLimit lim[128];        // what this thread knows to be set; limits only rise
   static thread_local int used = 0, nlim = 0;
   const void* kp = reinterpret_cast<const void*>(kern);
   const int dev = device_ordinal();
   if (smem > 48 * 1024) {
     int i = 0;
     for (; i < nlim; ++i) if (lim[i].k == kp && lim[i].dev == dev) break;
-    if (i == nlim && nlim < 128) lim[nlim++] = Lim{kp, dev, 0};
+    if (i == nlim && nlim < 128) lim[nlim++] = SmemLimit{kp, dev, 0};
     if (i >= 128 || lim[i].s < smem) {
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+      raise_dynamic_smem(kp, dev, smem);
       if (i < 128) lim[i].s = smem;
     }
   }

@@ -378,6 +378,40 @@ def test_streams_graphs_and_empty_calls(cuda):
     assert capi.lib().cacti_b200_device_error(capi.C.byref(err)) == capi.OK and err.value == 0
 
 
+def test_two_host_threads_with_rows_of_two_lengths(cuda):
+    """One kernel with two sizes of shared memory: what one thread's call asks for must not take away from the other's."""
+    import threading
+    cases = {v: (_logits(30, v, torch.float16, v), *ops.logits_topk(_logits(30, v, torch.float16, v + 1), 64)) for v in (32000, 20000)}
+    torch.cuda.synchronize()
+    got, errors = {}, []
+    turns = [threading.Semaphore(1), threading.Semaphore(0)]
+
+    def work(me, order):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for n, v in enumerate(order):
+                    turns[me].acquire()
+                    got[me, n, v] = [t.clone() for t in ops.distill_topk_fwd_bwd(*cases[v])[:3]]
+                    torch.cuda.current_stream().synchronize()
+                    turns[1 - me].release()
+        except Exception as e:                                          # (the other thread goes on without this one)
+            errors.append(e)
+            for _ in order:
+                turns[1 - me].release()
+
+    # a: the longer row; b: the shorter one, its thread's first; a: the longer row again
+    threads = [threading.Thread(target=work, args=a) for a in ((0, (32000, 32000, 20000)), (1, (20000, 32000, 20000)))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert not errors, errors
+    want = {v: ops.distill_topk_fwd_bwd(*cases[v])[:3] for v in cases}
+    assert len(got) == 6
+    for (_, _, v), out in got.items():
+        assert all(torch.equal(a, b) for a, b in zip(out, want[v]))
+
+
 def test_refusals(cuda):
     x = _logits(4, 100, torch.float16, 1)
     tv, ti, lse = ops.logits_topk(x, 10)
