@@ -382,10 +382,18 @@ static int ffn_operands(Operand (&o)[3], const uint64_t (&ptr)[3], const int64_t
   return check_launch();
 }
 
-// Sizes whose tile, k-block and vector counts fit 32-bit indices (any that fit the device's memory do).
+// Sizes whose tile, k-block and vector counts fit 32-bit indices, one operand at a time.
 static bool ffn_sizes_ok(int64_t tokens, int64_t D, int64_t F) {
   constexpr int64_t kMax = 1 << 24, kElems = 1LL << 34;
   return D > 0 && F > 0 && tokens <= kMax && D <= kMax && F <= kMax && tokens * (F + 64) < kElems && tokens * D < kElems && F * D < kElems;
+}
+// The repacking launch numbers the vectors of all the operands that it copies in 32 bits: three operands near the bound above, copies of
+// 64 GiB and more together, do not fit and are refused.
+static bool ffn_pack_ok(const uint64_t (&ptr)[3], const int64_t (&rows)[3], int64_t cols) {
+  int64_t n = 0;
+  for (int i = 0; i < 3; ++i)
+    if (!ffn_rows_aligned(ptr[i], cols)) n += rows[i] * (packed_cols(cols) / 8);
+  return n <= 0xffffffffLL - 256;                               // whole blocks of 256 threads
 }
 
 
@@ -888,6 +896,7 @@ int cacti_b200_gated_ffn_fwd(cacti_b200_dptr h, cacti_b200_dptr gate, cacti_b200
   if (tokens == 0) return CACTI_B200_OK;
   if (!h || !x || !w_gate || !w_up || !gate != !up) return CACTI_B200_ERR_INVALID_VALUE;
   if ((h | gate | up | x | w_gate | w_up) & 1) return CACTI_B200_ERR_INVALID_VALUE;
+  if (!ffn_pack_ok({x, w_gate, w_up}, {tokens, d_ffn, d_ffn}, d_model)) return CACTI_B200_ERR_SHAPE;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (dtype == CACTI_B200_R_16F)
     return ffn_fwd_run<__half>(h, gate, up, x, w_gate, w_up, tokens, d_model, d_ffn, workspace, workspace_bytes, st);
@@ -914,6 +923,7 @@ int cacti_b200_gated_ffn_bwd(cacti_b200_dptr dx, cacti_b200_dptr dw_gate, cacti_
   if (!dw_gate || !dw_up) return CACTI_B200_ERR_INVALID_VALUE;
   if (tokens > 0 && (!dx || !dh || !x || !w_gate || !w_up || !gate || !up)) return CACTI_B200_ERR_INVALID_VALUE;
   if ((dx | dw_gate | dw_up | dh | x | w_gate | w_up | gate | up) & 1) return CACTI_B200_ERR_INVALID_VALUE;
+  if (!ffn_pack_ok({x, w_gate, w_up}, {tokens, d_ffn, d_ffn}, d_model)) return CACTI_B200_ERR_SHAPE;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (tokens == 0) {                                            // an empty sum: the weight gradients are zero
     if (!beta_dw)

@@ -370,6 +370,7 @@ int cacti_b200_gemm_strided_batched_tri(cacti_b200_dptr c, cacti_b200_dptr a, ca
  *   dx = T(dg w_gate + du w_up + beta_dx dx),  dw_gate = T(dg^T x + beta_dw dw_gate),  dw_up = T(du^T x + beta_dw dw_up)
  * (sums in f32, one rounding; the old value is added in f32 before it, as in cacti_b200_gemm).  tokens = 0 is legal: the
  * adjoint then writes zero weight gradients (beta_dw = 0).  d_model = 0 or d_ffn = 0 is CACTI_B200_ERR_SHAPE.
+ * So are sizes above 2^24, operands of 2^34 elements, and operands to be repacked whose copies come to 64 GiB together.
  * Outputs may not overlap inputs or one another.  Workspaces: 256-byte aligned, one for each call at work at a time; `aligned` = 1 asks for what suffices when
  * d_model is a multiple of 8 and x, w_gate and w_up are 16-byte aligned (operands that are not are repacked), 0 for any. */
 size_t cacti_b200_gated_ffn_fwd_workspace_bytes(int64_t tokens, int64_t d_model, int64_t d_ffn, int aligned);

@@ -67,3 +67,15 @@ def test_gated_ffn_refusals():
     for t, d, f in ((1, 8, 8), (77, 1003, 277), (2048, 3200, 8640)):
         assert L.cacti_b200_gated_ffn_bwd_workspace_bytes(t, d, f, 0) >= L.cacti_b200_gated_ffn_bwd_workspace_bytes(t, d, f, 1) >= 4 * t * f
         assert L.cacti_b200_gated_ffn_fwd_workspace_bytes(t, d, f, 0) >= L.cacti_b200_gated_ffn_fwd_workspace_bytes(t, d, f, 1)
+
+
+def test_gated_ffn_refuses_copies_that_cannot_be_numbered():
+    """Operands whose repacked vectors together pass 32 bits; the counts wrapped to a small number, most rows were never copied and
+    the call answered OK.  Sizes one step below are refused for their workspace only."""
+    big, f = 1 << 62, 1 << 24
+    for d, off in ((1017, 0), (1023, 0), (1016, 2)):                    # odd sizes; aligned rows at an odd address
+        assert _fwd(t=2, d=d, f=f, x=P + off, wg=P + off, wu=P + off, ws=0x1000, wsb=big) == capi.ERR_SHAPE
+        assert _bwd(t=2, d=d, f=f, x=P + off, wg=P + off, wu=P + off, wsb=big) == capi.ERR_SHAPE
+    assert _fwd(t=2, d=1025, f=16700000, ws=0x1000, wsb=big) == _bwd(t=2, d=1025, f=16700000, wsb=big) == capi.ERR_SHAPE
+    assert _fwd(t=2, d=1017, f=f // 2, ws=0, wsb=0) == _bwd(t=2, d=1017, f=f // 2, ws=0, wsb=0) == capi.ERR_WORKSPACE
+    assert _fwd(t=2, d=1016, f=f, x=P + 2, ws=0, wsb=0) == _bwd(t=2, d=1016, f=f, x=P + 2, ws=0, wsb=0) == capi.ERR_WORKSPACE   # x alone
