@@ -378,6 +378,25 @@ def test_streams_graphs_and_empty_calls(cuda):
     assert capi.lib().cacti_b200_device_error(capi.C.byref(err)) == capi.OK and err.value == 0
 
 
+def test_more_lengths_of_rows_than_a_launch_cache_keeps(cuda):
+    """Two hundred sizes of shared memory for one kernel, and for its cluster form, then the first ones again."""
+    x, z = (_logits(1, 42000 + 16 * 200, torch.float16, s) for s in (1, 2))
+    first = {}
+    for n in list(range(200)) + [0, 1, 70, 135, 199]:
+        for base in (20000, 42000):
+            v = base + 16 * n                                           # each another number of vectors a row
+            xs, zs = x[:, :v].contiguous(), z[:, :v].contiguous()
+            k = 1 + 32 * (n % 8)
+            got = ops.distill_topk_fwd_bwd(xs, *ops.logits_topk(zs, k))
+            if v in first:
+                assert torch.equal(got[1], first[v][0]) and torch.equal(got[2], first[v][1])
+                continue
+            first[v] = got[1:3]
+            if n % 40 == 0 or n == 199:
+                tv, ti, lse = ops.logits_topk(zs, k)
+                _check(got[:3], _ref(xs, tv, ti, lse, 1.0, torch.ones(1, device="cuda")), torch.float16, v, what=f"{v}")
+
+
 def test_two_host_threads_with_rows_of_two_lengths(cuda):
     """One kernel with two sizes of shared memory: what one thread's call asks for must not take away from the other's."""
     import threading
