@@ -473,13 +473,13 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
       if (BWD) {
         T* dpart = dL + (int64_t)row * V + j0;
         const double wc = (double)h.w * p.inv_temp;
-        const double ga = mass != 0. ? quotient(wc * mass, f.z_all) * (f.ref.off == ref.off && f.ref.sub == ref.sub ? 1. : distill_pow2(distill_shift64(f.ref, ref, c))) : 0.;
+        const double ga = quotient(wc * mass, f.z_all) * (f.ref.off == ref.off && f.ref.sub == ref.sub ? 1. : distill_pow2(distill_shift64(f.ref, ref, c)));
         for (int k = lane; k < KP; k += 32) {
           const int at = li.idx[k] - j0;
           if (li.idx[k] >= 0 && at >= 0 && at < j1 - j0) {
             // (in Accumulate mode the old value is there already, unless it is added when the element is copied out)
             const int i = at / VEC;
-            distill_put<T>(sx + at, (float)(ga * (double)li.x[k] - wc * li.p[k]), beta && same && i >= ilo && i < ihi);
+            distill_put<T>(sx + at, mass != 0. ? (float)(ga * (double)li.x[k] - wc * li.p[k]) : 0.f, beta && same && i >= ilo && i < ihi);
           }
         }
         __syncwarp();
@@ -702,11 +702,12 @@ distill_kernel(T* __restrict__ dL, const T* __restrict__ L, const __grid_constan
             }
           }
         } else {
+          // a factor of 0 (no probability on the list and none beside it): 0 also where the logits are no numbers
           for (int i = t; i < n; i += MT) {
             float x[VEC];
             unpack<T>(srow[i], x);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) x[e] = distill_exp(x[e], empty ? all.ref : own, c) * g;
+            for (int e = 0; e < VEC; ++e) x[e] = g != 0.f ? distill_exp(x[e], empty ? all.ref : own, c) * g : 0.f;
             if (beta && same && i >= ilo && i < ihi) srow[i] = pack_accumulate<T>(x, ld_stream(dpart + i * VEC));
             else srow[i] = pack<T>(x);
           }

@@ -284,6 +284,29 @@ def test_masked_and_extreme_rows(cuda, dtype, tail, vocab):
             assert per_row[i] == ref[0][i]
 
 
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("vocab", [64, 5003, 50001, 200000])
+def test_rows_without_a_list_are_zero_whatever_their_logits(cuda, dtype, vocab):
+    """No used slot, or used slots that all hold -inf: loss 0, gradient 0, also where the student's logits are no numbers."""
+    dt, k, rows = DT[dtype], 12, 9
+    x = _logits(rows, vocab, dt, 1)
+    x[1], x[2, 3], x[3, vocab - 1], x[4], x[5, ::2] = math.nan, math.inf, math.nan, -math.inf, math.inf
+    tv, ti, lse = ops.logits_topk(_logits(rows, vocab, torch.float32, 2), k)
+    ti[:5] = -1
+    tv[5:7] = -math.inf
+    ti[7, 1:], ti[7, 0] = -1, vocab                                     # the only slot used is outside the vocabulary
+    empty, w = list(range(7)), torch.linspace(1, 3, rows, device="cuda")
+    keep = _logits(rows, vocab, dt, 3)
+    for ls, zero in ((None, empty), (lse, empty[:5])):                  # with the teacher's sum rows 5, 6 put everything on the rest
+        loss, per_row, grad, status = ops.distill_topk_fwd_bwd(x, tv, ti, ls, w=w)
+        assert not per_row[zero].any() and not grad[zero].any()
+        assert per_row[7].isnan() and not grad[7].any() and int(status) == capi.ERR_INDEX_RANGE and loss.isnan()
+        alone = ops.distill_topk_fwd_bwd(x[8:].contiguous(), tv[8:].contiguous(), ti[8:].contiguous(), None if ls is None else ls[8:], w=w[8:].contiguous())
+        assert per_row[8] > 0 and torch.equal(per_row[8:], alone[1])
+        acc = ops.distill_topk_fwd_bwd(x, tv, ti, ls, w=w, dlogits=keep.clone(), beta=1)[2]
+        assert torch.equal(acc[zero + [7]], keep[zero + [7]]) and not torch.equal(acc[8], keep[8])
+
+
 @pytest.mark.parametrize("tau,vocab,k,noise", [(1.5, 50001, 17, 0.05), (4.0, 32000, 64, 0.05), (1.0, 8000, 128, 0.2), (2.0, 131072, 100, 0.02)])
 def test_a_student_near_its_teacher(cuda, tau, vocab, k, noise):
     """Loss and gradient are then small differences of large terms.  What does not cancel: the error of the sum over the unlisted
