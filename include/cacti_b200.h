@@ -240,8 +240,9 @@ int cacti_b200_logits_topk(cacti_b200_dptr values, cacti_b200_dptr indices, cact
  * w, loss_sum, loss_rows, dlogits (0: forward only), beta_dlogits, status and workspace as in
  * cacti_b200_softmax_nll_fwd_bwd; workspace_bytes from the query below.
  *   t_values [rows, k] of t_dtype (R_32F, R_16F or R_16BF, independent of dtype), t_indices [rows, k] of R_32I or R_16U.
- * Index -1 (R_16U: 65535, where that is no index) marks an unused slot, anywhere in a list; a row without used slots (or
- * whose used logits are all -inf) has loss 0 and gradient 0.  Any other index outside [0, vocab), and an index listed
+ * Index -1 (R_16U: 65535, where that is no index) marks an unused slot, anywhere in a list; a row without used slots has
+ * loss 0 and gradient 0, whatever its logits.  Where all used logits are -inf the same holds with t_lse = 0 (the list has no
+ * mass); with t_lse given all of the teacher's mass is then beside the list: r = 1, loss_i = -log Q.  Any other index outside [0, vocab), and an index listed
  * twice (every slot but the first), writes CACTI_B200_ERR_INDEX_RANGE to *status; the slot is left out and the row's loss
  * is NaN.  A row of weight 0 is not read: loss 0, gradient 0 (beta 1: dlogits unchanged).
  * The teacher's probabilities, the listed exponentials, the row's sums and the loss are kept in f64; the exponentials of unlisted

@@ -307,6 +307,25 @@ def test_rows_without_a_list_are_zero_whatever_their_logits(cuda, dtype, vocab):
         assert torch.equal(acc[zero + [7]], keep[zero + [7]]) and not torch.equal(acc[8], keep[8])
 
 
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("vocab", [40, 5003, 50001])
+def test_a_list_without_mass_leaves_it_all_beside_the_list(cuda, dtype, vocab):
+    """Used slots that all hold -inf: nothing to learn when the list is renormalised, the loss -log Q with the teacher's sum."""
+    dt, k = DT[dtype], 9
+    x = _logits(4, vocab, dt, 1)
+    _, ti, lse = ops.logits_topk(_logits(4, vocab, torch.float32, 2), k)
+    tv = torch.full((4, k), -math.inf, device="cuda")
+    w = torch.ones(4, device="cuda")
+    total, per_row, grad, _ = ops.distill_topk_fwd_bwd(x, tv, ti, None, w=w)
+    assert not per_row.any() and not grad.any() and float(total) == 0.0
+    got = ops.distill_topk_fwd_bwd(x, tv, ti, lse, w=w)
+    ref = _ref(x, tv, ti, lse, 1.0, w)
+    logq = torch.log_softmax(x.double(), 1)
+    rest = torch.logsumexp(logq.scatter(1, ti.long(), -math.inf), 1)
+    assert torch.allclose(ref[0], -rest, rtol=1e-12, atol=1e-12)
+    _check(got[:3], ref, dt, vocab)
+
+
 @pytest.mark.parametrize("tau,vocab,k,noise", [(1.5, 50001, 17, 0.05), (4.0, 32000, 64, 0.05), (1.0, 8000, 128, 0.2), (2.0, 131072, 100, 0.02)])
 def test_a_student_near_its_teacher(cuda, tau, vocab, k, noise):
     """Loss and gradient are then small differences of large terms.  What does not cancel: the error of the sum over the unlisted
