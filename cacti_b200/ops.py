@@ -421,7 +421,7 @@ def gated_ffn_fwd(x, w_gate, w_up, save=False, h=None, gate=None, up=None, works
     tokens, d, f = _ffn_shapes(what, x, w_gate)
     dev, dt = x.device, (x.dtype,)
     _same(what, dev, x=(x, None, _HALF), w_gate=(w_gate, (f, d), dt), w_up=(w_up, (f, d), dt), h=(h, (tokens, f), dt),
-          gate=(gate, (tokens, f), dt), up=(up, (tokens, f), dt))
+          gate=(gate, (tokens, f), dt), up=(up, (tokens, f), dt), workspace=(workspace, None, (torch.uint8,)))
     with _on(dev):
         h = torch.empty(tokens, f, dtype=x.dtype, device=dev) if h is None else h
         if save or gate is not None or up is not None:
@@ -443,7 +443,7 @@ def gated_ffn_bwd(dh, x, w_gate, w_up, gate, up, dx=None, dw_gate=None, dw_up=No
     dev, dt = x.device, (x.dtype,)
     _same(what, dev, x=(x, None, _HALF), dh=(dh, (tokens, f), dt), w_gate=(w_gate, (f, d), dt), w_up=(w_up, (f, d), dt),
           gate=(gate, (tokens, f), dt), up=(up, (tokens, f), dt), dx=(dx, (tokens, d), dt), dw_gate=(dw_gate, (f, d), dt),
-          dw_up=(dw_up, (f, d), dt))
+          dw_up=(dw_up, (f, d), dt), workspace=(workspace, None, (torch.uint8,)))
     if (beta_dx and dx is None) or (beta_dw and (dw_gate is None or dw_up is None)):
         raise ValueError(f"{what}: beta = 1 adds to an output that is not given")
     with _on(dev):

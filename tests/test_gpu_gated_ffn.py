@@ -244,3 +244,20 @@ def test_refusals(cuda):
     small = torch.empty(256, dtype=torch.uint8, device="cuda")
     with pytest.raises(capi.CactiB200Error):
         ops.gated_ffn_bwd(dh, x, wg, wu, gate, up, workspace=small)
+
+
+def test_workspaces_of_another_place_or_type_are_refused(cuda):
+    """A workspace in host memory has an address like any other: the wrapper has to see it before a kernel does."""
+    x, wg, wu, dh = _inputs(4, 17, 24, torch.float16)
+    _, gate, up = ops.gated_ffn_fwd(x, wg, wu, save=True)
+    n = 1 << 20
+    for ws in (torch.empty(n, dtype=torch.uint8), torch.empty(2 * n, dtype=torch.uint8, device="cuda")[::2],
+               torch.empty(n, dtype=torch.float32, device="cuda")):
+        with pytest.raises(ValueError, match="workspace"):
+            ops.gated_ffn_fwd(x, wg, wu, workspace=ws)
+        with pytest.raises(ValueError, match="workspace"):
+            ops.gated_ffn_bwd(dh, x, wg, wu, gate, up, workspace=ws)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    assert torch.equal(ops.gated_ffn_fwd(x, wg, wu, workspace=ws)[0], ops.gated_ffn_fwd(x, wg, wu)[0])
+    for a, b in zip(ops.gated_ffn_bwd(dh, x, wg, wu, gate, up, workspace=ws), ops.gated_ffn_bwd(dh, x, wg, wu, gate, up)):
+        assert torch.equal(a, b)
