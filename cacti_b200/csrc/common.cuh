@@ -19,6 +19,10 @@ inline int check_launch() {
   return CACTI_B200_OK;
 }
 
+// Do two buffers share bytes?  A buffer that is not given (0) shares none.
+struct Span { uint64_t at; uint64_t bytes; };
+inline bool overlap(const Span& a, const Span& b) { return a.at && b.at && a.at < b.at + b.bytes && b.at < a.at + a.bytes; }
+
 inline bool aligned16(uint64_t p) { return (p & 15u) == 0; }
 
 // Ordinal of the current device, for caches of per-device state (function attributes, occupancy, symbol addresses).

@@ -832,6 +832,8 @@ int cacti_b200_distill_topk_fwd_bwd(cacti_b200_dptr loss_sum, cacti_b200_dptr lo
       return CACTI_B200_ERR_WORKSPACE;
     lrows = reinterpret_cast<float*>(workspace);
   }
+  const uint64_t bytes = (uint64_t)rows * vocab * es;
+  if (overlap({dlogits, bytes}, {logits, bytes})) return CACTI_B200_ERR_INVALID_VALUE;
   DistillParams p;
   p.t_values = reinterpret_cast<const void*>(t_values); p.t_indices = reinterpret_cast<const void*>(t_indices);
   p.t_lse = reinterpret_cast<const float*>(t_lse); p.w_rows = reinterpret_cast<const float*>(w_rows);

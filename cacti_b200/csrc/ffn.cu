@@ -382,6 +382,15 @@ static int ffn_operands(Operand (&o)[3], const uint64_t (&ptr)[3], const int64_t
   return check_launch();
 }
 
+// No output shares bytes with an input or with another output.
+template <int NO, int NI> static bool ffn_separate(const Span (&out)[NO], const Span (&in)[NI]) {
+  for (int o = 0; o < NO; ++o) {
+    for (int i = 0; i < NI; ++i) if (overlap(out[o], in[i])) return false;
+    for (int i = 0; i < o; ++i) if (overlap(out[o], out[i])) return false;
+  }
+  return true;
+}
+
 // Sizes whose tile, k-block and vector counts fit 32-bit indices, one operand at a time.
 static bool ffn_sizes_ok(int64_t tokens, int64_t D, int64_t F) {
   constexpr int64_t kMax = 1 << 24, kElems = 1LL << 34;
@@ -826,6 +835,9 @@ static int ffn_bwd_run(uint64_t dx, uint64_t dwg, uint64_t dwu, uint64_t dh, uin
     if (!ffn_rows_aligned(ptr, D)) off += packed_bytes(rows, D, 1);
   }
   if (ws_bytes < off) return CACTI_B200_ERR_WORKSPACE;
+  const uint64_t tok = 2ull * tokens * D, act = 2ull * tokens * F, wts = 2ull * F * D;
+  if (!ffn_separate({{dx, tok}, {dwg, wts}, {dwu, wts}}, {{dh, act}, {x, tok}, {wg, wts}, {wu, wts}, {gate, act}, {up, act}}))
+    return CACTI_B200_ERR_INVALID_VALUE;
   off = 256 + 2 * b.dpart + b.part;
   const unsigned vpr = (unsigned)(b.Fp / 8), nvec = (unsigned)(tokens * vpr);
   const unsigned want = (nvec + 255) / 256, cap = kNumSMs * 32;
@@ -897,6 +909,9 @@ int cacti_b200_gated_ffn_fwd(cacti_b200_dptr h, cacti_b200_dptr gate, cacti_b200
   if (!h || !x || !w_gate || !w_up || !gate != !up) return CACTI_B200_ERR_INVALID_VALUE;
   if ((h | gate | up | x | w_gate | w_up) & 1) return CACTI_B200_ERR_INVALID_VALUE;
   if (!ffn_pack_ok({x, w_gate, w_up}, {tokens, d_ffn, d_ffn}, d_model)) return CACTI_B200_ERR_SHAPE;
+  const uint64_t act = 2ull * tokens * d_ffn, wts = 2ull * d_ffn * d_model;
+  if (!ffn_separate({{h, act}, {gate, act}, {up, act}}, {{x, 2ull * tokens * d_model}, {w_gate, wts}, {w_up, wts}}))
+    return CACTI_B200_ERR_INVALID_VALUE;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (dtype == CACTI_B200_R_16F)
     return ffn_fwd_run<__half>(h, gate, up, x, w_gate, w_up, tokens, d_model, d_ffn, workspace, workspace_bytes, st);

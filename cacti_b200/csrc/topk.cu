@@ -376,6 +376,9 @@ int cacti_b200_logits_topk(cacti_b200_dptr values, cacti_b200_dptr indices, cact
   if (rows == 0) return CACTI_B200_OK;
   const int es = dtype == CACTI_B200_R_32F ? 4 : 2;
   if (!values || !indices || !logits || values % es || logits % es || (indices & 3) || (lse & 3)) return CACTI_B200_ERR_INVALID_VALUE;
+  const Span in{logits, (uint64_t)rows * vocab * es};
+  for (const Span& out : {Span{values, (uint64_t)rows * k * es}, Span{indices, (uint64_t)rows * k * 4}, Span{lse, (uint64_t)rows * 4}})
+    if (overlap(out, in)) return CACTI_B200_ERR_INVALID_VALUE;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return dispatch_dtype(dtype, [&](auto tag) -> int {
     return launch_topk<decltype(tag)>(values, indices, lse, logits, rows, vocab, k, 1.0 / (double)temperature, st);

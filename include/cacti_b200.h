@@ -228,7 +228,8 @@ int cacti_b200_softmax_nll_fwd_bwd(cacti_b200_dptr loss_sum, cacti_b200_dptr los
  * logits_topk is the teacher's side: the k largest logits of each row, largest first, equal values (+0 equals -0) by
  * ascending index, NaN above +inf, as values [rows, k] of dtype and indices [rows, k] int32; lse (optional, f32[rows]) is
  * log sum_j exp(x_j / temperature) over the whole row: -inf for a row of -inf, NaN for a row that holds a NaN.
- * 1 <= k <= 256, k <= vocab <= 262144 (else CACTI_B200_ERR_SHAPE), temperature in [1e-4, 1e4]. */
+ * 1 <= k <= 256, k <= vocab <= 262144 (else CACTI_B200_ERR_SHAPE), temperature in [1e-4, 1e4].  Outputs must not overlap
+ * logits (CACTI_B200_ERR_INVALID_VALUE). */
 int cacti_b200_logits_topk(cacti_b200_dptr values, cacti_b200_dptr indices, cacti_b200_dptr lse, cacti_b200_dptr logits,
                            int64_t rows, int64_t vocab, int64_t k, float temperature, int dtype, cacti_b200_stream stream);
 /* The student's side: with c = 1 / temperature, q = softmax(c x) over the row, and a list of k (index t, teacher logit z):
@@ -249,7 +250,7 @@ int cacti_b200_logits_topk(cacti_b200_dptr values, cacti_b200_dptr indices, cact
  * positions are f32, and so are their sums up to 32 threads' (f64 from there on).  Results are the same in every
  * run and do not depend on what the other rows hold.
  * 1 <= k <= 256, vocab <= 262144 (else CACTI_B200_ERR_SHAPE), temperature in [1e-4, 1e4].  dlogits must not overlap
- * logits. */
+ * logits (CACTI_B200_ERR_INVALID_VALUE).  rows = 0 and vocab = 0 are legal and, as in K5, write nothing. */
 size_t cacti_b200_distill_topk_workspace_bytes(int64_t rows);
 int cacti_b200_distill_topk_fwd_bwd(cacti_b200_dptr loss_sum, cacti_b200_dptr loss_rows, cacti_b200_dptr dlogits,
                                     cacti_b200_dptr logits, cacti_b200_dptr t_values, int t_dtype, cacti_b200_dptr t_indices,
@@ -372,7 +373,7 @@ int cacti_b200_gemm_strided_batched_tri(cacti_b200_dptr c, cacti_b200_dptr a, ca
  * (sums in f32, one rounding; the old value is added in f32 before it, as in cacti_b200_gemm).  tokens = 0 is legal: the
  * adjoint then writes zero weight gradients (beta_dw = 0).  d_model = 0 or d_ffn = 0 is CACTI_B200_ERR_SHAPE.
  * So are sizes above 2^24, operands of 2^34 elements, and operands to be repacked whose copies come to 64 GiB together.
- * Outputs may not overlap inputs or one another.  Workspaces: 256-byte aligned, one for each call at work at a time; `aligned` = 1 asks for what suffices when
+ * Outputs may not overlap inputs or one another (CACTI_B200_ERR_INVALID_VALUE).  Workspaces: 256-byte aligned, one for each call at work at a time; `aligned` = 1 asks for what suffices when
  * d_model is a multiple of 8 and x, w_gate and w_up are 16-byte aligned (operands that are not are repacked), 0 for any. */
 size_t cacti_b200_gated_ffn_fwd_workspace_bytes(int64_t tokens, int64_t d_model, int64_t d_ffn, int aligned);
 int cacti_b200_gated_ffn_fwd(cacti_b200_dptr h, cacti_b200_dptr gate, cacti_b200_dptr up, cacti_b200_dptr x,

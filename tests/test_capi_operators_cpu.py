@@ -77,5 +77,35 @@ def test_gated_ffn_refuses_copies_that_cannot_be_numbered():
         assert _fwd(t=2, d=d, f=f, x=P + off, wg=P + off, wu=P + off, ws=0x1000, wsb=big) == capi.ERR_SHAPE
         assert _bwd(t=2, d=d, f=f, x=P + off, wg=P + off, wu=P + off, wsb=big) == capi.ERR_SHAPE
     assert _fwd(t=2, d=1025, f=16700000, ws=0x1000, wsb=big) == _bwd(t=2, d=1025, f=16700000, wsb=big) == capi.ERR_SHAPE
-    assert _fwd(t=2, d=1017, f=f // 2, ws=0, wsb=0) == _bwd(t=2, d=1017, f=f // 2, ws=0, wsb=0) == capi.ERR_WORKSPACE
-    assert _fwd(t=2, d=1016, f=f, x=P + 2, ws=0, wsb=0) == _bwd(t=2, d=1016, f=f, x=P + 2, ws=0, wsb=0) == capi.ERR_WORKSPACE   # x alone
+    far = 1 << 50                                                       # the forward's output apart from its inputs
+    assert _fwd(h=far, t=2, d=1017, f=f // 2, ws=0, wsb=0) == _bwd(t=2, d=1017, f=f // 2, ws=0, wsb=0) == capi.ERR_WORKSPACE
+    assert _fwd(h=far, t=2, d=1016, f=f, x=P + 2, ws=0, wsb=0) == _bwd(t=2, d=1016, f=f, x=P + 2, ws=0, wsb=0) == capi.ERR_WORKSPACE   # x alone
+
+
+def test_outputs_that_share_bytes_with_inputs_are_refused():
+    """Also by one element, at either end; buffers that touch are apart (those calls are not made here: they would launch)."""
+    A = [(i + 1) << 40 for i in range(9)]                               # addresses of buffers far apart
+    n = 4 * 100 * 2                                                     # logits of 4 x 100, 16 bit
+    for at in (A[0], A[0] + 2, A[0] - 2, A[0] + n - 2, A[0] - n + 2):
+        assert _distill(logits=A[0], dlogits=at, loss_sum=A[1], loss_rows=A[2], tv=A[3], ti=A[4]) == capi.ERR_INVALID_VALUE
+    k = 10
+    for at in (A[0], A[0] + n - 2, A[0] - 4 * k * 2 + 2):
+        assert _topk(logits=A[0], values=at, indices=A[1], lse=A[2]) == capi.ERR_INVALID_VALUE
+    for at in (A[0], A[0] + n - 4, A[0] - 4 * k * 4 + 4):
+        assert _topk(logits=A[0], values=A[1], indices=at, lse=A[2]) == capi.ERR_INVALID_VALUE
+    assert _topk(logits=A[0], values=A[1], indices=A[2], lse=A[0] + 4) == _topk(logits=A[0], values=A[1], indices=A[2], lse=A[0] - 12) == capi.ERR_INVALID_VALUE
+    t, d, f = 4, 16, 24
+    fwd = dict(h=A[0], gate=A[1], up=A[2], x=A[3], wg=A[4], wu=A[5])
+    size = dict(h=t * f, gate=t * f, up=t * f, x=t * d, wg=f * d, wu=f * d)
+    for o in ("h", "gate", "up"):
+        for other in fwd:
+            if other != o:
+                for at in (fwd[other], fwd[other] + 2 * size[other] - 2, fwd[other] - 2 * size[o] + 2):
+                    assert _fwd(**{**fwd, o: at}, t=t, d=d, f=f) == capi.ERR_INVALID_VALUE, (o, other)
+    bwd = dict(dx=A[0], dwg=A[1], dwu=A[2], dh=A[3], x=A[4], wg=A[5], wu=A[6], gate=A[7], up=A[8])
+    size = dict(dx=t * d, dwg=f * d, dwu=f * d, dh=t * f, x=t * d, wg=f * d, wu=f * d, gate=t * f, up=t * f)
+    for o in ("dx", "dwg", "dwu"):
+        for other in bwd:
+            if other != o:
+                for at in (bwd[other], bwd[other] + 2 * size[other] - 2, bwd[other] - 2 * size[o] + 2):
+                    assert _bwd(**{**bwd, o: at}, t=t, d=d, f=f) == capi.ERR_INVALID_VALUE, (o, other)
