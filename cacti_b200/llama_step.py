@@ -263,8 +263,12 @@ class TrainStep:
             soft, _, dlogits, _ = ops.distill_topk_fwd_bwd(logits, teacher.values, teacher.indices, teacher.lse, teacher.temperature,
                                                             w_scalar=teacher.weight / self.loss_tokens, want_rows=False,
                                                             dlogits=dlogits, beta=int(dlogits is not None), status=self.status)
-            loss = soft if loss is None else ops.add(loss, soft)
             self.launches += 2
+            if loss is None:
+                loss = soft
+            else:
+                loss = ops.add(loss, soft)
+                self.launches += 1
         return loss, dlogits
 
     def forward_backward(self, tokens, targets, grads, on_layer_done=None, teacher: Teacher | None = None):

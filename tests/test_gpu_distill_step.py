@@ -80,6 +80,18 @@ def test_student_step_against_a_teacher(cuda, weight):
     assert abs(float(loss)) < 2.0 ** -19
 
 
+def test_launches_of_the_losses_are_counted(cuda):
+    """Two kernels a loss (rows, sum), one more that adds a mixed step's two sums."""
+    P, tok, tgt = _params(cuda, 1), _tokens(3), _tokens(4)
+    step, grads = LS.TrainStep(CFG, P, B), LS.zeros_like_params(P)
+    counts = []
+    for weight in (None, 1.0, 0.5):
+        teacher = None if weight is None else LS.TrainStep(CFG, P, B).teacher_topk(tok, 16, weight=weight)
+        step.forward_backward(tok, tgt, grads, teacher=teacher)
+        counts.append(step.launches)
+    assert counts[1] == counts[0] and counts[2] == counts[0] + 3
+
+
 def test_captured_student_step(cuda):
     P = _params(cuda, 1)
     toks, tgts = [_tokens(3), _tokens(5)], [_tokens(4), _tokens(6)]
