@@ -420,6 +420,62 @@ def test_streams_graphs_and_empty_calls(cuda):
     assert capi.lib().cacti_b200_device_error(capi.C.byref(err)) == capi.OK and err.value == 0
 
 
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("rows,vocab,k", [(4, 1030, 100), (4, 1500, 128), (148, 1999, 128), (2, 2050, 256), (4, 3000, 256), (3, 4090, 256)])
+def test_topk_of_few_rows_with_fewer_groups_than_k(cuda, dtype, rows, vocab, k):
+    """Few rows of 16-bit logits are read by 1024 threads; below 16 k words fewer than k of the groups that bound the k-th largest hold
+    any, and the exact search decides."""
+    x = _logits(rows, vocab, DT[dtype], vocab)
+    x[0, ::3] = -math.inf
+    for off in (0, 1):
+        xv, _ = _at_offset(x, off)
+        v, i, lse = ops.logits_topk(xv, k)
+        sv, si = torch.sort(x.float(), dim=1, descending=True, stable=True)
+        assert torch.equal(i.long(), si[:, :k]) and torch.equal(v.float(), sv[:, :k])
+        ref = torch.logsumexp(x.double(), 1)
+        assert ((lse.double() - ref).abs() <= 2.0 ** -23 * ref.abs() + (vocab / 256 + 24) * 2.0 ** -24 + 2.0 ** -22 * 20).all()
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("rows,vocab", [(70, 150001), (41, 200000)])
+def test_long_f32_rows_one_after_another_in_a_cluster(cuda, tail, rows, vocab):
+    """f32 rows above about 135000 words: parts that are not held in registers and have one slot, several rows to a cluster (a device
+    runs at most 18 clusters of eight blocks)."""
+    k, tau = 33, 1.3
+    x, z = _logits(rows, vocab, torch.float32, 1), _logits(rows, vocab, torch.float32, 2)
+    tv, ti, lse = ops.logits_topk(z, k, temperature=tau)
+    ti[::4, 5:] = -1
+    ti[1] = -1
+    lse = lse if tail else None
+    w = torch.linspace(0.5, 3.0, rows, device="cuda")
+    w[3::5] = 0.0
+    ref = _ref(x, tv, ti, lse, tau, w)
+    got = ops.distill_topk_fwd_bwd(x, tv, ti, lse, tau, w)
+    _check(got[:3], ref, torch.float32, vocab)
+    old = _logits(rows, vocab, torch.float32, 5, std=1.0)
+    acc = ops.distill_topk_fwd_bwd(x, tv, ti, lse, tau, w, dlogits=old.clone(), beta=1)[2]
+    _check((None, None, acc), ref, torch.float32, vocab, old=old, what="beta 1")
+    fwd = ops.distill_topk_fwd_bwd(x, tv, ti, lse, tau, w, want_grad=False)
+    assert torch.equal(fwd[1], got[1]) and int(got[3]) == 0
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("part", [256, 700])
+def test_shorter_parts_of_a_row(cuda, dtype, part):
+    """The tuning knob: rows shared by more blocks than they need, same results within the same bounds."""
+    dt, rows, vocab, k = DT[dtype], 40, 9001, 20
+    x, z = _logits(rows, vocab, dt, 1), _logits(rows, vocab, torch.float32, 2)
+    tv, ti, lse = ops.logits_topk(z, k)
+    w = torch.ones(rows, device="cuda")
+    L = capi.lib()
+    try:
+        assert L.cacti_b200_tune(b"distill_part", part) == capi.OK
+        got = ops.distill_topk_fwd_bwd(x, tv, ti, lse, w=w)
+    finally:
+        assert L.cacti_b200_tune(b"distill_part", 4096) == capi.OK
+    _check(got[:3], _ref(x, tv, ti, lse, 1.0, w), dt, vocab)
+
+
 def test_more_lengths_of_rows_than_a_launch_cache_keeps(cuda):
     """Two hundred sizes of shared memory for one kernel, and for its cluster form, then the first ones again."""
     x, z = (_logits(1, 42000 + 16 * 200, torch.float16, s) for s in (1, 2))

@@ -127,6 +127,23 @@ def test_both_directions_at_larger_sizes(cuda, dtype, t, d, f):
 
 
 @pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("t,d,f", [(256, 256, 128), (513, 264, 184), (2048, 2560, 2048)])
+def test_everything_added_through_the_tma_epilogue(cuda, dtype, t, d, f):
+    """Aligned results and a contraction of dx that is not cut: old values of all three arrive by TMA."""
+    x, wg, wu, dh = _inputs(t, d, f, DT[dtype], 8)
+    _, gate, up = ops.gated_ffn_fwd(x, wg, wu, save=True)
+    want = ops.gated_ffn_bwd(dh, x, wg, wu, gate, up)
+    zeros = ops.gated_ffn_bwd(dh, x, wg, wu, gate, up, *(torch.zeros_like(o) for o in want), beta_dx=1, beta_dw=1)
+    assert all(torch.equal(a, b) for a, b in zip(zeros, want))
+    g = torch.Generator(device="cuda").manual_seed(9)
+    old = [torch.randn(o.shape, device="cuda", generator=g).to(x.dtype) for o in want]
+    acc = ops.gated_ffn_bwd(dh, x, wg, wu, gate, up, *(o.clone() for o in old), beta_dx=1, beta_dw=1)
+    _check_bwd(acc, dh, x, wg, wu, gate, up, old, "added")
+    only = ops.gated_ffn_bwd(dh, x, wg, wu, gate, up, dx=old[0].clone(), beta_dx=1)
+    assert torch.equal(only[0], acc[0]) and torch.equal(only[1], want[1]) and torch.equal(only[2], want[2])
+
+
+@pytest.mark.parametrize("dtype", list(DT))
 @pytest.mark.parametrize("t,d,f,dx_off", [(16, 3200, 8640, 0), (77, 1024, 2048, 0), (300, 640, 8640, 1)])
 def test_partial_sums_and_accumulating_tiles_in_one_staging(cuda, dtype, t, d, f, dx_off):
     """Few tokens cut dx's contraction (and a dx at an odd address cannot leave by TMA): its tiles leave the staging by ordinary
