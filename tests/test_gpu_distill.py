@@ -326,6 +326,30 @@ def test_a_list_without_mass_leaves_it_all_beside_the_list(cuda, dtype, vocab):
     _check(got[:3], ref, dt, vocab)
 
 
+def test_exponentials_and_logarithms_of_the_list(cuda):
+    """Two words, both listed: the loss is then made of the list's own exponentials and logarithms alone.  The exponentials are good to
+    3e-10 (the series' next term over its smallest value), a logarithm passes that on: two sums and their two logarithms, 1.2e-9; the
+    probabilities' 3e-10 multiplies log p - log q; c is rounded to f32, 2^-24 of the student's exponents, which acts on the
+    difference of the distributions; one rounding to f32."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    n = 4000
+    a = (torch.rand(n, device="cuda", generator=g) * 12 - 5).exp()                           # 0.007 to 1100
+    b = a * (1 + torch.randn(n, device="cuda", generator=g) * torch.logspace(-6, -0.5, n, device="cuda"))
+    shift = torch.randn(n, 1, device="cuda", generator=g) * 30
+    x = torch.stack([torch.zeros_like(a), -a], 1) + shift
+    z = torch.stack([torch.zeros_like(b), -b], 1)
+    ti = torch.tensor([[0, 1]], dtype=torch.int32, device="cuda").repeat(n, 1)
+    w = torch.ones(n, device="cuda")
+    _, rows, _, status = ops.distill_topk_fwd_bwd(x, z, ti, w=w)
+    loss = _ref(x, z, ti, None, 1.0, w)[0]
+    lp, lq = torch.log_softmax(z.double(), 1), torch.log_softmax(x.double(), 1)
+    p, q = lp.exp(), lq.exp()
+    A = (x.double() - x.double().amax(1, keepdim=True)).abs().amax(1)
+    tol = 1.2e-9 + 3e-10 * (p * (lp - lq).abs()).sum(1) + 2.0 ** -24 * A * (p - q).abs().sum(1) + 2.0 ** -24 * loss + 2.0 ** -149
+    err = (rows.double() - loss).abs()
+    assert int(status) == 0 and (err <= tol).all(), (err / tol).max()
+
+
 @pytest.mark.parametrize("tau,vocab,k,noise", [(1.5, 50001, 17, 0.05), (4.0, 32000, 64, 0.05), (1.0, 8000, 128, 0.2), (2.0, 131072, 100, 0.02)])
 def test_a_student_near_its_teacher(cuda, tau, vocab, k, noise):
     """Loss and gradient are then small differences of large terms.  What does not cancel: the error of the sum over the unlisted
@@ -527,6 +551,24 @@ def test_two_host_threads_with_rows_of_two_lengths(cuda):
     assert len(got) == 6
     for (_, _, v), out in got.items():
         assert all(torch.equal(a, b) for a, b in zip(out, want[v]))
+
+
+def test_more_elements_than_32_bits_count(cuda):
+    """70000 x 32768 f16: the last rows' results are those of a call on them alone."""
+    rows, vocab, n = 70000, 32768, 9
+    x = torch.empty(rows, vocab, dtype=torch.float16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for i in range(0, rows, 10000):
+        x[i:i + 10000].normal_(generator=g)
+    top = ops.logits_topk(x, 16)
+    assert all(torch.equal(a[-n:], b) for a, b in zip(top[:2], ops.logits_topk(x[-n:], 16)))
+    # (few rows are read by more threads, whose sums have another order: the sum is held to 64 bits, at this file's tolerance)
+    ref = torch.logsumexp(x[-n:].double(), 1)
+    assert ((top[2][-n:].double() - ref).abs() <= 2.0 ** -23 * ref.abs() + (vocab / 256 + 24) * 2.0 ** -24 + 2.0 ** -22 * 20).all()
+    top = [t.roll(1, 0) for t in top]                                   # each row against its neighbour's list
+    _, loss, grad, _ = ops.distill_topk_fwd_bwd(x, *top, w_scalar=100.0)
+    alone = ops.distill_topk_fwd_bwd(x[-n:], *(t[-n:] for t in top), w_scalar=100.0)
+    assert torch.equal(loss[-n:], alone[1]) and torch.equal(grad[-n:], alone[2]) and alone[2].any(1).all()
 
 
 def test_refusals(cuda):

@@ -278,3 +278,19 @@ def test_workspaces_of_another_place_or_type_are_refused(cuda):
     assert torch.equal(ops.gated_ffn_fwd(x, wg, wu, workspace=ws)[0], ops.gated_ffn_fwd(x, wg, wu)[0])
     for a, b in zip(ops.gated_ffn_bwd(dh, x, wg, wu, gate, up, workspace=ws), ops.gated_ffn_bwd(dh, x, wg, wu, gate, up)):
         assert torch.equal(a, b)
+
+
+def test_more_elements_than_32_bits_count(cuda):
+    """270000 tokens x 8192: the last tokens' results are those of a call on them alone; the weight gradients see them."""
+    t, d, f, n = 270000, 64, 8192, 300
+    x, wg, wu, _ = _inputs(1, d, f, torch.float16, 10)
+    g = torch.Generator(device="cuda").manual_seed(11)
+    x = torch.randn(t, d, device="cuda", generator=g).half()
+    h, gate, up = ops.gated_ffn_fwd(x, wg, wu, save=True)
+    few = ops.gated_ffn_fwd(x[-n:], wg, wu, save=True)
+    assert all(torch.equal(a[-n:], b) for a, b in zip((h, gate, up), few))
+    dh = h.zero_()                                                      # only the last tokens have a gradient
+    dh[-n:] = torch.randn(n, f, device="cuda", generator=g).half()
+    dx, dwg, dwu = ops.gated_ffn_bwd(dh, x, wg, wu, gate, up)
+    assert not dx[:-n].any()
+    _check_bwd((dx[-n:], dwg, dwu), dh[-n:], x[-n:], wg, wu, few[1], few[2])
