@@ -15,6 +15,10 @@
 // sweeps, as softmax_nll does it, and lists handled by the same warps took 2.32 ms.  What is left is not bandwidth: a row's phases
 // follow one another (listed logits out of the row, exponentials and sum, gradient, listed positions, copy out), and with one
 // row in work a CTA and two waiting the instruction issue is a third busy.  Shared memory holds no fourth row of 64 KB.
+// Other forms, 8192 x 32000 f16 with a list of 64: forward only 146 us; Accumulate mode 568 us (the old values are loaded where they are
+// needed, nothing ahead).  Where gradient and logits start at different places in a 16-byte vector, a list warp copies the row out by
+// elements: 443 us, 6.6 ms in Accumulate mode.  f32 rows above about 135000 words have one slot and form their exponentials twice:
+// 1024 x 151936 697 us (0.28 of the copy rate), 1024 x 131072 265 us (0.63).
 #include "row_vec.cuh"
 #include <type_traits>
 
@@ -82,9 +86,10 @@ struct DistillRow {              // from the list warp to the main warps
   double px, pown;               // sum of p log2 e(x) and of p over this CTA's listed positions
 };
 // A sum of exponentials under its reference.  Listed and unlisted positions keep references of their own until the end: where
-// the list holds nearly everything, the rest is still known.  f64 from a warp's sum on, and the listed exponentials are exact to 1e-10:
-// near the teacher both the loss and the gradient are small differences, in which the errors of single exponentials average out or
-// are multiplied by a difference, but an error of the whole sum is not.
+// the list holds nearly everything, the rest is still known.  f64 from a warp's sum on, and the listed exponentials are f64 (good to
+// 3e-10 for the c they are given; c itself is f32, the same for listed and unlisted positions: the temperature is off by up to 2^-24
+// relative).  Near the teacher both the loss and the gradient are small differences, in which the errors of single exponentials average
+// out or are multiplied by a difference, but an error of the whole sum is not.
 struct alignas(16) DistillSum { DistillRef ref; double z; };
 struct DistillFin { DistillRef ref; double z_all, z_rest, shift_rest, px; };             // back to the list warp
 struct alignas(16) DistillRec { DistillSum rest, top; double px, pown; };  // a CTA's part of a row, to the cluster
@@ -189,8 +194,8 @@ template <typename T> __device__ __forceinline__ void distill_put(T* o, float v,
 // What a list warp knows of a row.
 struct DistillHead { float w; double psum, ent, r; bool bad; };
 
-// exp(d) to about 1e-10: 2^n times the Taylor series of exp(f ln2), |f| <= 1/2, to the eighth power (the next term is
-// (ln2 / 2)^9 / 9! = 2e-10).  A third of the latency of the library's, which a single warp does not hide.  The f32 functions
+// exp(d) to 3e-10 relative: 2^n times the Taylor series of exp(f ln2), |f| <= 1/2, to the eighth power (the next term is
+// (ln2 / 2)^9 / 9! = 2e-10, and the series is at least 0.7).  A third of the latency of the library's, which a single warp does not hide.  The f32 functions
 // would do for ordinary rows; where the student gives a listed word a logit of -65504, the loss shows their 1e-7.
 __device__ __forceinline__ double exp_list(double d) {
   const double y = d * 1.4426950408889634;
@@ -209,7 +214,7 @@ __device__ __forceinline__ double exp_list(double d) {
   return s * __hiloint2double(((int)n + 1023) << 20, 0);
 }
 
-// ln z to about 1e-12: the f32 logarithm and one Newton step on exp.
+// ln z to 3e-10 absolute: the f32 logarithm and one Newton step on exp_list, whose error passes on.
 __device__ __forceinline__ double log_list(double z) {
   const float y = logf((float)z);
   if (!(fabsf(y) < 80.f)) return log(z);                        // 0, infinities, NaN, the ends of f32's range

@@ -17,12 +17,14 @@
 // Calls may overlap on any streams and graphs: the forward's tile walk is static, the backward's draws its items from a
 // counter in the call's own workspace.  The backward's items differ in length (2 F and T deep), and their contractions are so long
 // that workers on a static walk drift apart and no longer share operand panels in L2: at 16384 x 3200 x 8640, sustained, the
-// static walk took 3.58 ms. against 2.94 ms.
+// static walk took 3.58 ms against 2.94 ms.
 //
 // Bound: the tensor cores, 4 T D F operations forward and 8 T D F backward, at the measured
-// cuBLAS rate (1.67 PFLOP/s burst, 1.40 sustained under the power cap).  16384 x 3200 x 8640 f16: forward 1.29 to 1.35 ms in a loop without
-// the projections kept (1.34 to 1.40 PFLOP/s, 0.96 to 1.0 of the sustained rate), 1.36 to 1.44 ms with them (0.57 GB more written);
-// backward 2.92 to 2.97 ms, of which the adjoint pass (1.4 GB, 215 us) and the products at 1.32 PFLOP/s.  2048 tokens: backward 381 us.
+// cuBLAS rate (1.67 PFLOP/s burst, 1.40 sustained under the power cap).  16384 x 3200 x 8640 f16 in a loop at the power cap, which differs
+// from card to card: forward 1.29 to 1.43 ms without the projections kept (1.27 to 1.40 PFLOP/s), 1.36 to 1.52 ms with them (0.57 GB more
+// written); backward 2.92 to 3.38 ms (1.07 to 1.24 PFLOP/s), of which the adjoint pass is 1.4 GB and 215 us.  2048 tokens: 381 to 418 us.
+// The separate operators (matmuls and swiglu) in the same run and graphs: 16384 tokens 1645 us forward (this file 1505) and 3446 us
+// backward (3364); 2048 tokens 224 (196) and 488 (409); 333 tokens 62 (55) and 171 (125).
 // Tensor pipes are active 87 percent of the cycles forward and 85 percent backward at 2048 tokens.
 #include "gemm_common.cuh"
 #include <utility>
@@ -31,8 +33,9 @@ namespace cb {
 
 struct FfnMaps { CUtensorMap a[2], b[3], c[3], ak[2]; };
 
-// silu's sigmoid, f32 with the fast exponential and division: relative error below 2^-20 for |g| < 30, far below the 16-bit
-// rounding that follows; g = -inf gives s = 0.
+// silu's sigmoid, f32 with the fast exponential and division.  By their documented bounds its relative error is at most
+// (5 + 1.2 |g|) 2^-23 for negative g (2^-20 at -3, 2^-17.6 at -30) and 2^-20 for positive g: far below the 16-bit rounding that
+// follows.  g = -inf gives s = 0.
 __device__ __forceinline__ float sigmoid_f32(float g) { return __fdividef(1.f, 1.f + __expf(-g)); }
 
 // ---- forward ------------------------------------------------------------------------------------------------------

@@ -10,6 +10,10 @@
 //           one warp finds it, or a value just below it, by bisection on counts.
 //   pass 2: vectors with a position at or above t are put aside, then these positions, hardly more than K for ordinary rows, are
 //           collected and ranked by counting.
+// The exponentials are taken against 1; a row whose sum then leaves 2^-60 .. 2^60 (all logits beyond about 41 temperatures from 0) is swept
+// once more for its sum: 8192 x 32000 f16 182 us around 0, 252 us around -60.
+// Fewer than K groups that hold anything (16-bit rows of fewer than 16 K words read by 1024 threads): the bound is -inf, and the exact
+// search below runs on ordinary rows too: 4 x 3000 with K = 256 61 us, with K = 64 12 us.
 // More than kTopkCap of them: with many equal to t (few distinct values, masks) only those above t are collected, and the first
 // positions equal to t fill the rest in index order.  More than kTopkCap above t (values arranged against the kernel's order): the
 // exact K-th largest is found by bisection over the whole row, and at most K - 1 lie above that.  Nothing depends on the order in
